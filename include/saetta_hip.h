@@ -525,6 +525,143 @@ int saetta_attn_gemm(saetta_stream_t stream, int bits, const uint16_t *q_f16, sa
                      saetta_flash_params p, uint32_t slice_tokens, uint32_t stages, void *workspace,
                      size_t workspace_bytes);
 
+/* ---- a cache in blocks that several requests share --------------------------- */
+
+/* The reference serves one sequence over a cache that is a plain row array (src/gpu_layers.rs:183-293); these entry
+ * points have no counterpart in it.  They serve several requests (conversations) at once: their keys and values lie
+ * in blocks of 16, 32, 64 or 128 tokens, which the requests' rows of a block table name in order.  A step is
+ *     saetta_paged_tables    blocks for the new tokens, their slots and positions, from the requests' lengths
+ *     saetta_paged_split     which workgroup takes which keys, once for all layers
+ *     per layer: saetta_paged_store (the new keys and values), saetta_paged_attn
+ * All lengths, tables and slots lie in device memory and are read when the kernels run, so a recorded step (a plan, a
+ * HIP graph) serves every state of the requests.  A number out of range in them (a block that does not exist, a length
+ * past a row of the table) never leads outside the buffers: the tokens that it would name are not stored and not seen.
+ * Heads: head dim 256, 1, 2, 4, 8 or 16 q heads per kv head. */
+enum {
+    SAETTA_F32 = 0,
+    SAETTA_F16 = 1,
+    SAETTA_BF16 = 2
+};
+
+/* The blocks of one layer.  keys, values: [blocks][kv_heads][block_tokens * 256] bytes, 16-byte aligned, OCP e4m3
+ * codes in units of 16 tokens (4096 bytes).  Inside a unit the byte of token t, dim d is, of keys, at
+ *     d / 64 * 1024 + (d / 16 % 4 * 16 + t) * 16 + d % 16,
+ * of values at
+ *     d / 64 * 1024 + (t / 4 * 16 + d % 16) * 16 + d / 16 % 4 * 4 + t % 4:
+ * the order in which the matrix cores take them.  key_scales, value_scales: [blocks][kv_heads], 127 + e: a code stands
+ * for its value times 2^e.  blocks * block_tokens is less than 2^31.  Nothing needs clearing before the first store. */
+typedef struct saetta_paged_cache {
+    uint8_t *keys;
+    uint8_t *values;
+    uint8_t *key_scales;
+    uint8_t *value_scales;
+    uint32_t blocks;
+    uint32_t block_tokens;
+    uint32_t kv_heads;
+} saetta_paged_cache;
+
+/* What the requests hold: row r of block_table [requests][max_blocks] names request r's blocks in order, of which the
+ * first held[r] are its own.  free_list [blocks]: the blocks that nobody holds, the first *free_count of it. */
+typedef struct saetta_paged_state {
+    int32_t *block_table;
+    uint32_t *held;
+    int32_t *free_list;
+    uint32_t *free_count;
+} saetta_paged_state;
+
+/* What a step is given: query_starts [requests + 1], the first new token of each request and the number of all; kv_lens
+ * [requests], the tokens behind which it stands, new ones included; slots, positions [tokens]; unplaced [1]. */
+typedef struct saetta_paged_step {
+    uint32_t *query_starts;
+    uint32_t *kv_lens;
+    int32_t *slots;
+    int32_t *positions;
+    uint32_t *unplaced;
+} saetta_paged_step;
+
+typedef struct saetta_paged_tables_params {
+    uint32_t requests;
+    uint32_t max_blocks;   /* a row of the table */
+    uint32_t block_tokens; /* 16, 32, 64 or 128 */
+    uint32_t blocks;       /* of the cache, and room of free_list */
+    uint32_t tokens;       /* room of slots and positions */
+} saetta_paged_tables_params;
+
+/* A step's tables from context_lens [requests], the tokens a request has in its blocks, and new_lens [requests], those
+ * that come now.  Request r is to hold ceil((context + new) / block_tokens) blocks, at most max_blocks.  Who holds fewer
+ * gets what is missing from the end of the free list (request by request, a request's blocks in the order of the list;
+ * where they do not suffice the later requests go without), who holds more (a finished request has length 0, a
+ * rejected draft is a shorter context) gives the rest back behind those that are left, its entries set to -1.  Token
+ * i of request r is token query_starts[r] + i of the step, at position context_lens[r] + i, in slot
+ * block * block_tokens + position % block_tokens, or -1 where it has no block.  Past the last token slots and positions
+ * are -1.  query_starts are at most p.tokens, and tokens past the room have no place.  *unplaced: the tokens without
+ * a slot.  kv_lens may be context_lens itself: then the call, replayed, goes on by new_lens each time. */
+int saetta_paged_tables(saetta_stream_t stream, const uint32_t *context_lens, const uint32_t *new_lens,
+                        saetta_paged_state state, saetta_paged_step step, saetta_paged_tables_params p);
+
+/* Rows of `heads` rows of 256 values, of a type of the call's: token t's head h begins at data + t * token_stride +
+ * h * head_stride, both in values.  data is 16-byte aligned and the strides are multiples of 16 bytes. */
+typedef struct saetta_strided_rows {
+    void *data;
+    uint64_t token_stride;
+    uint64_t head_stride;
+} saetta_strided_rows;
+
+/* The keys and values of `tokens` tokens into the slots (or nowhere, where the slot is not one of the cache).  A block
+ * and kv head of keys or of values has one e: the least of -40..60 for which the largest finite magnitude in it is at
+ * most 448 * 2^e.  A token in a block's first place begins the block anew; a later one can raise e, and then the codes before it
+ * become what they stand for times 2^(their e - e), rounded to nearest even like the new ones; e falls only when the
+ * block begins anew.  A value that is not finite, or larger than 448 * 2^60, is stored as NaN.  The tokens of one block follow each other
+ * in the call, at rising slots without a gap, as saetta_paged_tables gives them; what a block holds that a call
+ * names by two such runs is undefined. */
+int saetta_paged_store(saetta_stream_t stream, int type, saetta_strided_rows keys, saetta_strided_rows values,
+                       const int32_t *slots, saetta_paged_cache cache, uint32_t tokens);
+
+/* The other way: the keys and values of `tokens` slots, in any order, as contiguous [tokens][kv_heads][256] of the type,
+ * rounded to nearest even.  A row whose slot is not one of the cache is left as it was.  Either of keys and values may
+ * be NULL. */
+int saetta_paged_gather(saetta_stream_t stream, int type, saetta_paged_cache cache, const int32_t *slots, void *keys,
+                        void *values, uint32_t tokens);
+
+/* What the attention of a step reads besides the cache.  block_table and its max_blocks as above. */
+typedef struct saetta_paged_batch {
+    const uint32_t *query_starts;
+    const uint32_t *kv_lens;
+    const int32_t *block_table;
+    uint32_t requests;
+    uint32_t max_blocks;
+    uint32_t block_tokens;
+} saetta_paged_batch;
+
+typedef struct saetta_paged_attn_params {
+    uint32_t heads;
+    uint32_t kv_heads;
+    uint32_t tokens; /* rows of q and out: the room for a step's new tokens */
+    uint32_t rows;   /* the most new tokens that a request has; with up to 16 (tokens * q heads per kv head) a
+                        kernel for few rows runs, with more one for chunks, which takes any mixture */
+    float scale;
+} saetta_paged_attn_params;
+
+/* Bytes of `split` and of `workspace` for calls with these parameters and up to `requests` requests, for the current
+ * device. */
+size_t saetta_paged_split_bytes(saetta_paged_attn_params p, uint32_t requests);
+size_t saetta_paged_workspace_bytes(saetta_paged_attn_params p, uint32_t requests);
+
+/* Deals the step's rows and keys to the workgroups of saetta_paged_attn, from the lengths alone: once a step, for all its layers.
+ * split is 16-byte aligned device memory of saetta_paged_split_bytes, read by the calls after it. */
+int saetta_paged_split(saetta_stream_t stream, saetta_paged_batch batch, saetta_paged_attn_params p, void *split);
+
+/* out = softmax(q K^T scale) V [* sigmoid(gate)] for the new tokens of all requests, whose keys and values are in
+ * the cache already: token i of the n that request r has now sits at position kv_lens[r] - n + i and sees the positions up to its
+ * own.  q, gate and out are f16 or bf16 (type) rows of p.heads heads; gate.data NULL: no gate.  out may be q.  Rows past the step's last token,
+ * and tokens of a request past p.rows where p.rows is for few rows, are left as they were; a row that sees nothing (its position is
+ * below 0, or its blocks are not there) becomes zeros.  split: made by saetta_paged_split with the same batch and p.
+ * workspace: 16-byte aligned, of saetta_paged_workspace_bytes, the call's own until its kernels have run; calls that may
+ * overlap bring different ones. */
+int saetta_paged_attn(saetta_stream_t stream, int type, saetta_strided_rows q, saetta_paged_cache cache,
+                      saetta_paged_batch batch, const void *split, saetta_strided_rows gate, saetta_strided_rows out,
+                      saetta_paged_attn_params p, void *workspace, size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -40,6 +40,9 @@ int setup_deltanet();
 int setup_deltanet_chunk();
 int setup_decode();
 int setup_prefill();
+int setup_paged_tables();
+int setup_paged_cache();
+int setup_paged_attn();
 // The chunked delta rule (deltanet_chunk.hip): the workspace a call needs (0: the call keeps to the
 // token-by-token kernels), and the call itself (the delta rule only; the gated norm follows as for the
 // token-by-token kernels) with a workspace of the caller's.

@@ -1,0 +1,794 @@
+// Attention of a step's new tokens over a cache in blocks that several requests share.
+//
+// For row i of request r, at position p = kv_lens[r] - n + i, and q head h over kv head h / group:
+//     out = sum_t 2^(s_t) v_t / sum_t 2^(s_t) [* sigmoid(gate)],  s_t = log2(e) scale (q . k_t),  t = 0 .. p.
+// The cache holds codes a, b and exponents: k_t = 2^ek a_t, v_t = 2^ev b_t, one ek and ev per block and kv head.  With
+//     x_t = log2(e) scale 2^ek (q . a_t) + ev,   w_t = 2^(x_t - M),   M = max x_t so far,
+// out = sum w_t b_t / sum w_t 2^-ev: the values' scale is an addend of the score, the running maximum is that of what a
+// token can add to the output, and the matrix cores see codes alone, which f16 and bf16 hold exactly.  Only w_t is rounded (to
+// f16, half a step 2^-12 of it, as operand of the second product: the sums are f32).
+//
+// The three kernels: paged_split_kernel deals rows and keys out as items from the lengths; the attention kernel, one
+// workgroup to an item and kv head, paged_few_kernel for tiles of up to 16 rows and paged_chunk_kernel for tiles of
+// 256; paged_merge_kernel where a tile's keys were taken in parts.
+//
+// Both attention kernels compute S^T = K Q^T and O^T += V^T P^T: a lane owns one query row (column), the running
+// maximum and sum are its own, and the probabilities go from the accumulators of the first product into the operand of the
+// second as they lie.  The cache's order of bytes is that of the operands: a load of a wave is one contiguous kilobyte.
+#include "common.hpp"
+#include "lanes.hpp"
+#include "paged_device.hpp"
+
+namespace saetta {
+namespace {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4_ __attribute__((ext_vector_type(4)));
+typedef _Float16 half2_ __attribute__((ext_vector_type(2)));
+typedef __bf16 brain8 __attribute__((ext_vector_type(8)));
+typedef __bf16 brain2 __attribute__((ext_vector_type(2)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int DIM = SAETTA_HEAD_DIM;
+constexpr float NO_SCORE = -1e30f;               // of a key that a row does not see
+constexpr float NO_MAXIMUM = 0.25f * NO_SCORE;   // where nothing was seen: 2^(NO_SCORE - NO_MAXIMUM) is 0
+constexpr float TAU = 8.0f;                      // the reference maximum is raised only past this many powers of two
+constexpr uint32_t STEP_KEYS = 32;               // keys of a step: two units
+constexpr uint32_t FEW_ROWS = 16, CHUNK_ROWS = 256;
+constexpr int FEW_WAVES = 4, CHUNK_WAVES = 8;
+
+// ---- what is dealt out -------------------------------------------------------------------------------------------
+
+// Rows of a request and keys that a workgroup takes.
+struct alignas(16) Item {
+    uint32_t request, row0, tokens;  // rows of q from row0 on
+    int32_t pos0;                    // position of the first of them
+    uint32_t key0, key1;             // keys that are taken (up to what the last row sees)
+    uint32_t part, parts;            // of the tile's keys; parts 0: nothing to do.  The parts of a tile are items side by side
+};
+struct alignas(16) SplitHead {
+    uint32_t items, tiles;  // items dealt out; tiles in parts (their first items, behind the items)
+    uint32_t unused[2];
+};
+
+struct Shape {
+    uint32_t group, tile_tokens, tile_rows;
+    uint32_t target;  // items that fill the device
+    uint32_t most_items, most_tiles;
+};
+Shape shape_of(const saetta_paged_attn_params &p, uint32_t requests) {
+    Shape s;
+    s.group = p.heads / p.kv_heads;
+    const bool few = uint64_t(p.rows) * s.group <= FEW_ROWS;
+    s.tile_rows = few ? FEW_ROWS : CHUNK_ROWS;
+    s.tile_tokens = few ? (p.rows ? p.rows : 1) : CHUNK_ROWS / s.group;
+    const uint32_t workgroups = cu_count() * (few ? 2 : 1);
+    s.target = workgroups / p.kv_heads ? workgroups / p.kv_heads : 1;
+    s.most_tiles = few ? requests : p.tokens / s.tile_tokens + requests;
+    s.most_items = s.most_tiles > s.target ? s.most_tiles : s.target;
+    return s;
+}
+
+struct SplitArgs {
+    saetta_paged_batch batch;
+    SplitHead *head;
+    Item *items;
+    uint32_t *tiles;
+    uint32_t tile_tokens, target, most_items, tokens, rows;
+    uint32_t few, granule;
+};
+
+constexpr int SPLIT_THREADS = 1024, SPLIT_WAVES = SPLIT_THREADS / 64;
+
+__device__ __forceinline__ uint32_t total_of(uint32_t x, uint32_t *waves) {
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) x += __shfl_xor(x, d);
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = x;
+    __syncthreads();
+    uint32_t all = 0;
+#pragma unroll
+    for (int w = 0; w < SPLIT_WAVES; w++) all += waves[w];
+    __syncthreads();
+    return all;
+}
+
+// A request as the split sees it.
+struct Work {
+    uint32_t row0, tokens, tiles, keys;  // keys: what its last row sees, in whole rows of the table
+    int32_t pos0;
+};
+__device__ __forceinline__ Work work_of(const SplitArgs &a, uint32_t r) {
+    Work w = {0, 0, 0, 0, 0};
+    if (r >= a.batch.requests) return w;
+    const uint32_t start = min(a.batch.query_starts[r], a.tokens), end = min(a.batch.query_starts[r + 1], a.tokens);
+    const uint32_t n = end > start ? end - start : 0;
+    const uint32_t length = min(a.batch.kv_lens[r], 0x7fffffffu);
+    w.row0 = start, w.tokens = a.few ? min(n, a.rows) : n;
+    w.pos0 = int32_t(length) - int32_t(n);
+    w.tiles = (w.tokens + a.tile_tokens - 1) / a.tile_tokens;
+    w.keys = min(uint32_t(max(w.pos0 + int32_t(w.tokens), 0)), a.batch.max_blocks * a.batch.block_tokens);
+    return w;
+}
+__device__ __forceinline__ uint32_t parts_of(uint32_t keys, uint32_t length) { return keys > length ? (keys + length - 1) / length : 1; }
+
+// The keys of every tile in parts of at most `length`, the least length for which there are at most `target` items; with as many tiles as
+// that, whole.  A request's parts are then made equal.
+__global__ __launch_bounds__(SPLIT_THREADS) void paged_split_kernel(SplitArgs a) {
+    __shared__ uint32_t waves[SPLIT_WAVES], starts[SPLIT_THREADS], tiles_there;
+    const uint32_t tid = threadIdx.x, requests = a.batch.requests;
+    if (tid == 0) tiles_there = 0;
+
+    uint32_t tiles = 0, longest = 0;
+    for (uint32_t r = tid; r < requests; r += SPLIT_THREADS) {
+        const Work w = work_of(a, r);
+        tiles += w.tiles, longest = max(longest, w.keys);
+    }
+    const uint32_t all_tiles = total_of(tiles, waves);
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) longest = max(longest, uint32_t(__shfl_xor(longest, d)));
+    if ((tid & 63) == 0) waves[tid >> 6] = longest;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < SPLIT_WAVES; w++) longest = max(longest, waves[w]);
+    __syncthreads();
+    uint32_t high = (longest + a.granule - 1) / a.granule;  // granules: the least length is known to be no more
+    if (high == 0) high = 1;
+    if (all_tiles < a.target) {
+        uint32_t low = 1;
+        while (low < high) {
+            const uint32_t mid = (low + high) / 2;
+            uint32_t items = 0;
+            for (uint32_t r = tid; r < requests; r += SPLIT_THREADS) {
+                const Work w = work_of(a, r);
+                items += w.tiles * parts_of(w.keys, mid * a.granule);  // (at most tiles * 2^31 / granule; few tiles here)
+            }
+            if (total_of(min(items, 1u << 20), waves) <= a.target) high = mid;
+            else low = mid + 1;
+        }
+    }
+    const uint32_t length = high * a.granule;
+
+    uint32_t before = 0;
+    for (uint32_t r0 = 0; r0 < requests; r0 += SPLIT_THREADS) {
+        const Work mine = work_of(a, r0 + tid);
+        const uint32_t items = mine.tiles * parts_of(mine.keys, length);
+        // prefix sum over the workgroup
+        uint32_t through = items;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const uint32_t other = __shfl_up(through, d);
+            if ((tid & 63) >= uint32_t(d)) through += other;
+        }
+        if ((tid & 63) == 63) waves[tid >> 6] = through;
+        __syncthreads();
+        uint32_t base = 0, all = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < SPLIT_WAVES; w++) {
+            if (w < (tid >> 6)) base += waves[w];
+            all += waves[w];
+        }
+        starts[tid] = base + through - items;
+        __syncthreads();
+        for (uint32_t k = tid; k < all; k += SPLIT_THREADS) {
+            uint32_t i = 0, n = SPLIT_THREADS;  // the last request whose items start at k or before
+            while (n > 1) {
+                const uint32_t half = n / 2;
+                if (starts[i + half] <= k) i += half, n -= half;
+                else n = half;
+            }
+            const Work w = work_of(a, r0 + i);
+            const uint32_t parts = parts_of(w.keys, length), at = k - starts[i];
+            const uint32_t even = (w.keys + parts - 1) / parts, each = max((even + a.granule - 1) / a.granule * a.granule, a.granule);
+            const uint32_t tile = w.tiles - 1 - at / parts;  // the tiles with the most keys first
+            Item item;
+            item.request = r0 + i, item.part = at % parts;
+            item.row0 = w.row0 + tile * a.tile_tokens, item.tokens = min(a.tile_tokens, w.tokens - tile * a.tile_tokens);
+            item.pos0 = w.pos0 + int32_t(tile * a.tile_tokens);
+            const uint32_t keys = min(uint32_t(max(item.pos0 + int32_t(item.tokens), 0)), w.keys);
+            item.parts = parts_of(keys, each);
+            item.key0 = item.part * each, item.key1 = min(item.key0 + each, keys);
+            if (item.part >= item.parts) item.parts = 0;
+            const uint32_t where = before + k;
+            if (where >= a.most_items) continue;  // (never: most_items has room for every split that this makes)
+            a.items[where] = item;
+            if (item.part == 0 && item.parts > 1) {
+                const uint32_t t = atomicAdd(&tiles_there, 1u);  // (their order does not matter: each is joined by itself)
+                a.tiles[t] = where;
+            }
+        }
+        before += all;
+        __syncthreads();
+    }
+    if (tid == 0) *a.head = {min(before, a.most_items), tiles_there, {0, 0}};
+}
+
+// ---- the attention kernels ----------------------------------------------------------------------------------------
+
+struct AttnArgs {
+    saetta_strided_rows q, gate, out;
+    saetta_paged_cache cache;
+    const int32_t *block_table;
+    const SplitHead *head;
+    const Item *items;
+    float *part_o;   // [item][kv head][tile rows][256], relative to M
+    float *part_ml;  // [item][kv head][tile rows][M, sum]
+    uint32_t requests, max_blocks, tokens, group, group_shift, block_shift, target, tile_tokens;
+    float scale;
+};
+
+// Codes of one dword as four halves.
+__device__ __forceinline__ u32x2 halves_of(uint32_t w) {
+    const half2_ a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true);
+    return u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+}
+template <int TYPE>
+__device__ __forceinline__ u32x2 operands_of(uint32_t w) {
+    if constexpr (TYPE == SAETTA_F16) return halves_of(w);
+    const brain2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true);
+    return u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+}
+template <int TYPE>
+__device__ __forceinline__ u32x4 operands_of(uint32_t w0, uint32_t w1) {
+    const u32x2 a = operands_of<TYPE>(w0), b = operands_of<TYPE>(w1);
+    return u32x4{a.x, a.y, b.x, b.y};
+}
+template <int TYPE>
+__device__ __forceinline__ floatx4 product16(u32x4 a, u32x4 b, floatx4 c) {
+    if constexpr (TYPE == SAETTA_F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(brain8, a), __builtin_bit_cast(brain8, b), c, 0, 0, 0);
+}
+template <int TYPE>
+__device__ __forceinline__ floatx16 product32(u32x4 a, u32x4 b, floatx16 c) {
+    if constexpr (TYPE == SAETTA_F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(brain8, a), __builtin_bit_cast(brain8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+    const half2_ h = {(_Float16)a, (_Float16)b};
+    return __builtin_bit_cast(uint32_t, h);
+}
+__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.4426950408889634f)); }
+
+// Where a unit of 16 tokens lies and what its codes are scaled by.  Units that are not there (no block, or not one of the
+// cache) are read from the cache's first block and masked.
+struct Unit {
+    uint32_t block;     // row of [blocks][kv_heads]; of the first block where there is none
+    uint32_t scales;    // 127 + ek | (127 + ev) << 8 | there << 16
+};
+constexpr uint32_t WINDOW = 512;  // units whose places a workgroup keeps in LDS
+
+__device__ __forceinline__ void find_units(const AttnArgs &a, Unit *units, uint32_t request, uint32_t head, uint32_t first, uint32_t end, uint32_t threads) {
+    const uint32_t shift = a.block_shift - 4;
+    for (uint32_t u = threadIdx.x; u < WINDOW && first + u < end; u += threads) {
+        const uint32_t entry = (first + u) >> shift;
+        uint32_t block = entry < a.max_blocks ? uint32_t(a.block_table[size_t(request) * a.max_blocks + entry]) : ~0u;
+        const bool there = block < a.cache.blocks;
+        if (!there) block = 0;
+        const uint32_t row = block * a.cache.kv_heads + head;
+        units[u] = {row, uint32_t(a.cache.key_scales[row]) | uint32_t(a.cache.value_scales[row]) << 8 | uint32_t(there) << 16};
+    }
+}
+// (exponents as the store writes them: what else a byte says would make scores no numbers)
+__device__ __forceinline__ float key_scale(uint32_t scales) { return power_of_two(min(max(int(scales & 0xff) - 127, LOWEST_EXPONENT), HIGHEST_EXPONENT)); }
+__device__ __forceinline__ int value_exponent(uint32_t scales) { return min(max(int(scales >> 8 & 0xff) - 127, LOWEST_EXPONENT), HIGHEST_EXPONENT); }
+
+// An item that the split has made for these buffers.  (A split of other parameters is not followed out of them.)
+__device__ __forceinline__ bool item_ok(const AttnArgs &a, const Item &item, uint32_t index) {
+    return item.parts > 0 && item.request < a.requests && item.tokens > 0 && item.tokens <= a.tile_tokens && item.row0 <= a.tokens && item.tokens <= a.tokens - item.row0 &&
+           item.part < item.parts && (item.parts == 1 || index < a.target) && item.key1 <= a.max_blocks << a.block_shift;
+}
+
+// Bytes of a dword of four tokens' values that are NaN, as 0x80 in each.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+// Bytes of the first n of four tokens.
+__device__ __forceinline__ uint32_t first_bytes(int n) { return n <= 0 ? 0u : n >= 4 ? ~0u : (1u << (8 * n)) - 1; }
+
+// A dword of four tokens' values of one dim, cleared where no row may see it: from key `limit` on what a block happens to
+// hold, and NaN from key `all` on, where the tile's first rows end (0 * NaN would reach rows that do not see the token; nan_from
+// [256] keeps the first such key of a dim, and the rows that do see it become NaN at the end).
+__device__ __forceinline__ uint32_t clean_values(uint32_t w, uint32_t key, uint32_t limit, uint32_t all, uint32_t dim, uint32_t *nan_from) {
+    w &= first_bytes(int(limit) - int(key));
+    const uint32_t bad = nan_bytes(w) & ~first_bytes(int(all) - int(key));
+    if (bad) {
+        atomicMin(&nan_from[dim], key + (__builtin_ctz(bad) >> 3));
+        w &= ~((bad >> 7) * 0xffu);
+    }
+    return w;
+}
+
+// out of a row's four dims
+template <int TYPE>
+__device__ __forceinline__ void put_row(const AttnArgs &a, uint64_t row, uint32_t head, uint32_t dim, float (&o)[4]) {
+    typedef typename Row<TYPE>::value V;
+    if (a.gate.data) {
+        float g[4];
+        load_values<TYPE, 4>(static_cast<const V *>(a.gate.data) + row * a.gate.token_stride + head * a.gate.head_stride + dim, g);
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] *= sigmoid(g[i]);
+    }
+    store_values<TYPE, 4>(static_cast<V *>(a.out.data) + row * a.out.token_stride + head * a.out.head_stride + dim, o);
+}
+
+// Few rows: a workgroup of 4 waves walks an item's keys, every wave 32 of 128 at a time, straight from memory into registers, the next
+// step's codes on their way while this one's are worked on.  Bound by memory: 16 KB a step of a wave, against 64 + 64
+// conversions of two codes and 16 + 16 products.  Row l % 16 of the tile is lane l's; the waves' sums are joined in LDS.
+struct Codes {
+    u32x4 k[2][4], v[2][4];  // [unit][64 dims]
+};
+constexpr int FEW_STRIDE = DIM + 4;  // floats of a row in LDS: neighbouring rows on other banks
+template <int TYPE>
+__global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(AttnArgs a) {
+    typedef typename Row<TYPE>::value V;
+    __shared__ Unit units[WINDOW];
+    __shared__ __attribute__((aligned(16))) float sums[FEW_WAVES][FEW_ROWS][FEW_STRIDE];
+    __shared__ float ml[FEW_WAVES][FEW_ROWS][2];
+    __shared__ uint32_t nan_from[DIM];
+    const uint32_t index = blockIdx.x / a.cache.kv_heads, kv = blockIdx.x % a.cache.kv_heads;
+    if (index >= a.head->items) return;
+    const Item item = a.items[index];
+    if (!item_ok(a, item, index)) return;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t col = lane & 15, quarter = lane >> 4;
+    const uint32_t rows = item.tokens << a.group_shift;  // of the tile that are there
+    for (uint32_t i = tid; i < DIM; i += 64 * FEW_WAVES) nan_from[i] = ~0u;
+
+    const uint32_t row = min(col, rows - 1), token = row >> a.group_shift, head = kv * a.group + (row & (a.group - 1));
+    const V *qp = static_cast<const V *>(a.q.data) + (uint64_t(item.row0) + token) * a.q.token_stride + head * a.q.head_stride;
+    u32x4 q[8];  // [64 dims][8 of 16]
+#pragma unroll
+    for (int i = 0; i < 8; i++) q[i] = *reinterpret_cast<const u32x4 *>(qp + (i >> 1) * 64 + quarter * 16 + (i & 1) * 8);
+    const float c = a.scale * 1.4426950408889634f;
+    const int32_t sees = item.pos0 + int32_t(token) + 1;  // keys of this row
+    const uint32_t all_see = uint32_t(max(item.pos0 + 1, 0));  // of the first row, and so of all
+
+    floatx4 acc[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) acc[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = NO_MAXIMUM, l = 0.0f;
+
+    const size_t block_bytes = size_t(DIM) << a.block_shift;
+    const uint32_t unit_mask = (1u << (a.block_shift - 4)) - 1;
+    const uint32_t end_unit = (item.key1 + UNIT_TOKENS - 1) / UNIT_TOKENS;
+    for (uint32_t first = item.key0 / UNIT_TOKENS; first < end_unit; first += WINDOW) {
+        __syncthreads();
+        find_units(a, units, item.request, kv, first, end_unit, 64 * FEW_WAVES);
+        __syncthreads();
+        const uint32_t in_window = min(WINDOW, end_unit - first), steps = (in_window + 1) / 2;
+        auto unit_at = [&](uint32_t step, int i) {  // (a step's second unit may be past the end: the first once more, masked)
+            const uint32_t u = min(2 * step + i, in_window - 1);
+            return Unit{uint32_t(__builtin_amdgcn_readfirstlane(units[u].block)), uint32_t(__builtin_amdgcn_readfirstlane(units[u].scales))};
+        };
+        auto fetch = [&](uint32_t step, Codes &x) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const Unit u = unit_at(step, i);
+                const size_t at = u.block * block_bytes + ((first + min(2 * step + i, in_window - 1)) & unit_mask) * UNIT_BYTES + lane * 16;
+#pragma unroll
+                for (int j = 0; j < 4; j++) x.k[i][j] = *reinterpret_cast<const u32x4 *>(a.cache.keys + at + j * 1024);
+#pragma unroll
+                for (int j = 0; j < 4; j++) x.v[i][j] = *reinterpret_cast<const u32x4 *>(a.cache.values + at + j * 1024);
+            }
+        };
+        auto work = [&](uint32_t step, Codes &x) {
+            const uint32_t key = (first + 2 * step) * UNIT_TOKENS;
+            const Unit u0 = unit_at(step, 0), u1 = unit_at(step, 1);
+            floatx4 s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    s[i] = product16<TYPE>(operands_of<TYPE>(x.k[i][j].x, x.k[i][j].y), q[2 * j], s[i]);
+                    s[i] = product16<TYPE>(operands_of<TYPE>(x.k[i][j].z, x.k[i][j].w), q[2 * j + 1], s[i]);
+                }
+            }
+            const int ev[2] = {value_exponent(u0.scales), value_exponent(u1.scales)};
+            const float ck[2] = {c * key_scale(u0.scales), c * key_scale(u1.scales)};
+            float p[2][4], top = NO_SCORE;
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) p[i][r] = fmaf(s[i][r], ck[i], float(ev[i]));
+            const bool there = u0.scales & u1.scales & 0x10000;
+            if (key + STEP_KEYS > min(all_see, item.key1) || !there) {
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const bool unit_there = (i ? u1.scales : u0.scales) & 0x10000;
+                    const uint32_t from = key + i * UNIT_TOKENS + quarter * 4;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const uint32_t t = from + r;
+                        p[i][r] = unit_there && t < item.key1 && int32_t(t) < sees ? p[i][r] : NO_SCORE;
+                    }
+                    const uint32_t limit = unit_there ? item.key1 : 0;
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+#pragma unroll
+                        for (int t = 0; t < 4; t++) x.v[i][j][t] = clean_values(x.v[i][j][t], from, limit, all_see, (4 * j + t) * 16 + col, nan_from);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) top = fmaxf(top, p[i][r]);
+            top = across_rows<16, 64>(top, MaxOp());
+            if (__any(top > m + TAU)) {
+                const float next = top > m + TAU ? top : m, down = __builtin_amdgcn_exp2f(m - next);
+                m = next, l *= down;
+#pragma unroll
+                for (int i = 0; i < 16; i++) acc[i] *= down;
+            }
+            float part[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) p[i][r] = __builtin_amdgcn_exp2f(p[i][r] - m), part[i] += p[i][r];
+            l = fmaf(part[0], power_of_two(-ev[0]), fmaf(part[1], power_of_two(-ev[1]), l));
+            const u32x4 w = {pack_half2(p[0][0], p[0][1]), pack_half2(p[0][2], p[0][3]), pack_half2(p[1][0], p[1][1]), pack_half2(p[1][2], p[1][3])};
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const u32x2 v0 = halves_of(x.v[0][j][t]), v1 = halves_of(x.v[1][j][t]);
+                    acc[4 * j + t] = product16<SAETTA_F16>(u32x4{v0.x, v0.y, v1.x, v1.y}, w, acc[4 * j + t]);
+                }
+        };
+        Codes x, y;
+        if (wave < steps) {
+            fetch(wave, x);
+            for (uint32_t step = wave; step < steps; step += 2 * FEW_WAVES) {
+                const uint32_t next = step + FEW_WAVES, after = step + 2 * FEW_WAVES;
+                if (next < steps) fetch(next, y);
+                work(step, x);
+                if (after < steps) fetch(after, x);
+                if (next < steps) work(next, y);
+            }
+        }
+    }
+
+    l = across_rows<16, 64>(l, SumOp());
+#pragma unroll
+    for (int i = 0; i < 16; i++) *reinterpret_cast<floatx4 *>(&sums[wave][col][i * 16 + quarter * 4]) = acc[i];
+    if (quarter == 0) ml[wave][col][0] = m, ml[wave][col][1] = l;
+    __syncthreads();
+    for (uint32_t r = wave; r < rows; r += FEW_WAVES) {
+        float top = NO_MAXIMUM, sum = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < FEW_WAVES; w++) top = fmaxf(top, ml[w][r][0]);
+        const uint32_t dim = lane * 4;
+#pragma unroll
+        for (int w = 0; w < FEW_WAVES; w++) {
+            const float f = __builtin_amdgcn_exp2f(ml[w][r][0] - top);
+            sum = fmaf(ml[w][r][1], f, sum);
+            const floatx4 x = *reinterpret_cast<const floatx4 *>(&sums[w][r][dim]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[i] = fmaf(x[i], f, o[i]);
+        }
+        const uint32_t tok = r >> a.group_shift;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (nan_from[dim + i] != ~0u && int32_t(nan_from[dim + i]) < item.pos0 + int32_t(tok) + 1) o[i] = __builtin_nanf("");
+        if (item.parts > 1) {
+            const size_t slot = (size_t(index) * a.cache.kv_heads + kv) * FEW_ROWS + r;
+            *reinterpret_cast<floatx4 *>(a.part_o + slot * DIM + dim) = floatx4{o[0], o[1], o[2], o[3]};
+            if (lane == 0) *reinterpret_cast<float2 *>(a.part_ml + slot * 2) = float2{top, sum};
+        } else {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[i] *= inv;
+            put_row<TYPE>(a, uint64_t(item.row0) + tok, kv * a.group + (r & (a.group - 1)), dim, o);
+        }
+    }
+}
+
+// Chunks: a workgroup of 8 waves takes 256 rows (256 / group tokens of the q heads of a kv head), 32 a wave, over an item's keys, 32 a step.  Every thread
+// converts 16 codes of keys and 16 of values of the next step and puts them into LDS in the order of the operands, once for all 8 waves.
+constexpr uint32_t PART_BYTES = STEP_KEYS * DIM * 2;  // a step's keys, or values, as halves
+template <int TYPE>
+__global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnArgs a) {
+    typedef typename Row<TYPE>::value V;
+    extern __shared__ __attribute__((aligned(1024))) unsigned char tiles[];  // keys, keys, values, values
+    __shared__ Unit units[WINDOW];
+    __shared__ uint32_t nan_from[DIM];
+    const uint32_t index = blockIdx.x / a.cache.kv_heads, kv = blockIdx.x % a.cache.kv_heads;
+    if (index >= a.head->items) return;
+    const Item item = a.items[index];
+    if (!item_ok(a, item, index)) return;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t col = lane & 31, hf = lane >> 5;
+    const uint32_t rows = item.tokens << a.group_shift;
+    for (uint32_t i = tid; i < DIM; i += 64 * CHUNK_WAVES) nan_from[i] = ~0u;
+
+    const uint32_t my_row = wave * 32 + col, row = min(my_row, rows - 1), token = row >> a.group_shift, head = kv * a.group + (row & (a.group - 1));
+    const V *qp = static_cast<const V *>(a.q.data) + (uint64_t(item.row0) + token) * a.q.token_stride + head * a.q.head_stride;
+    u32x4 q[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) q[i] = *reinterpret_cast<const u32x4 *>(qp + i * 16 + hf * 8);
+    const float c = a.scale * 1.4426950408889634f;
+    const int32_t sees = item.pos0 + int32_t(token) + 1;
+    const uint32_t all_see = uint32_t(max(item.pos0 + 1, 0));
+    // what the wave's first and last rows see
+    const uint32_t first_row = min(wave * 32, rows - 1), last_row = min(wave * 32 + 31, rows - 1);
+    const uint32_t wave_all = uint32_t(max(item.pos0 + int32_t(first_row >> a.group_shift) + 1, 0));
+    const uint32_t wave_end = wave * 32 < rows ? min(uint32_t(max(item.pos0 + int32_t(last_row >> a.group_shift) + 1, 0)), item.key1) : 0;
+
+    floatx16 acc[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[i][r] = 0.0f;
+    float m = NO_MAXIMUM, l = 0.0f;
+
+    const size_t block_bytes = size_t(DIM) << a.block_shift;
+    const uint32_t unit_mask = (1u << (a.block_shift - 4)) - 1;
+    const uint32_t end_unit = (item.key1 + UNIT_TOKENS - 1) / UNIT_TOKENS;
+    for (uint32_t first = item.key0 / UNIT_TOKENS; first < end_unit; first += WINDOW) {
+        __syncthreads();
+        find_units(a, units, item.request, kv, first, end_unit, 64 * CHUNK_WAVES);
+        __syncthreads();
+        const uint32_t in_window = min(WINDOW, end_unit - first), steps = (in_window + 1) / 2;
+        u32x4 kc, vc;  // codes on their way: 16 bytes of a unit, keys and values
+        const uint32_t mine = tid >> 8, piece = tid & 255;
+        auto fetch = [&](uint32_t step) {
+            const uint32_t u = min(2 * step + mine, in_window - 1);
+            const size_t at = units[u].block * block_bytes + ((first + u) & unit_mask) * UNIT_BYTES + piece * 16;
+            kc = *reinterpret_cast<const u32x4 *>(a.cache.keys + at);
+            vc = *reinterpret_cast<const u32x4 *>(a.cache.values + at);
+        };
+        auto put = [&](uint32_t step) {
+            unsigned char *kt = tiles + (step & 1) * PART_BYTES, *vt = tiles + (2 + (step & 1)) * PART_BYTES;
+            const uint32_t t = piece & 15, quarter = piece >> 4 & 3, j = piece >> 6;
+            // keys: token t, dims 64 j + 16 quarter .. + 15: both halves of fragment 4 j + quarter
+            unsigned char *kd = kt + (4 * j + quarter) * 1024 + (mine * 16 + t) * 16;
+            *reinterpret_cast<u32x4 *>(kd) = operands_of<TYPE>(kc.x, kc.y);
+            *reinterpret_cast<u32x4 *>(kd + 512) = operands_of<TYPE>(kc.z, kc.w);
+            // values: tokens 4 quarter .. + 3 of dims 16 (4 j + i) + t
+            const uint32_t u = 2 * step + mine, key = (first + u) * UNIT_TOKENS;
+            if (key + UNIT_TOKENS > min(all_see, item.key1) || u >= in_window || !(units[min(u, in_window - 1)].scales & 0x10000)) {
+                const uint32_t limit = u < in_window && (units[u].scales & 0x10000) ? item.key1 : 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) vc[i] = clean_values(vc[i], key + 4 * quarter, limit, all_see, (4 * j + i) * 16 + t, nan_from);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t dim = (4 * j + i) * 16 + t;
+                *reinterpret_cast<u32x2 *>(vt + (2 * (dim >> 5) + mine) * 1024 + (quarter & 1) * 512 + (dim & 31) * 16 + (quarter >> 1) * 8) = halves_of(vc[i]);
+            }
+        };
+        fetch(0);
+        put(0);
+        for (uint32_t step = 0; step < steps; step++) {
+            if (step + 1 < steps) fetch(step + 1);
+            __syncthreads();  // this step's keys and values are in LDS, and the last step's have been read
+            const uint32_t key = (first + 2 * step) * UNIT_TOKENS;
+            if (key < wave_end) {
+                const unsigned char *kt = tiles + (step & 1) * PART_BYTES + lane * 16, *vt = tiles + (2 + (step & 1)) * PART_BYTES + lane * 16;
+                floatx16 s;
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[r] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; i++) s = product32<TYPE>(*reinterpret_cast<const u32x4 *>(kt + i * 1024), q[i], s);
+                const uint32_t scales[2] = {units[2 * step].scales, units[min(2 * step + 1, in_window - 1)].scales};
+                float ck[2], sum[2] = {0.0f, 0.0f}, top = NO_SCORE;
+                int ev[2];
+#pragma unroll
+                for (int i = 0; i < 2; i++) ck[i] = c * key_scale(scales[i]), ev[i] = value_exponent(scales[i]);
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[r] = fmaf(s[r], ck[r >> 3], float(ev[r >> 3]));
+                if (key + STEP_KEYS > min(wave_all, item.key1) || !(scales[0] & scales[1] & 0x10000)) {
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        const uint32_t t = key + 4 * hf + (r & 3) + 8 * (r >> 2);
+                        s[r] = (scales[r >> 3] & 0x10000) && t < item.key1 && int32_t(t) < sees ? s[r] : NO_SCORE;
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < 16; r++) top = fmaxf(top, s[r]);
+                top = across_rows<32, 64>(top, MaxOp());
+                if (__any(top > m + TAU)) {
+                    const float next = top > m + TAU ? top : m, down = __builtin_amdgcn_exp2f(m - next);
+                    m = next, l *= down;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) acc[i] *= down;
+                }
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[r] = __builtin_amdgcn_exp2f(s[r] - m), sum[r >> 3] += s[r];
+                l = fmaf(sum[0], power_of_two(-ev[0]), fmaf(sum[1], power_of_two(-ev[1]), l));
+#pragma unroll
+                for (int sp = 0; sp < 2; sp++) {
+                    const u32x4 w = {pack_half2(s[8 * sp], s[8 * sp + 1]), pack_half2(s[8 * sp + 2], s[8 * sp + 3]),
+                                     pack_half2(s[8 * sp + 4], s[8 * sp + 5]), pack_half2(s[8 * sp + 6], s[8 * sp + 7])};
+#pragma unroll
+                    for (int i = 0; i < 8; i++) acc[i] = product32<SAETTA_F16>(*reinterpret_cast<const u32x4 *>(vt + (2 * i + sp) * 1024), w, acc[i]);
+                }
+            }
+            if (step + 1 < steps) put(step + 1);
+        }
+    }
+
+    __syncthreads();  // nan_from is whole
+    l = across_rows<32, 64>(l, SumOp());
+    if (my_row >= rows) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const size_t slot = (size_t(index) * a.cache.kv_heads + kv) * CHUNK_ROWS + my_row;
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const uint32_t dim = 32 * i + 4 * hf + 8 * k;
+            float o[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                o[j] = acc[i][4 * k + j];
+                if (nan_from[dim + j] != ~0u && int32_t(nan_from[dim + j]) < sees) o[j] = __builtin_nanf("");
+            }
+            if (item.parts > 1) {
+                *reinterpret_cast<floatx4 *>(a.part_o + slot * DIM + dim) = floatx4{o[0], o[1], o[2], o[3]};
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[j] *= inv;
+                put_row<TYPE>(a, uint64_t(item.row0) + token, head, dim, o);
+            }
+        }
+    if (item.parts > 1 && hf == 0) *reinterpret_cast<float2 *>(a.part_ml + slot * 2) = float2{m, l};
+}
+
+// Joins the parts of the tiles that were taken in parts: out = sum_p 2^(M_p - M) O_p / sum_p 2^(M_p - M) l_p.  A wave a row, a
+// lane four dims; where rows are few, the four waves of a workgroup take a row's parts by turns and join through LDS.
+template <int TYPE, bool FEW>
+__global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, const uint32_t *tiles) {
+    if (blockIdx.x >= a.head->tiles) return;
+    const uint32_t index = tiles[blockIdx.x], kv = blockIdx.z;
+    if (index >= a.target) return;
+    const Item item = a.items[index];
+    if (!item_ok(a, item, index) || item.parts > a.target - index) return;
+    constexpr uint32_t TILE = FEW ? FEW_ROWS : CHUNK_ROWS;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t r = FEW ? blockIdx.y : blockIdx.y * 4 + wave, rows = item.tokens << a.group_shift;
+    if (r >= rows) return;  // (FEW: the whole workgroup)
+    const size_t stride = size_t(a.cache.kv_heads) * TILE, slot = (size_t(index) * a.cache.kv_heads + kv) * TILE + r;
+    float m = NO_MAXIMUM, l = 0.0f;
+    floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t p = FEW ? wave : 0; p < item.parts; p += FEW ? 4 : 1) {
+        const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + (slot + p * stride) * 2);
+        const floatx4 x = *reinterpret_cast<const floatx4 *>(a.part_o + (slot + p * stride) * DIM + lane * 4);
+        const float next = fmaxf(m, ml.x), f = __builtin_amdgcn_exp2f(m - next), g = __builtin_amdgcn_exp2f(ml.x - next);
+        m = next, l = l * f + ml.y * g;
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] = o[i] * f + x[i] * g;
+    }
+    if constexpr (FEW) {
+        __shared__ __attribute__((aligned(16))) float part[4][64][4];
+        __shared__ float pml[4][2];
+        *reinterpret_cast<floatx4 *>(part[wave][lane]) = o;
+        if (lane == 0) pml[wave][0] = m, pml[wave][1] = l;
+        __syncthreads();
+        if (wave > 0) return;
+        float top = NO_MAXIMUM;
+#pragma unroll
+        for (int w = 0; w < 4; w++) top = fmaxf(top, pml[w][0]);
+        l = 0.0f, o = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float f = __builtin_amdgcn_exp2f(pml[w][0] - top);
+            l += pml[w][1] * f;
+            const floatx4 x = *reinterpret_cast<const floatx4 *>(part[w][lane]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[i] += x[i] * f;
+        }
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    float x[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = o[i] * inv;
+    put_row<TYPE>(a, uint64_t(item.row0) + (r >> a.group_shift), kv * a.group + (r & (a.group - 1)), lane * 4, x);
+}
+
+int check_attn(const saetta_paged_attn_params &p, uint32_t requests, const char *what) {
+    SAETTA_REQUIRE(p.kv_heads > 0 && p.heads % p.kv_heads == 0 && p.kv_heads <= 32767, SAETTA_E_SHAPE, "%s: %u q heads over %u kv heads", what, p.heads, p.kv_heads);
+    const uint32_t group = p.heads / p.kv_heads;
+    SAETTA_REQUIRE(group == 1 || group == 2 || group == 4 || group == 8 || group == 16, SAETTA_E_SHAPE, "%s: %u q heads per kv head (1, 2, 4, 8 or 16)", what, group);
+    SAETTA_REQUIRE(p.tokens < (1u << 31) && requests < (1u << 24), SAETTA_E_SHAPE, "%s: %u tokens of %u requests", what, p.tokens, requests);
+    SAETTA_REQUIRE(p.rows > 0, SAETTA_E_SHAPE, "%s: rows 0", what);
+    // (one workgroup to an item and kv head)
+    SAETTA_REQUIRE(uint64_t(shape_of(p, requests).most_items) * p.kv_heads < (1u << 31), SAETTA_E_SHAPE, "%s: %u tokens of %u requests over %u kv heads", what,
+                   p.tokens, requests, p.kv_heads);
+    return SAETTA_OK;
+}
+int check_batch(const saetta_paged_batch &b, const char *what) {
+    SAETTA_REQUIRE(b.query_starts && b.kv_lens && b.block_table, SAETTA_E_NULL, "%s: null buffer", what);
+    SAETTA_REQUIRE(aligned(b.query_starts, 4) && aligned(b.kv_lens, 4) && aligned(b.block_table, 4), SAETTA_E_ALIGN, "%s: the batch must be 4-byte aligned", what);
+    SAETTA_REQUIRE(block_tokens_ok(b.block_tokens), SAETTA_E_SHAPE, "%s: blocks of %u tokens (16, 32, 64 or 128)", what, b.block_tokens);
+    SAETTA_REQUIRE(b.max_blocks > 0 && uint64_t(b.max_blocks) * b.block_tokens < (1ull << 31), SAETTA_E_SHAPE, "%s: rows of %u blocks", what, b.max_blocks);
+    return SAETTA_OK;
+}
+size_t items_offset() { return sizeof(SplitHead); }
+size_t tiles_offset(const Shape &s) { return items_offset() + sizeof(Item) * s.most_items; }
+
+constexpr uint32_t CHUNK_LDS = 4 * PART_BYTES;
+uint32_t shift_of(uint32_t n) { return uint32_t(__builtin_ctz(n)); }
+
+template <int TYPE>
+void launch_attn(hipStream_t stream, const AttnArgs &a, const Shape &s, const saetta_paged_attn_params &p, const uint32_t *tiles) {
+    const dim3 grid(s.most_items * p.kv_heads);
+    // a tile in parts has two at least, and all of them are among the first `target` items
+    const uint32_t joined = s.target / 2 < s.most_tiles ? s.target / 2 : s.most_tiles;
+    if (s.tile_rows == FEW_ROWS) {
+        launch(paged_few_kernel<TYPE>, grid, dim3(64 * FEW_WAVES), 0, stream, a);
+        if (joined) launch(paged_merge_kernel<TYPE, true>, dim3(joined, p.rows * s.group, p.kv_heads), dim3(256), 0, stream, a, tiles);
+    } else {
+        launch(paged_chunk_kernel<TYPE>, grid, dim3(64 * CHUNK_WAVES), CHUNK_LDS, stream, a);
+        if (joined) launch(paged_merge_kernel<TYPE, false>, dim3(joined, CHUNK_ROWS / 4, p.kv_heads), dim3(256), 0, stream, a, tiles);
+    }
+}
+
+}  // namespace
+
+int setup_paged_attn() {
+    for (const void *k : {reinterpret_cast<const void *>(paged_chunk_kernel<SAETTA_F16>), reinterpret_cast<const void *>(paged_chunk_kernel<SAETTA_BF16>)}) {
+        if (int rc = load_kernel(k)) return rc;
+        if (int rc = int(hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, CHUNK_LDS))) return rc;
+    }
+    return 0;
+}
+
+}  // namespace saetta
+
+using namespace saetta;
+
+extern "C" size_t saetta_paged_split_bytes(saetta_paged_attn_params p, uint32_t requests) {
+    if (check_attn(p, requests, "paged_split_bytes")) return 0;
+    const Shape s = shape_of(p, requests);
+    return tiles_offset(s) + 4 * size_t(s.most_items);
+}
+
+extern "C" size_t saetta_paged_workspace_bytes(saetta_paged_attn_params p, uint32_t requests) {
+    if (check_attn(p, requests, "paged_workspace_bytes")) return 0;
+    const Shape s = shape_of(p, requests);
+    return size_t(s.target) * p.kv_heads * s.tile_rows * (DIM + 2) * sizeof(float);
+}
+
+extern "C" int saetta_paged_split(saetta_stream_t stream, saetta_paged_batch batch, saetta_paged_attn_params p, void *split) {
+    if (int rc = check_attn(p, batch.requests, "paged_split")) return rc;
+    if (int rc = check_batch(batch, "paged_split")) return rc;
+    SAETTA_REQUIRE(split, SAETTA_E_NULL, "paged_split: null buffer");
+    SAETTA_REQUIRE(aligned(split, 16), SAETTA_E_ALIGN, "paged_split: split must be 16-byte aligned");
+    if (int rc = ensure_device()) return rc;
+    const Shape s = shape_of(p, batch.requests);
+    unsigned char *at = static_cast<unsigned char *>(split);
+    const bool few = s.tile_rows == FEW_ROWS;
+    const SplitArgs a = {batch, reinterpret_cast<SplitHead *>(at), reinterpret_cast<Item *>(at + items_offset()), reinterpret_cast<uint32_t *>(at + tiles_offset(s)),
+                         s.tile_tokens, s.target, s.most_items, p.tokens, p.rows, few, few ? STEP_KEYS * FEW_WAVES : 256u};
+    launch(paged_split_kernel, dim3(1), dim3(SPLIT_THREADS), 0, as_stream(stream), a);
+    return launch_status("paged_split");
+}
+
+extern "C" int saetta_paged_attn(saetta_stream_t stream, int type, saetta_strided_rows q, saetta_paged_cache cache, saetta_paged_batch batch,
+                                 const void *split, saetta_strided_rows gate, saetta_strided_rows out, saetta_paged_attn_params p, void *workspace,
+                                 size_t workspace_bytes) {
+    SAETTA_REQUIRE(type == SAETTA_F16 || type == SAETTA_BF16, SAETTA_E_BITS, "paged_attn: type %d (f16 or bf16)", type);
+    if (int rc = check_attn(p, batch.requests, "paged_attn")) return rc;
+    if (int rc = check_batch(batch, "paged_attn")) return rc;
+    if (int rc = check_cache(cache, "paged_attn")) return rc;
+    SAETTA_REQUIRE(cache.kv_heads == p.kv_heads && cache.block_tokens == batch.block_tokens, SAETTA_E_SHAPE,
+                   "paged_attn: a cache of %u kv heads and blocks of %u tokens, a call of %u and %u", cache.kv_heads, cache.block_tokens, p.kv_heads, batch.block_tokens);
+    SAETTA_REQUIRE(q.data && out.data && split && workspace, SAETTA_E_NULL, "paged_attn: null buffer");
+    SAETTA_REQUIRE(rows_aligned(q, type) && rows_aligned(out, type) && rows_aligned(gate, type), SAETTA_E_ALIGN,
+                   "paged_attn: q, gate and out must be 16-byte aligned, with strides of multiples of 16 bytes");
+    SAETTA_REQUIRE(aligned(split, 16) && aligned(workspace, 16), SAETTA_E_ALIGN, "paged_attn: split and workspace must be 16-byte aligned");
+    const size_t need = saetta_paged_workspace_bytes(p, batch.requests);
+    SAETTA_REQUIRE(workspace_bytes >= need, SAETTA_E_SCRATCH, "paged_attn: workspace of %zu bytes (%zu needed)", workspace_bytes, need);
+    if (int rc = ensure_device()) return rc;
+    if (batch.requests == 0 || p.tokens == 0) return SAETTA_OK;
+    const Shape s = shape_of(p, batch.requests);
+    const unsigned char *at = static_cast<const unsigned char *>(split);
+    float *part_o = static_cast<float *>(workspace);
+    const AttnArgs a = {q, gate, out, cache, batch.block_table, reinterpret_cast<const SplitHead *>(at), reinterpret_cast<const Item *>(at + items_offset()),
+                        part_o, part_o + size_t(s.target) * p.kv_heads * s.tile_rows * DIM, batch.requests, batch.max_blocks, p.tokens,
+                        s.group, shift_of(s.group), shift_of(cache.block_tokens), s.target, s.tile_tokens, p.scale};
+    const uint32_t *tiles = reinterpret_cast<const uint32_t *>(at + tiles_offset(s));
+    if (type == SAETTA_F16) launch_attn<SAETTA_F16>(as_stream(stream), a, s, p, tiles);
+    else launch_attn<SAETTA_BF16>(as_stream(stream), a, s, p, tiles);
+    return launch_status("paged_attn");
+}

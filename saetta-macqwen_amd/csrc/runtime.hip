@@ -76,7 +76,8 @@ int ensure_device() {
             d.status_host = static_cast<volatile uint32_t *>(host);
             d.status_dev = static_cast<uint32_t *>(devp);
         }
-        int (*const setups[])() = {setup_runtime, setup_kv_quant, setup_prep, setup_deltanet, setup_decode, setup_prefill};
+        int (*const setups[])() = {setup_runtime, setup_kv_quant, setup_prep, setup_deltanet, setup_decode, setup_prefill,
+                                 setup_paged_tables, setup_paged_cache, setup_paged_attn};
         for (auto setup : setups) {
             if (int rc = setup()) {
                 d.status = SAETTA_E_DEVICE;

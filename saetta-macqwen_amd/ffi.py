@@ -19,6 +19,8 @@ SYMBOLS = [
     "saetta_part_o_bytes", "saetta_part_ml_bytes", "saetta_attn_decode", "saetta_attn_decode_quant",
     "saetta_attn_rows", "saetta_attn_rows_quant", "saetta_static_scratch_bytes", "saetta_attn_decode_quant_static", "saetta_prefill_workspace_bytes", "saetta_attn_prefill", "saetta_attn_prefill_quant",
     "saetta_attn_gemm_workspace_bytes", "saetta_attn_gemm",
+    "saetta_paged_tables", "saetta_paged_store", "saetta_paged_gather", "saetta_paged_split_bytes", "saetta_paged_workspace_bytes",
+    "saetta_paged_split", "saetta_paged_attn",
 ]
 
 STAGE_PARTIAL, STAGE_REDUCE, STAGE_ALL, STAGE_NO_LOADERS = 1, 2, 3, 4
@@ -50,6 +52,44 @@ class FlashParamsC(ctypes.Structure):
 
 class QuantRowsC(ctypes.Structure):
     _fields_ = [("data", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("biases", ctypes.c_void_p)]
+
+
+F32, F16, BF16 = 0, 1, 2  # SAETTA_F32 ..
+
+
+class PagedCacheC(ctypes.Structure):
+    _fields_ = [("keys", ctypes.c_void_p), ("values", ctypes.c_void_p), ("key_scales", ctypes.c_void_p),
+                ("value_scales", ctypes.c_void_p), ("blocks", ctypes.c_uint32), ("block_tokens", ctypes.c_uint32),
+                ("kv_heads", ctypes.c_uint32)]
+
+
+class PagedStateC(ctypes.Structure):
+    _fields_ = [("block_table", ctypes.c_void_p), ("held", ctypes.c_void_p), ("free_list", ctypes.c_void_p),
+                ("free_count", ctypes.c_void_p)]
+
+
+class PagedStepC(ctypes.Structure):
+    _fields_ = [("query_starts", ctypes.c_void_p), ("kv_lens", ctypes.c_void_p), ("slots", ctypes.c_void_p),
+                ("positions", ctypes.c_void_p), ("unplaced", ctypes.c_void_p)]
+
+
+class PagedTablesParamsC(ctypes.Structure):
+    _fields_ = [("requests", ctypes.c_uint32), ("max_blocks", ctypes.c_uint32), ("block_tokens", ctypes.c_uint32),
+                ("blocks", ctypes.c_uint32), ("tokens", ctypes.c_uint32)]
+
+
+class StridedRowsC(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_uint64), ("head_stride", ctypes.c_uint64)]
+
+
+class PagedBatchC(ctypes.Structure):
+    _fields_ = [("query_starts", ctypes.c_void_p), ("kv_lens", ctypes.c_void_p), ("block_table", ctypes.c_void_p),
+                ("requests", ctypes.c_uint32), ("max_blocks", ctypes.c_uint32), ("block_tokens", ctypes.c_uint32)]
+
+
+class PagedAttnParamsC(ctypes.Structure):
+    _fields_ = [("heads", ctypes.c_uint32), ("kv_heads", ctypes.c_uint32), ("tokens", ctypes.c_uint32),
+                ("rows", ctypes.c_uint32), ("scale", ctypes.c_float)]
 
 
 class SaettaError(RuntimeError):
@@ -172,6 +212,18 @@ def lib():
         l.saetta_attn_gemm.restype = i32
         l.saetta_attn_gemm.argtypes = [vp, i32, vp, QuantRowsC, QuantRowsC, vp, vp, FlashParamsC, u32, u32, vp,
                                        ctypes.c_size_t]
+        l.saetta_paged_tables.restype = i32
+        l.saetta_paged_tables.argtypes = [vp, vp, vp, PagedStateC, PagedStepC, PagedTablesParamsC]
+        l.saetta_paged_store.restype = i32
+        l.saetta_paged_store.argtypes = [vp, i32, StridedRowsC, StridedRowsC, vp, PagedCacheC, u32]
+        l.saetta_paged_gather.restype = i32
+        l.saetta_paged_gather.argtypes = [vp, i32, PagedCacheC, vp, vp, vp, u32]
+        l.saetta_paged_split_bytes.restype, l.saetta_paged_split_bytes.argtypes = sz, [PagedAttnParamsC, u32]
+        l.saetta_paged_workspace_bytes.restype, l.saetta_paged_workspace_bytes.argtypes = sz, [PagedAttnParamsC, u32]
+        l.saetta_paged_split.restype, l.saetta_paged_split.argtypes = i32, [vp, PagedBatchC, PagedAttnParamsC, vp]
+        l.saetta_paged_attn.restype = i32
+        l.saetta_paged_attn.argtypes = [vp, i32, StridedRowsC, PagedCacheC, PagedBatchC, vp, StridedRowsC, StridedRowsC,
+                                        PagedAttnParamsC, vp, sz]
         _lib = l
     return _lib
 

@@ -622,6 +622,215 @@ class GpuKvCache:
         self.capacity = capacity
 
 
+_TYPES = {torch.float32: ffi.F32, torch.float16: ffi.F16, torch.bfloat16: ffi.BF16}
+_HALVES = (torch.float16, torch.bfloat16)
+
+
+def _here(what, *tensors):
+    """The tensors lie on the current device, which is where a call launches."""
+    device = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t.get_device() != device:
+            raise ValueError(f"{what}: a tensor is on {t.device}, the current device is cuda:{device}")
+
+
+def _rows_of(t, heads, dtypes, what):
+    """[tokens, heads, 256] with any strides that the library takes, as StridedRowsC."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes):
+        raise TypeError(f"{what}: expected a tensor of {' or '.join(str(d) for d in dtypes)} on the GPU")
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != DIM or t.stride(2) != 1:
+        raise ValueError(f"{what}: expected [tokens, {heads}, {DIM}] with contiguous rows")
+    # (a dim of one has whatever stride torch left there)
+    return ffi.StridedRowsC(t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if heads > 1 else 0)
+
+
+def _do(plan, stream, kernel, name, what, args, keep):
+    """One call of the library, now on a stream or as an op of a plan."""
+    if plan is not None:
+        plan.op(kernel, _Call(name, what, args, keep))
+    else:
+        _here(what, *[t for t in keep if t is not None])
+        ffi.check(getattr(ffi.lib(), name)(_stream(stream), *args), what)
+
+
+class PagedCache:
+    """The keys and values of one layer for several requests at once, in blocks of 16, 32, 64 or 128 tokens: 8-bit
+    floating point codes (e4m3) with one power of two per block and kv head, for keys and for values.  The reference
+    has no counterpart (its caches are one sequence's).  Slot s is token s % block_tokens of block s // block_tokens."""
+
+    def __init__(self, kv_heads, head_dim, blocks, block_tokens=64, device="cuda"):
+        if head_dim != DIM:
+            raise ValueError("a paged cache is written for head dim 256")
+        if block_tokens not in (16, 32, 64, 128) or blocks < 1 or blocks * block_tokens >= 1 << 31:
+            raise ValueError("PagedCache: blocks of 16, 32, 64 or 128 tokens, fewer than 2^31 in all")
+        self.kv_heads, self.head_dim, self.blocks, self.block_tokens = kv_heads, head_dim, blocks, block_tokens
+        self.keys, self.values = (torch.zeros(blocks, kv_heads, block_tokens * DIM, dtype=torch.uint8, device=device) for _ in range(2))
+        self.key_scales, self.value_scales = (torch.full((blocks, kv_heads), 127 - 40, dtype=torch.uint8, device=device) for _ in range(2))
+
+    def c(self):
+        return ffi.PagedCacheC(self.keys.data_ptr(), self.values.data_ptr(), self.key_scales.data_ptr(),
+                               self.value_scales.data_ptr(), self.blocks, self.block_tokens, self.kv_heads)
+
+    def tensors(self):
+        return self.keys, self.values, self.key_scales, self.value_scales
+
+    def bytes_per_token(self):
+        return 2 * self.kv_heads * (DIM + 1 / self.block_tokens)
+
+    def _store(self, plan, stream, k, v, slots):
+        rows = [_rows_of(t, self.kv_heads, tuple(_TYPES), what) for t, what in ((k, "PagedCache k"), (v, "PagedCache v"))]
+        _need(slots, torch.int32, "PagedCache slots")
+        if k.dtype is not v.dtype or k.shape[0] != v.shape[0] or slots.numel() != k.shape[0]:
+            raise ValueError("PagedCache: k, v and slots must be of as many tokens, k and v of one type")
+        _do(plan, stream, "paged_store", "saetta_paged_store", "paged_store",
+            (_TYPES[k.dtype], *rows, slots.data_ptr(), self.c(), slots.numel()), (k, v, slots, *self.tensors()))
+
+    def record(self, plan, k, v, slots):
+        """The keys and values [tokens, kv_heads, 256] of a step's tokens into their slots; -1: nowhere."""
+        self._store(plan, None, k, v, slots)
+
+    def encode(self, k, v, slots, stream=None):
+        self._store(None, stream, k, v, slots)
+
+    def _gather(self, plan, stream, slots, keys, values):
+        _need(slots, torch.int32, "PagedCache slots")
+        outs = [t for t in (keys, values) if t is not None]
+        for t in outs:
+            if not (isinstance(t, torch.Tensor) and t.dtype in _TYPES):
+                raise TypeError("PagedCache: keys and values must be tensors of f32, f16 or bf16")
+            _need(t, t.dtype, "PagedCache keys and values")
+            if t.numel() < slots.numel() * self.kv_heads * DIM:
+                raise ValueError("PagedCache: keys and values do not hold the slots' rows")
+        if not outs or outs[0].dtype is not outs[-1].dtype:
+            raise ValueError("PagedCache: keys or values or both, of one type")
+        _do(plan, stream, "paged_gather", "saetta_paged_gather", "paged_gather",
+            (_TYPES[outs[0].dtype], self.c(), slots.data_ptr(), *[None if t is None else t.data_ptr() for t in (keys, values)],
+             slots.numel()), (slots, keys, values, *self.tensors()))
+
+    def record_dequantize(self, plan, slots, keys, values):
+        """What the slots hold, as contiguous [tokens, kv_heads, 256]; either of the two may be None."""
+        self._gather(plan, None, slots, keys, values)
+
+    def encode_dequantize(self, slots, keys, values, stream=None):
+        self._gather(None, stream, slots, keys, values)
+
+
+class PagedTables:
+    """Which blocks the requests hold, and what a step's tokens are given: all on the GPU, from the requests' lengths.
+    `requests` rows, room for `tokens` new tokens a step, up to `max_blocks` blocks a request of a cache of `blocks`.
+    (The tensors are a program's own to fill, too, where it keeps tables on the host.)"""
+
+    def __init__(self, requests, tokens, max_blocks, blocks, block_tokens=64, device="cuda"):
+        if requests < 1 or tokens < 1 or max_blocks < 1 or blocks < 1:
+            raise ValueError("PagedTables: sizes of one at least")
+        if block_tokens not in (16, 32, 64, 128) or blocks * block_tokens >= 1 << 31 or max_blocks * block_tokens >= 1 << 31:
+            raise ValueError("PagedTables: blocks of 16, 32, 64 or 128 tokens, fewer than 2^31 in all")
+        self.requests, self.tokens, self.max_blocks, self.blocks, self.block_tokens = requests, tokens, max_blocks, blocks, block_tokens
+        ints = {"dtype": torch.int32, "device": device}
+        self.block_table = torch.full((requests, max_blocks), -1, **ints)
+        self.held = torch.zeros(requests, **ints)
+        self.free_list = torch.arange(blocks, **ints)
+        self.free_count = torch.full((1,), blocks, **ints)
+        self.query_starts, self.kv_lens = torch.zeros(requests + 1, **ints), torch.zeros(requests, **ints)
+        self.slots, self.positions = torch.full((tokens,), -1, **ints), torch.full((tokens,), -1, **ints)
+        self.unplaced = torch.zeros(1, **ints)
+
+    def tensors(self):
+        return (self.block_table, self.held, self.free_list, self.free_count, self.query_starts, self.kv_lens, self.slots,
+                self.positions, self.unplaced)
+
+    def batch(self):
+        return ffi.PagedBatchC(self.query_starts.data_ptr(), self.kv_lens.data_ptr(), self.block_table.data_ptr(), self.requests,
+                               self.max_blocks, self.block_tokens)
+
+    def _tables(self, plan, stream, context_lens, new_lens):
+        for t, what in ((context_lens, "context_lens"), (new_lens, "new_lens")):
+            _need(t, torch.int32, f"PagedTables {what}")
+            if t.numel() != self.requests:
+                raise ValueError(f"PagedTables: {what} must be of {self.requests} requests")
+        at = [t.data_ptr() for t in self.tensors()]
+        params = ffi.PagedTablesParamsC(self.requests, self.max_blocks, self.block_tokens, self.blocks, self.tokens)
+        _do(plan, stream, "paged_tables", "saetta_paged_tables", "paged_tables",
+            (context_lens.data_ptr(), new_lens.data_ptr(), ffi.PagedStateC(*at[:4]), ffi.PagedStepC(*at[4:]), params),
+            (context_lens, new_lens, *self.tensors()))
+
+    def record(self, plan, context_lens, new_lens):
+        """A step of new_lens[r] tokens behind context_lens[r]: blocks taken or given back, slots, positions, query_starts,
+        kv_lens.  context_lens may be kv_lens: a recorded step then goes on from where the last one ended."""
+        self._tables(plan, None, context_lens, new_lens)
+
+    def encode(self, context_lens, new_lens, stream=None):
+        self._tables(None, stream, context_lens, new_lens)
+
+
+class PagedAttention:
+    """Attention of a step's new tokens over paged caches: scratch and launches for tables of one size and up to `rows`
+    new tokens a request (1: a token each; a verify step's rows; a chunk's tokens; any mixture).  The scratch is one
+    call's at a time: calls, or graphs of them, that may overlap want objects of their own."""
+
+    def __init__(self, heads, kv_heads, head_dim, tables, rows, device=None):
+        if head_dim != DIM:
+            raise ValueError("paged attention is written for head dim 256")
+        if kv_heads < 1 or heads % kv_heads or heads // kv_heads not in (1, 2, 4, 8, 16):
+            raise ValueError("paged attention needs 1, 2, 4, 8 or 16 q heads per kv head")
+        if rows < 1:
+            raise ValueError("paged attention: rows of one at least")
+        self.heads, self.kv_heads, self.rows = heads, kv_heads, rows
+        self.shape = (tables.requests, tables.tokens, tables.max_blocks, tables.block_tokens)
+        self.scale = 1.0 / math.sqrt(DIM)
+        device = tables.block_table.device if device is None else device
+        l, p = ffi.lib(), self._params()
+        with torch.cuda.device(device):  # (the sizes are of the device's compute units)
+            split, workspace = l.saetta_paged_split_bytes(p, tables.requests), l.saetta_paged_workspace_bytes(p, tables.requests)
+        if not split or not workspace:
+            raise ValueError("paged attention: " + l.saetta_last_error().decode())
+        self.split = torch.empty(split, dtype=torch.uint8, device=device)
+        self.workspace = torch.empty(workspace, dtype=torch.uint8, device=device)
+
+    def _params(self):
+        return ffi.PagedAttnParamsC(self.heads, self.kv_heads, self.shape[1], self.rows, self.scale)
+
+    def _check(self, tables):
+        if (tables.requests, tables.tokens, tables.max_blocks, tables.block_tokens) != self.shape:
+            raise ValueError("paged attention: made for tables of another size")
+
+    def _split(self, plan, stream, tables):
+        self._check(tables)
+        _do(plan, stream, "paged_split", "saetta_paged_split", "paged_split", (tables.batch(), self._params(), self.split.data_ptr()),
+            (self.split, tables.query_starts, tables.kv_lens, tables.block_table))
+
+    def record_split(self, plan, tables):
+        """Deals a step's rows and keys out, once for all layers: behind the tables, before the first layer's attention."""
+        self._split(plan, None, tables)
+
+    def encode_split(self, tables, stream=None):
+        self._split(None, stream, tables)
+
+    def _attend(self, plan, stream, q, cache, tables, out, gate):
+        self._check(tables)
+        if (cache.kv_heads, cache.block_tokens) != (self.kv_heads, tables.block_tokens):
+            raise ValueError("paged attention: a cache of other kv heads or blocks")
+        rows = [_rows_of(t, self.heads, _HALVES, what) for t, what in ((q, "q"), (out, "out"))]
+        gate_rows = ffi.StridedRowsC(None, 0, 0) if gate is None else _rows_of(gate, self.heads, _HALVES, "gate")
+        for t, what in ((q, "q"), (out, "out"), (gate, "gate")):
+            if t is not None and (t.dtype is not q.dtype or t.shape[0] < tables.tokens):
+                raise ValueError(f"paged attention: {what} must be of q's type and of {tables.tokens} tokens")
+        if 0 in (out.stride(0) if out.shape[0] > 1 else 1, out.stride(1) if self.heads > 1 else 1):
+            raise ValueError("paged attention: out's rows must lie apart")
+        _do(plan, stream, "paged_attention", "saetta_paged_attn", "paged_attn",
+            (_TYPES[q.dtype], rows[0], cache.c(), tables.batch(), self.split.data_ptr(), gate_rows, rows[1], self._params(),
+             self.workspace.data_ptr(), self.workspace.numel()),
+            (q, out, gate, *cache.tensors(), tables.query_starts, tables.kv_lens, tables.block_table, self.split, self.workspace))
+
+    def record(self, plan, q, cache, tables, out, gate=None):
+        """q, out and gate [tokens, heads, 256] in f16 or bf16, any strides of multiples of 16 bytes: the halves of a projection's
+        output as they are.  Rows past the step's last token are left as they were."""
+        self._attend(plan, None, q, cache, tables, out, gate)
+
+    def encode(self, q, cache, tables, out, gate=None, stream=None):
+        self._attend(None, stream, q, cache, tables, out, gate)
+
+
 class RowBackup:
     """RowBackup (src/gpu_cache.rs:196-283): a copy of KV rows from..from + n of every attention
     layer, for a short detour that writes over a long conversation; `restore` puts them back."""
