@@ -82,17 +82,17 @@ struct SplitArgs {
 };
 
 constexpr int SPLIT_THREADS = 1024, SPLIT_WAVES = SPLIT_THREADS / 64;
+constexpr uint32_t SPLIT_HELD = 1024;  // requests whose tiles and keys are kept in LDS
 
-__device__ __forceinline__ uint32_t total_of(uint32_t x, uint32_t *waves) {
+__device__ __forceinline__ uint32_t wave_sum(uint32_t x) {
 #pragma unroll
     for (int d = 32; d > 0; d /= 2) x += __shfl_xor(x, d);
-    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = x;
-    __syncthreads();
-    uint32_t all = 0;
+    return x;
+}
+__device__ __forceinline__ uint64_t wave_sum(uint64_t x) {
 #pragma unroll
-    for (int w = 0; w < SPLIT_WAVES; w++) all += waves[w];
-    __syncthreads();
-    return all;
+    for (int d = 32; d > 0; d /= 2) x += __shfl_xor(x, d);
+    return x;
 }
 
 // A request as the split sees it.
@@ -114,42 +114,53 @@ __device__ __forceinline__ Work work_of(const SplitArgs &a, uint32_t r) {
 }
 __device__ __forceinline__ uint32_t parts_of(uint32_t keys, uint32_t length) { return keys > length ? (keys + length - 1) / length : 1; }
 
-// The keys of every tile in parts of at most `length`, the least length for which there are at most `target` items; with as many tiles as
-// that, whole.  A request's parts are then made equal.
+// The keys of every tile in parts of at most `length`, the least length (in granules) for which there are at most `target` items; with as
+// many tiles as that, whole.  A request's parts are then made equal.  For a length p the items are between total / p and total / p + tiles,
+// which leaves few lengths to try: one wave bisects them, without barriers.
 __global__ __launch_bounds__(SPLIT_THREADS) void paged_split_kernel(SplitArgs a) {
-    __shared__ uint32_t waves[SPLIT_WAVES], starts[SPLIT_THREADS], tiles_there;
+    __shared__ uint32_t waves[SPLIT_WAVES], starts[SPLIT_THREADS], tiles_there, chosen;
+    __shared__ uint2 held[SPLIT_HELD];  // tiles, keys
     const uint32_t tid = threadIdx.x, requests = a.batch.requests;
-    if (tid == 0) tiles_there = 0;
-
-    uint32_t tiles = 0, longest = 0;
-    for (uint32_t r = tid; r < requests; r += SPLIT_THREADS) {
+    for (uint32_t r = tid; r < min(requests, SPLIT_HELD); r += SPLIT_THREADS) {
         const Work w = work_of(a, r);
-        tiles += w.tiles, longest = max(longest, w.keys);
+        held[r] = uint2{w.tiles, w.keys};
     }
-    const uint32_t all_tiles = total_of(tiles, waves);
-#pragma unroll
-    for (int d = 32; d > 0; d /= 2) longest = max(longest, uint32_t(__shfl_xor(longest, d)));
-    if ((tid & 63) == 0) waves[tid >> 6] = longest;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < SPLIT_WAVES; w++) longest = max(longest, waves[w]);
-    __syncthreads();
-    uint32_t high = (longest + a.granule - 1) / a.granule;  // granules: the least length is known to be no more
-    if (high == 0) high = 1;
-    if (all_tiles < a.target) {
-        uint32_t low = 1;
-        while (low < high) {
-            const uint32_t mid = (low + high) / 2;
-            uint32_t items = 0;
-            for (uint32_t r = tid; r < requests; r += SPLIT_THREADS) {
-                const Work w = work_of(a, r);
-                items += w.tiles * parts_of(w.keys, mid * a.granule);  // (at most tiles * 2^31 / granule; few tiles here)
-            }
-            if (total_of(min(items, 1u << 20), waves) <= a.target) high = mid;
-            else low = mid + 1;
+    if (tid < 64) {
+        auto shape = [&](uint32_t r) {
+            if (r < SPLIT_HELD) return held[r];
+            const Work w = work_of(a, r);
+            return uint2{w.tiles, w.keys};
+        };
+        uint32_t tiles = 0, longest = 0;
+        uint64_t total = 0;
+        for (uint32_t r = tid; r < requests; r += 64) {
+            const uint2 w = shape(r);
+            tiles += w.x, longest = max(longest, w.y), total += uint64_t(w.x) * w.y;
         }
+        tiles = wave_sum(tiles), total = wave_sum(total);
+#pragma unroll
+        for (int d = 32; d > 0; d /= 2) longest = max(longest, uint32_t(__shfl_xor(longest, d)));
+        uint32_t high = max((longest + a.granule - 1) / a.granule, 1u);  // in granules: a length that will do
+        if (tiles < a.target) {
+            const uint64_t enough = total / (uint64_t(a.target - tiles) * a.granule) + 1, least = total / (uint64_t(a.target) * a.granule);
+            high = uint32_t(min(uint64_t(high), enough));
+            uint32_t low = uint32_t(max(min(least, uint64_t(high)), uint64_t(1)));
+            while (low < high) {
+                const uint32_t mid = (low + high) / 2;
+                uint32_t items = 0;  // (tiles * parts: with so few tiles no more than some thousands)
+                for (uint32_t r = tid; r < requests; r += 64) {
+                    const uint2 w = shape(r);
+                    items += w.x * parts_of(w.y, mid * a.granule);
+                }
+                if (wave_sum(items) <= a.target) high = mid;
+                else low = mid + 1;
+            }
+        }
+        if (tid == 0) chosen = high, tiles_there = 0;
     }
-    const uint32_t length = high * a.granule;
+    __syncthreads();
+    const uint32_t length = chosen * a.granule;
 
     uint32_t before = 0;
     for (uint32_t r0 = 0; r0 < requests; r0 += SPLIT_THREADS) {
@@ -311,34 +322,67 @@ __device__ __forceinline__ void put_row(const AttnArgs &a, uint64_t row, uint32_
     store_values<TYPE, 4>(static_cast<V *>(a.out.data) + row * a.out.token_stride + head * a.out.head_stride + dim, o);
 }
 
-// Few rows: a workgroup of 4 waves walks an item's keys, every wave 32 of 128 at a time, straight from memory into registers, the next
-// step's codes on their way while this one's are worked on.  Bound by memory: 16 KB a step of a wave, against 64 + 64
-// conversions of two codes and 16 + 16 products.  Row l % 16 of the tile is lane l's; the waves' sums are joined in LDS.
-struct Codes {
-    u32x4 k[2][4], v[2][4];  // [unit][64 dims]
-};
-constexpr int FEW_STRIDE = DIM + 4;  // floats of a row in LDS: neighbouring rows on other banks
+// Few rows: a workgroup of 4 waves walks an item's keys, every wave 32 of 128 at a time, straight from memory into registers, the
+// keys of its next step on their way while this one's values are worked on, and the other way round.  Bound by memory: 16 KB a step of a
+// wave, against 64 + 64 conversions of two codes and 16 + 16 products.  Row l % 16 of the tile is lane l's; the waves' sums are joined in LDS.
+// A wave looks up the places of the units of its next 32 steps by itself, a unit a lane: no barrier in the walk, and the scales, which only the
+// scores want, come behind the first codes.
+constexpr uint32_t FEW_STEPS = 32;     // steps that a wave looks up at a time
+constexpr int FEW_STRIDE = DIM + 4;    // floats of a row in LDS: neighbouring rows on other banks
 template <int TYPE>
 __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(AttnArgs a) {
     typedef typename Row<TYPE>::value V;
-    __shared__ Unit units[WINDOW];
     __shared__ __attribute__((aligned(16))) float sums[FEW_WAVES][FEW_ROWS][FEW_STRIDE];
     __shared__ float ml[FEW_WAVES][FEW_ROWS][2];
     __shared__ uint32_t nan_from[DIM];
     const uint32_t index = blockIdx.x / a.cache.kv_heads, kv = blockIdx.x % a.cache.kv_heads;
-    if (index >= a.head->items) return;
+    const uint32_t items = a.head->items;
     const Item item = a.items[index];
-    if (!item_ok(a, item, index)) return;
+    if (!(int(index < items) & int(item_ok(a, item, index)))) return;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t col = lane & 15, quarter = lane >> 4;
     const uint32_t rows = item.tokens << a.group_shift;  // of the tile that are there
     for (uint32_t i = tid; i < DIM; i += 64 * FEW_WAVES) nan_from[i] = ~0u;
+
+    const size_t block_bytes = size_t(DIM) << a.block_shift;
+    const uint32_t unit_shift = a.block_shift - 4, unit_mask = (1u << unit_shift) - 1;
+    const uint32_t end_unit = (item.key1 + UNIT_TOKENS - 1) / UNIT_TOKENS;
+    uint32_t first = item.key0 / UNIT_TOKENS + 2 * wave;  // the wave's first unit; its steps are 2 * FEW_WAVES units apart
+    // Lane 2 i + j: unit j of step i, its row of [blocks][kv heads] (of block 0 where there is none) and whether there is one.
+    uint32_t place = 0, scales = 0;
+    auto look_up = [&] {
+        const uint32_t unit = first + (lane >> 1) * (2 * FEW_WAVES) + (lane & 1), entry = unit >> unit_shift;
+        uint32_t block = ~0u;
+        if (unit < end_unit && entry < a.max_blocks) block = uint32_t(a.block_table[size_t(item.request) * a.max_blocks + entry]);
+        const bool there = block < a.cache.blocks;
+        place = (there ? block : 0) * a.cache.kv_heads + kv;
+        scales = uint32_t(there) << 16;
+    };
+    auto look_up_scales = [&] { scales |= uint32_t(a.cache.key_scales[place]) | uint32_t(a.cache.value_scales[place]) << 8; };
+    u32x4 k[2][4], v[2][4];  // codes of a step: [unit][64 dims]
+    auto fetch = [&](const uint8_t *codes, uint32_t step, u32x4 (&x)[2][4]) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const uint32_t row = __builtin_amdgcn_readlane(place, 2 * step + i), unit = (first + step * (2 * FEW_WAVES) + i) & unit_mask;
+            const uint8_t *at = codes + row * block_bytes + unit * UNIT_BYTES;
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[i][j] = *reinterpret_cast<const u32x4 *>(at + j * 1024 + lane * 16);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // (on their way from here on, not where they are wanted)
+    };
+    uint32_t steps = first < end_unit ? (end_unit - first + 2 * FEW_WAVES - 1) / (2 * FEW_WAVES) : 0;  // that are left
+    if (steps) {
+        look_up();
+        fetch(a.cache.keys, 0, k);
+        look_up_scales();
+    }
 
     const uint32_t row = min(col, rows - 1), token = row >> a.group_shift, head = kv * a.group + (row & (a.group - 1));
     const V *qp = static_cast<const V *>(a.q.data) + (uint64_t(item.row0) + token) * a.q.token_stride + head * a.q.head_stride;
     u32x4 q[8];  // [64 dims][8 of 16]
 #pragma unroll
     for (int i = 0; i < 8; i++) q[i] = *reinterpret_cast<const u32x4 *>(qp + (i >> 1) * 64 + quarter * 16 + (i & 1) * 8);
+    if (steps) fetch(a.cache.values, 0, v);
     const float c = a.scale * 1.4426950408889634f;
     const int32_t sees = item.pos0 + int32_t(token) + 1;  // keys of this row
     const uint32_t all_see = uint32_t(max(item.pos0 + 1, 0));  // of the first row, and so of all
@@ -347,65 +391,45 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(AttnArgs a
 #pragma unroll
     for (int i = 0; i < 16; i++) acc[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = NO_MAXIMUM, l = 0.0f;
+    __syncthreads();  // nan_from is clear
 
-    const size_t block_bytes = size_t(DIM) << a.block_shift;
-    const uint32_t unit_mask = (1u << (a.block_shift - 4)) - 1;
-    const uint32_t end_unit = (item.key1 + UNIT_TOKENS - 1) / UNIT_TOKENS;
-    for (uint32_t first = item.key0 / UNIT_TOKENS; first < end_unit; first += WINDOW) {
-        __syncthreads();
-        find_units(a, units, item.request, kv, first, end_unit, 64 * FEW_WAVES);
-        __syncthreads();
-        const uint32_t in_window = min(WINDOW, end_unit - first), steps = (in_window + 1) / 2;
-        auto unit_at = [&](uint32_t step, int i) {  // (a step's second unit may be past the end: the first once more, masked)
-            const uint32_t u = min(2 * step + i, in_window - 1);
-            return Unit{uint32_t(__builtin_amdgcn_readfirstlane(units[u].block)), uint32_t(__builtin_amdgcn_readfirstlane(units[u].scales))};
-        };
-        auto fetch = [&](uint32_t step, Codes &x) {
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const Unit u = unit_at(step, i);
-                const size_t at = u.block * block_bytes + ((first + min(2 * step + i, in_window - 1)) & unit_mask) * UNIT_BYTES + lane * 16;
-#pragma unroll
-                for (int j = 0; j < 4; j++) x.k[i][j] = *reinterpret_cast<const u32x4 *>(a.cache.keys + at + j * 1024);
-#pragma unroll
-                for (int j = 0; j < 4; j++) x.v[i][j] = *reinterpret_cast<const u32x4 *>(a.cache.values + at + j * 1024);
-            }
-        };
-        auto work = [&](uint32_t step, Codes &x) {
-            const uint32_t key = (first + 2 * step) * UNIT_TOKENS;
-            const Unit u0 = unit_at(step, 0), u1 = unit_at(step, 1);
+    while (steps) {
+        const uint32_t here = min(steps, FEW_STEPS);
+        for (uint32_t step = 0; step < here; step++) {
+            const uint32_t key = (first + step * (2 * FEW_WAVES)) * UNIT_TOKENS;
             floatx4 s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
             for (int j = 0; j < 4; j++) {
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    s[i] = product16<TYPE>(operands_of<TYPE>(x.k[i][j].x, x.k[i][j].y), q[2 * j], s[i]);
-                    s[i] = product16<TYPE>(operands_of<TYPE>(x.k[i][j].z, x.k[i][j].w), q[2 * j + 1], s[i]);
+                    s[i] = product16<TYPE>(operands_of<TYPE>(k[i][j].x, k[i][j].y), q[2 * j], s[i]);
+                    s[i] = product16<TYPE>(operands_of<TYPE>(k[i][j].z, k[i][j].w), q[2 * j + 1], s[i]);
                 }
             }
-            const int ev[2] = {value_exponent(u0.scales), value_exponent(u1.scales)};
-            const float ck[2] = {c * key_scale(u0.scales), c * key_scale(u1.scales)};
+            if (step + 1 < here) fetch(a.cache.keys, step + 1, k);
+            const uint32_t scale[2] = {uint32_t(__builtin_amdgcn_readlane(scales, 2 * step)), uint32_t(__builtin_amdgcn_readlane(scales, 2 * step + 1))};
+            const int ev[2] = {value_exponent(scale[0]), value_exponent(scale[1])};
+            const float ck[2] = {c * key_scale(scale[0]), c * key_scale(scale[1])};
             float p[2][4], top = NO_SCORE;
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) p[i][r] = fmaf(s[i][r], ck[i], float(ev[i]));
-            const bool there = u0.scales & u1.scales & 0x10000;
-            if (key + STEP_KEYS > min(all_see, item.key1) || !there) {
+            if (key + STEP_KEYS > min(all_see, item.key1) || !(scale[0] & scale[1] & 0x10000)) {
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    const bool unit_there = (i ? u1.scales : u0.scales) & 0x10000;
+                    const bool there = scale[i] & 0x10000;
                     const uint32_t from = key + i * UNIT_TOKENS + quarter * 4;
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
                         const uint32_t t = from + r;
-                        p[i][r] = unit_there && t < item.key1 && int32_t(t) < sees ? p[i][r] : NO_SCORE;
+                        p[i][r] = there && t < item.key1 && int32_t(t) < sees ? p[i][r] : NO_SCORE;
                     }
-                    const uint32_t limit = unit_there ? item.key1 : 0;
+                    const uint32_t limit = there ? item.key1 : 0;
 #pragma unroll
                     for (int j = 0; j < 4; j++)
 #pragma unroll
-                        for (int t = 0; t < 4; t++) x.v[i][j][t] = clean_values(x.v[i][j][t], from, limit, all_see, (4 * j + t) * 16 + col, nan_from);
+                        for (int t = 0; t < 4; t++) v[i][j][t] = clean_values(v[i][j][t], from, limit, all_see, (4 * j + t) * 16 + col, nan_from);
                 }
             }
 #pragma unroll
@@ -430,20 +454,18 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(AttnArgs a
             for (int j = 0; j < 4; j++)
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
-                    const u32x2 v0 = halves_of(x.v[0][j][t]), v1 = halves_of(x.v[1][j][t]);
+                    const u32x2 v0 = halves_of(v[0][j][t]), v1 = halves_of(v[1][j][t]);
                     acc[4 * j + t] = product16<SAETTA_F16>(u32x4{v0.x, v0.y, v1.x, v1.y}, w, acc[4 * j + t]);
                 }
-        };
-        Codes x, y;
-        if (wave < steps) {
-            fetch(wave, x);
-            for (uint32_t step = wave; step < steps; step += 2 * FEW_WAVES) {
-                const uint32_t next = step + FEW_WAVES, after = step + 2 * FEW_WAVES;
-                if (next < steps) fetch(next, y);
-                work(step, x);
-                if (after < steps) fetch(after, x);
-                if (next < steps) work(next, y);
-            }
+            if (step + 1 < here) fetch(a.cache.values, step + 1, v);
+        }
+        steps -= here;
+        if (steps) {
+            first += FEW_STEPS * 2 * FEW_WAVES;
+            look_up();
+            fetch(a.cache.keys, 0, k);
+            look_up_scales();
+            fetch(a.cache.values, 0, v);
         }
     }
 
@@ -492,9 +514,9 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
     __shared__ Unit units[WINDOW];
     __shared__ uint32_t nan_from[DIM];
     const uint32_t index = blockIdx.x / a.cache.kv_heads, kv = blockIdx.x % a.cache.kv_heads;
-    if (index >= a.head->items) return;
+    const uint32_t items = a.head->items;
     const Item item = a.items[index];
-    if (!item_ok(a, item, index)) return;
+    if (!(int(index < items) & int(item_ok(a, item, index)))) return;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t col = lane & 31, hf = lane >> 5;
     const uint32_t rows = item.tokens << a.group_shift;
