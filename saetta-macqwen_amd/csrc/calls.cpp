@@ -26,6 +26,11 @@ struct Library {
     decltype(&saetta_attn_prefill_quant) attn_prefill_quant;
     decltype(&saetta_token_params_set) token_params_set;
     decltype(&saetta_plan_run) plan_run;
+    decltype(&saetta_paged_tables) paged_tables;
+    decltype(&saetta_paged_store) paged_store;
+    decltype(&saetta_paged_gather) paged_gather;
+    decltype(&saetta_paged_split) paged_split;
+    decltype(&saetta_paged_attn) paged_attn;
 };
 
 // What a copy of the package has set up (`setup`), kept with its module.
@@ -62,6 +67,8 @@ const Library &library(State &st) {
         find(lib.last_error, "saetta_last_error"), find(lib.to_half, "saetta_to_half"), find(lib.kv_quantize, "saetta_kv_quantize");
         find(lib.attn_prefill, "saetta_attn_prefill"), find(lib.attn_prefill_quant, "saetta_attn_prefill_quant");
         find(lib.token_params_set, "saetta_token_params_set"), find(lib.plan_run, "saetta_plan_run");
+        find(lib.paged_tables, "saetta_paged_tables"), find(lib.paged_store, "saetta_paged_store"), find(lib.paged_gather, "saetta_paged_gather");
+        find(lib.paged_split, "saetta_paged_split"), find(lib.paged_attn, "saetta_paged_attn");
         lib.loaded = true;
     }
     return lib;
@@ -258,9 +265,177 @@ PyObject *plan_run(PyObject *module, PyObject *const *a, Py_ssize_t n) {
     });
 }
 
+// ---- a cache in blocks ------------------------------------------------------------------------------------------------
+// The objects of host.py hand their buffers and sizes over as one tuple, made once; what changes from call to call is checked here.
+
+PyObject *item(PyObject *tuple, Py_ssize_t i, Py_ssize_t n, const char *what) {
+    if (!PyTuple_Check(tuple) || PyTuple_GET_SIZE(tuple) != n) raise(PyExc_TypeError, "%s: expected a tuple of %zd", what, n);
+    return PyTuple_GET_ITEM(tuple, i);
+}
+// A contiguous tensor of `dtype` on the current device.
+const at::Tensor &here(PyObject *o, at::ScalarType dtype, const char *what) {
+    if (!THPVariable_Check(o)) raise(PyExc_TypeError, "%s: expected a tensor", what);
+    const at::Tensor &t = THPVariable_Unpack(o);
+    if (t.scalar_type() != dtype || !t.is_cuda() || !t.is_contiguous())
+        raise(PyExc_TypeError, "%s: expected a contiguous torch.%s tensor on the GPU", what, dtype == at::kInt ? "int32" : "uint8");
+    if (t.get_device() != c10::hip::current_device())
+        raise(PyExc_ValueError, "%s is on cuda:%d, the current device is cuda:%d", what, int(t.get_device()), int(c10::hip::current_device()));
+    return t;
+}
+int type_of(const at::Tensor &t, bool floats, const char *what) {
+    if (t.scalar_type() == at::kHalf) return SAETTA_F16;
+    if (t.scalar_type() == at::kBFloat16) return SAETTA_BF16;
+    if (t.scalar_type() == at::kFloat && floats) return SAETTA_F32;
+    raise(PyExc_TypeError, "%s: expected a tensor of %storch.float16 or torch.bfloat16 on the GPU", what, floats ? "torch.float32, " : "");
+}
+// [tokens, heads, 256] with rows that are contiguous.
+struct Rows {
+    saetta_strided_rows rows;
+    long long tokens;
+    int type;
+};
+Rows rows_of(PyObject *o, long long heads, bool floats, const char *what) {
+    if (!THPVariable_Check(o)) raise(PyExc_TypeError, "%s: expected a tensor", what);
+    const at::Tensor &t = THPVariable_Unpack(o);
+    const int type = type_of(t, floats, what);
+    if (!t.is_cuda()) raise(PyExc_TypeError, "%s: expected a tensor on the GPU", what);
+    if (t.get_device() != c10::hip::current_device())
+        raise(PyExc_ValueError, "%s is on cuda:%d, the current device is cuda:%d", what, int(t.get_device()), int(c10::hip::current_device()));
+    if (t.dim() != 3 || t.size(1) != heads || t.size(2) != SAETTA_HEAD_DIM || t.stride(2) != 1)
+        raise(PyExc_ValueError, "%s: expected [tokens, %lld, %d] with contiguous rows", what, heads, SAETTA_HEAD_DIM);
+    // (a dim of one has whatever stride torch left there)
+    return {{t.data_ptr(), uint64_t(t.size(0) > 1 ? t.stride(0) : 0), uint64_t(heads > 1 ? t.stride(1) : 0)}, t.size(0), type};
+}
+// (keys, values, key_scales, value_scales, blocks, block_tokens, kv_heads)
+saetta_paged_cache paged_cache(PyObject *o) {
+    auto codes = [&](Py_ssize_t i) { return pointer<uint8_t>(here(item(o, i, 7, "paged cache"), at::kByte, "paged cache")); };
+    return {codes(0), codes(1), codes(2), codes(3), u32(item(o, 4, 7, "paged cache")), u32(item(o, 5, 7, "paged cache")), u32(item(o, 6, 7, "paged cache"))};
+}
+// (query_starts, kv_lens, block_table, requests, max_blocks, block_tokens)
+saetta_paged_batch paged_batch(PyObject *o) {
+    auto ints = [&](Py_ssize_t i) { return pointer<uint32_t>(here(item(o, i, 6, "paged batch"), at::kInt, "paged batch")); };
+    return {ints(0), ints(1), reinterpret_cast<const int32_t *>(ints(2)), u32(item(o, 3, 6, "paged batch")), u32(item(o, 4, 6, "paged batch")),
+            u32(item(o, 5, 6, "paged batch"))};
+}
+// (heads, kv_heads, tokens, rows, scale)
+saetta_paged_attn_params paged_params(PyObject *o) {
+    const double scale = PyFloat_AsDouble(item(o, 4, 5, "paged attention"));
+    if (scale == -1.0 && PyErr_Occurred()) throw Raised{};
+    return {u32(item(o, 0, 5, "paged attention")), u32(item(o, 1, 5, "paged attention")), u32(item(o, 2, 5, "paged attention")),
+            u32(item(o, 3, 5, "paged attention")), float(scale)};
+}
+
+// paged_tables(context_lens, new_lens, (the nine tensors of PagedTables.tensors), (requests, max_blocks, block_tokens, blocks, tokens), stream)
+PyObject *paged_tables(PyObject *module, PyObject *const *a, Py_ssize_t n) {
+    return guarded(n, 5, "paged_tables", [&] {
+        const saetta_paged_tables_params p{u32(item(a[3], 0, 5, "PagedTables")), u32(item(a[3], 1, 5, "PagedTables")), u32(item(a[3], 2, 5, "PagedTables")),
+                                           u32(item(a[3], 3, 5, "PagedTables")), u32(item(a[3], 4, 5, "PagedTables"))};
+        if (PyErr_Occurred()) throw Raised{};
+        const at::Tensor &context = here(a[0], at::kInt, "PagedTables context_lens"), &fresh = here(a[1], at::kInt, "PagedTables new_lens");
+        if (context.numel() != p.requests || fresh.numel() != p.requests)
+            raise(PyExc_ValueError, "PagedTables: context_lens and new_lens must be of %u requests", p.requests);
+        auto ints = [&](Py_ssize_t i) { return pointer<int32_t>(here(item(a[2], i, 9, "PagedTables"), at::kInt, "PagedTables")); };
+        auto lengths = [&](Py_ssize_t i) { return reinterpret_cast<uint32_t *>(ints(i)); };
+        const saetta_paged_state state{ints(0), lengths(1), ints(2), lengths(3)};
+        const saetta_paged_step step{lengths(4), lengths(5), ints(6), ints(7), lengths(8)};
+        State &st = state_of(module);
+        const Library &lib = library(st);
+        const saetta_stream_t s = stream_of(a[4]);
+        const uint32_t *c = pointer<uint32_t>(context), *f = pointer<uint32_t>(fresh);
+        return call("paged_tables", st, [&] { return lib.paged_tables(s, c, f, state, step, p); });
+    });
+}
+
+// paged_store(k, v, slots, cache, stream)
+PyObject *paged_store(PyObject *module, PyObject *const *a, Py_ssize_t n) {
+    return guarded(n, 5, "paged_store", [&] {
+        const saetta_paged_cache cache = paged_cache(a[3]);
+        if (PyErr_Occurred()) throw Raised{};
+        const Rows k = rows_of(a[0], cache.kv_heads, true, "PagedCache k"), v = rows_of(a[1], cache.kv_heads, true, "PagedCache v");
+        const at::Tensor &slots = here(a[2], at::kInt, "PagedCache slots");
+        if (k.type != v.type || k.tokens != v.tokens || slots.numel() != k.tokens)
+            raise(PyExc_ValueError, "PagedCache: k, v and slots must be of as many tokens, k and v of one type");
+        State &st = state_of(module);
+        const Library &lib = library(st);
+        const saetta_stream_t s = stream_of(a[4]);
+        const int32_t *at = pointer<int32_t>(slots);
+        return call("paged_store", st, [&] { return lib.paged_store(s, k.type, k.rows, v.rows, at, cache, uint32_t(k.tokens)); });
+    });
+}
+
+// paged_gather(slots, keys or None, values or None, cache, stream)
+PyObject *paged_gather(PyObject *module, PyObject *const *a, Py_ssize_t n) {
+    return guarded(n, 5, "paged_gather", [&] {
+        const saetta_paged_cache cache = paged_cache(a[3]);
+        if (PyErr_Occurred()) throw Raised{};
+        const at::Tensor &slots = here(a[0], at::kInt, "PagedCache slots");
+        int type = -1;
+        void *to[2] = {nullptr, nullptr};
+        for (int i = 0; i < 2; i++) {
+            if (a[1 + i] == Py_None) continue;
+            if (!THPVariable_Check(a[1 + i])) raise(PyExc_TypeError, "PagedCache: keys and values must be tensors");
+            const at::Tensor &t = THPVariable_Unpack(a[1 + i]);
+            const int is = type_of(t, true, "PagedCache keys and values");
+            if (!t.is_cuda() || !t.is_contiguous()) raise(PyExc_TypeError, "PagedCache keys and values: expected contiguous tensors on the GPU");
+            if (t.get_device() != c10::hip::current_device())
+                raise(PyExc_ValueError, "PagedCache keys and values: on cuda:%d, the current device is cuda:%d", int(t.get_device()), int(c10::hip::current_device()));
+            if (type >= 0 && is != type) raise(PyExc_ValueError, "PagedCache: keys and values of one type");
+            if (t.numel() < slots.numel() * int64_t(cache.kv_heads) * SAETTA_HEAD_DIM) raise(PyExc_ValueError, "PagedCache: keys and values do not hold the slots' rows");
+            type = is, to[i] = t.data_ptr();
+        }
+        if (type < 0) raise(PyExc_ValueError, "PagedCache: keys or values or both");
+        State &st = state_of(module);
+        const Library &lib = library(st);
+        const saetta_stream_t s = stream_of(a[4]);
+        const int32_t *at = pointer<int32_t>(slots);
+        const uint32_t tokens = uint32_t(slots.numel());
+        return call("paged_gather", st, [&] { return lib.paged_gather(s, type, cache, at, to[0], to[1], tokens); });
+    });
+}
+
+// paged_split(batch, params, split, stream)
+PyObject *paged_split(PyObject *module, PyObject *const *a, Py_ssize_t n) {
+    return guarded(n, 4, "paged_split", [&] {
+        const saetta_paged_batch batch = paged_batch(a[0]);
+        const saetta_paged_attn_params p = paged_params(a[1]);
+        if (PyErr_Occurred()) throw Raised{};
+        void *split = here(a[2], at::kByte, "paged attention").data_ptr();
+        State &st = state_of(module);
+        const Library &lib = library(st);
+        const saetta_stream_t s = stream_of(a[3]);
+        return call("paged_split", st, [&] { return lib.paged_split(s, batch, p, split); });
+    });
+}
+
+// paged_attn(q, gate or None, out, cache, batch, params, split, workspace, stream)
+PyObject *paged_attn(PyObject *module, PyObject *const *a, Py_ssize_t n) {
+    return guarded(n, 9, "paged_attn", [&] {
+        const saetta_paged_cache cache = paged_cache(a[3]);
+        const saetta_paged_batch batch = paged_batch(a[4]);
+        const saetta_paged_attn_params p = paged_params(a[5]);
+        if (PyErr_Occurred()) throw Raised{};
+        const Rows q = rows_of(a[0], p.heads, false, "q"), out = rows_of(a[2], p.heads, false, "out");
+        Rows gate{{nullptr, 0, 0}, q.tokens, q.type};
+        if (a[1] != Py_None) gate = rows_of(a[1], p.heads, false, "gate");
+        for (const Rows *r : {&q, static_cast<const Rows *>(&gate), &out})
+            if (r->type != q.type || r->tokens < p.tokens) raise(PyExc_ValueError, "paged attention: q, gate and out must be of one type and of %u tokens", p.tokens);
+        if ((out.tokens > 1 && out.rows.token_stride == 0) || (p.heads > 1 && out.rows.head_stride == 0))
+            raise(PyExc_ValueError, "paged attention: out's rows must lie apart");
+        void *split = here(a[6], at::kByte, "paged attention").data_ptr();
+        const at::Tensor &ws = here(a[7], at::kByte, "paged attention");
+        void *workspace = ws.data_ptr();
+        const size_t bytes = size_t(ws.numel());
+        State &st = state_of(module);
+        const Library &lib = library(st);
+        const saetta_stream_t s = stream_of(a[8]);
+        return call("paged_attn", st, [&] { return lib.paged_attn(s, q.type, q.rows, cache, batch, split, gate.rows, out.rows, p, workspace, bytes); });
+    });
+}
+
 #define FUNCTION(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(name)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {FUNCTION(setup), FUNCTION(to_half), FUNCTION(kv_encode), FUNCTION(prefill), FUNCTION(prefill_quant),
-                           FUNCTION(token_params_set), FUNCTION(plan_run), {nullptr, nullptr, 0, nullptr}};
+                           FUNCTION(token_params_set), FUNCTION(plan_run), FUNCTION(paged_tables), FUNCTION(paged_store), FUNCTION(paged_gather),
+                           FUNCTION(paged_split), FUNCTION(paged_attn), {nullptr, nullptr, 0, nullptr}};
 #undef FUNCTION
 
 int traverse(PyObject *module, visitproc visit, void *arg) {

@@ -50,7 +50,7 @@ struct alignas(16) Item {
     uint32_t part, parts;            // of the tile's keys; parts 0: nothing to do.  The parts of a tile are items side by side
 };
 struct alignas(16) SplitHead {
-    uint32_t items, tiles;  // items dealt out; tiles in parts (their first items, behind the items)
+    uint32_t items, tiles;  // items dealt out; tiles in parts: their first items once more, `part` the place among the items
     uint32_t unused[2];
 };
 
@@ -75,9 +75,8 @@ Shape shape_of(const saetta_paged_attn_params &p, uint32_t requests) {
 struct SplitArgs {
     saetta_paged_batch batch;
     SplitHead *head;
-    Item *items;
-    uint32_t *tiles;
-    uint32_t tile_tokens, target, most_items, tokens, rows;
+    Item *items, *tiles;
+    uint32_t tile_tokens, target, most_items, most_joined, tokens, rows;
     uint32_t few, granule;
 };
 
@@ -207,13 +206,14 @@ __global__ __launch_bounds__(SPLIT_THREADS) void paged_split_kernel(SplitArgs a)
             a.items[where] = item;
             if (item.part == 0 && item.parts > 1) {
                 const uint32_t t = atomicAdd(&tiles_there, 1u);  // (their order does not matter: each is joined by itself)
-                a.tiles[t] = where;
+                item.part = where;
+                if (t < a.most_joined) a.tiles[t] = item;
             }
         }
         before += all;
         __syncthreads();
     }
-    if (tid == 0) *a.head = {min(before, a.most_items), tiles_there, {0, 0}};
+    if (tid == 0) *a.head = {min(before, a.most_items), min(tiles_there, a.most_joined), {0, 0}};
 }
 
 // ---- the attention kernels ----------------------------------------------------------------------------------------
@@ -656,29 +656,53 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
     if (item.parts > 1 && hf == 0) *reinterpret_cast<float2 *>(a.part_ml + slot * 2) = float2{m, l};
 }
 
-// Joins the parts of the tiles that were taken in parts: out = sum_p 2^(M_p - M) O_p / sum_p 2^(M_p - M) l_p.  A wave a row, a
-// lane four dims; where rows are few, the four waves of a workgroup take a row's parts by turns and join through LDS.
+// Joins the parts of the tiles that were taken in parts: out = sum_p 2^(M_p - M) O_p / sum_p 2^(M_p - M) l_p.  A lane has four
+// dims of a row.  Latency: the tile, then maxima, sums, parts and gate at once, then the output.  Few rows: a workgroup a row, the parts dealt to
+// its four waves in turn.  Chunks: a wave a row.  (Joining in the attention kernel, by the workgroup that ends last, costs more than this launch:
+// all workgroups run at once, so their stores' way to the memory that the XCDs share, the count and the loads come on top of the longest walk;
+// 48 ragged contexts 67 -> 72 us, one of 517 tokens 9.3 -> 9.7.)
 template <int TYPE, bool FEW>
-__global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, const uint32_t *tiles) {
-    if (blockIdx.x >= a.head->tiles) return;
-    const uint32_t index = tiles[blockIdx.x], kv = blockIdx.z;
-    if (index >= a.target) return;
-    const Item item = a.items[index];
-    if (!item_ok(a, item, index) || item.parts > a.target - index) return;
-    constexpr uint32_t TILE = FEW ? FEW_ROWS : CHUNK_ROWS;
+__global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, const Item *tiles) {
+    typedef typename Row<TYPE>::value V;
+    constexpr uint32_t TILE = FEW ? FEW_ROWS : CHUNK_ROWS, BY = FEW ? 4 : 1;
+    const uint32_t there = a.head->tiles, kv = blockIdx.z;
+    Item item = tiles[blockIdx.x];
+    const uint32_t index = item.part;
+    item.part = 0;
+    if (!(int(blockIdx.x < there) & int(index < a.target) & int(item_ok(a, item, index)) & int(item.parts <= a.target - min(index, a.target)))) return;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t r = FEW ? blockIdx.y : blockIdx.y * 4 + wave, rows = item.tokens << a.group_shift;
-    if (r >= rows) return;  // (FEW: the whole workgroup)
+    const uint32_t r = FEW ? blockIdx.y : blockIdx.y * 4 + wave;
+    if (r >= item.tokens << a.group_shift) return;  // (FEW: the whole workgroup)
     const size_t stride = size_t(a.cache.kv_heads) * TILE, slot = (size_t(index) * a.cache.kv_heads + kv) * TILE + r;
+    const uint64_t row = uint64_t(item.row0) + (r >> a.group_shift);
+    const uint32_t head = kv * a.group + (r & (a.group - 1)), dim = lane * 4;
+    float gate[4];
+    if (a.gate.data) load_values<TYPE, 4>(static_cast<const V *>(a.gate.data) + row * a.gate.token_stride + head * a.gate.head_stride + dim, gate);
+
     float m = NO_MAXIMUM, l = 0.0f;
     floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t p = FEW ? wave : 0; p < item.parts; p += FEW ? 4 : 1) {
-        const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + (slot + p * stride) * 2);
-        const floatx4 x = *reinterpret_cast<const floatx4 *>(a.part_o + (slot + p * stride) * DIM + lane * 4);
-        const float next = fmaxf(m, ml.x), f = __builtin_amdgcn_exp2f(m - next), g = __builtin_amdgcn_exp2f(ml.x - next);
-        m = next, l = l * f + ml.y * g;
+    for (uint32_t p0 = FEW ? wave : 0; p0 < item.parts; p0 += BY * 8) {
+        float2 ml[8];
+        floatx4 x[8];
 #pragma unroll
-        for (int i = 0; i < 4; i++) o[i] = o[i] * f + x[i] * g;
+        for (uint32_t i = 0; i < 8; i++) {
+            const size_t at = slot + min(p0 + i * BY, item.parts - 1) * stride;
+            ml[i] = *reinterpret_cast<const float2 *>(a.part_ml + at * 2);
+            x[i] = *reinterpret_cast<const floatx4 *>(a.part_o + at * DIM + dim);
+            if (p0 + i * BY >= item.parts) ml[i] = float2{NO_MAXIMUM, 0.0f}, x[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        float top = m;
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) top = fmaxf(top, ml[i].x);
+        const float down = __builtin_amdgcn_exp2f(m - top);
+        m = top, l *= down, o *= down;
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) {
+            const float f = __builtin_amdgcn_exp2f(ml[i].x - top);
+            l = fmaf(ml[i].y, f, l);
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[j] = fmaf(x[i][j], f, o[j]);
+        }
     }
     if constexpr (FEW) {
         __shared__ __attribute__((aligned(16))) float part[4][64][4];
@@ -694,17 +718,17 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, const uint
 #pragma unroll
         for (int w = 0; w < 4; w++) {
             const float f = __builtin_amdgcn_exp2f(pml[w][0] - top);
-            l += pml[w][1] * f;
+            l = fmaf(pml[w][1], f, l);
             const floatx4 x = *reinterpret_cast<const floatx4 *>(part[w][lane]);
 #pragma unroll
-            for (int i = 0; i < 4; i++) o[i] += x[i] * f;
+            for (int i = 0; i < 4; i++) o[i] = fmaf(x[i], f, o[i]);
         }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     float x[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) x[i] = o[i] * inv;
-    put_row<TYPE>(a, uint64_t(item.row0) + (r >> a.group_shift), kv * a.group + (r & (a.group - 1)), lane * 4, x);
+    for (int i = 0; i < 4; i++) x[i] = a.gate.data ? o[i] * inv * sigmoid(gate[i]) : o[i] * inv;
+    store_values<TYPE, 4>(static_cast<V *>(a.out.data) + row * a.out.token_stride + head * a.out.head_stride + dim, x);
 }
 
 int check_attn(const saetta_paged_attn_params &p, uint32_t requests, const char *what) {
@@ -725,6 +749,8 @@ int check_batch(const saetta_paged_batch &b, const char *what) {
     SAETTA_REQUIRE(b.max_blocks > 0 && uint64_t(b.max_blocks) * b.block_tokens < (1ull << 31), SAETTA_E_SHAPE, "%s: rows of %u blocks", what, b.max_blocks);
     return SAETTA_OK;
 }
+// Tiles in parts that there can be: each has two at least, all among the first `target` items.
+uint32_t joined_tiles(const Shape &s) { return s.target / 2 < s.most_tiles ? s.target / 2 : s.most_tiles; }
 size_t items_offset() { return sizeof(SplitHead); }
 size_t tiles_offset(const Shape &s) { return items_offset() + sizeof(Item) * s.most_items; }
 
@@ -732,10 +758,9 @@ constexpr uint32_t CHUNK_LDS = 4 * PART_BYTES;
 uint32_t shift_of(uint32_t n) { return uint32_t(__builtin_ctz(n)); }
 
 template <int TYPE>
-void launch_attn(hipStream_t stream, const AttnArgs &a, const Shape &s, const saetta_paged_attn_params &p, const uint32_t *tiles) {
+void launch_attn(hipStream_t stream, const AttnArgs &a, const Shape &s, const saetta_paged_attn_params &p, const Item *tiles) {
     const dim3 grid(s.most_items * p.kv_heads);
-    // a tile in parts has two at least, and all of them are among the first `target` items
-    const uint32_t joined = s.target / 2 < s.most_tiles ? s.target / 2 : s.most_tiles;
+    const uint32_t joined = joined_tiles(s);
     if (s.tile_rows == FEW_ROWS) {
         launch(paged_few_kernel<TYPE>, grid, dim3(64 * FEW_WAVES), 0, stream, a);
         if (joined) launch(paged_merge_kernel<TYPE, true>, dim3(joined, p.rows * s.group, p.kv_heads), dim3(256), 0, stream, a, tiles);
@@ -762,7 +787,7 @@ using namespace saetta;
 extern "C" size_t saetta_paged_split_bytes(saetta_paged_attn_params p, uint32_t requests) {
     if (check_attn(p, requests, "paged_split_bytes")) return 0;
     const Shape s = shape_of(p, requests);
-    return tiles_offset(s) + 4 * size_t(s.most_items);
+    return tiles_offset(s) + sizeof(Item) * size_t(joined_tiles(s));
 }
 
 extern "C" size_t saetta_paged_workspace_bytes(saetta_paged_attn_params p, uint32_t requests) {
@@ -780,8 +805,8 @@ extern "C" int saetta_paged_split(saetta_stream_t stream, saetta_paged_batch bat
     const Shape s = shape_of(p, batch.requests);
     unsigned char *at = static_cast<unsigned char *>(split);
     const bool few = s.tile_rows == FEW_ROWS;
-    const SplitArgs a = {batch, reinterpret_cast<SplitHead *>(at), reinterpret_cast<Item *>(at + items_offset()), reinterpret_cast<uint32_t *>(at + tiles_offset(s)),
-                         s.tile_tokens, s.target, s.most_items, p.tokens, p.rows, few, few ? STEP_KEYS * FEW_WAVES : 256u};
+    const SplitArgs a = {batch, reinterpret_cast<SplitHead *>(at), reinterpret_cast<Item *>(at + items_offset()), reinterpret_cast<Item *>(at + tiles_offset(s)),
+                         s.tile_tokens, s.target, s.most_items, joined_tiles(s), p.tokens, p.rows, few, few ? STEP_KEYS * FEW_WAVES : 256u};
     launch(paged_split_kernel, dim3(1), dim3(SPLIT_THREADS), 0, as_stream(stream), a);
     return launch_status("paged_split");
 }
@@ -809,7 +834,7 @@ extern "C" int saetta_paged_attn(saetta_stream_t stream, int type, saetta_stride
     const AttnArgs a = {q, gate, out, cache, batch.block_table, reinterpret_cast<const SplitHead *>(at), reinterpret_cast<const Item *>(at + items_offset()),
                         part_o, part_o + size_t(s.target) * p.kv_heads * s.tile_rows * DIM, batch.requests, batch.max_blocks, p.tokens,
                         s.group, shift_of(s.group), shift_of(cache.block_tokens), s.target, s.tile_tokens, p.scale};
-    const uint32_t *tiles = reinterpret_cast<const uint32_t *>(at + tiles_offset(s));
+    const Item *tiles = reinterpret_cast<const Item *>(at + tiles_offset(s));
     if (type == SAETTA_F16) launch_attn<SAETTA_F16>(as_stream(stream), a, s, p, tiles);
     else launch_attn<SAETTA_BF16>(as_stream(stream), a, s, p, tiles);
     return launch_status("paged_attn");

@@ -626,14 +626,6 @@ _TYPES = {torch.float32: ffi.F32, torch.float16: ffi.F16, torch.bfloat16: ffi.BF
 _HALVES = (torch.float16, torch.bfloat16)
 
 
-def _here(what, *tensors):
-    """The tensors lie on the current device, which is where a call launches."""
-    device = torch._C._cuda_getDevice()
-    for t in tensors:
-        if t.get_device() != device:
-            raise ValueError(f"{what}: a tensor is on {t.device}, the current device is cuda:{device}")
-
-
 def _rows_of(t, heads, dtypes, what):
     """[tokens, heads, 256] with any strides that the library takes, as StridedRowsC."""
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes):
@@ -644,15 +636,6 @@ def _rows_of(t, heads, dtypes, what):
     return ffi.StridedRowsC(t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if heads > 1 else 0)
 
 
-def _do(plan, stream, kernel, name, what, args, keep):
-    """One call of the library, now on a stream or as an op of a plan."""
-    if plan is not None:
-        plan.op(kernel, _Call(name, what, args, keep))
-    else:
-        _here(what, *[t for t in keep if t is not None])
-        ffi.check(getattr(ffi.lib(), name)(_stream(stream), *args), what)
-
-
 class PagedCache:
     """The keys and values of one layer for several requests at once, in blocks of 16, 32, 64 or 128 tokens: 8-bit
     floating point codes (e4m3) with one power of two per block and kv head, for keys and for values.  The reference
@@ -661,11 +644,12 @@ class PagedCache:
     def __init__(self, kv_heads, head_dim, blocks, block_tokens=64, device="cuda"):
         if head_dim != DIM:
             raise ValueError("a paged cache is written for head dim 256")
-        if block_tokens not in (16, 32, 64, 128) or blocks < 1 or blocks * block_tokens >= 1 << 31:
+        if kv_heads < 1 or block_tokens not in (16, 32, 64, 128) or blocks < 1 or blocks * block_tokens >= 1 << 31:
             raise ValueError("PagedCache: blocks of 16, 32, 64 or 128 tokens, fewer than 2^31 in all")
         self.kv_heads, self.head_dim, self.blocks, self.block_tokens = kv_heads, head_dim, blocks, block_tokens
         self.keys, self.values = (torch.zeros(blocks, kv_heads, block_tokens * DIM, dtype=torch.uint8, device=device) for _ in range(2))
         self.key_scales, self.value_scales = (torch.full((blocks, kv_heads), 127 - 40, dtype=torch.uint8, device=device) for _ in range(2))
+        self._parts = (*self.tensors(), blocks, block_tokens, kv_heads)  # as the extension's calls take it
 
     def c(self):
         return ffi.PagedCacheC(self.keys.data_ptr(), self.values.data_ptr(), self.key_scales.data_ptr(),
@@ -677,42 +661,34 @@ class PagedCache:
     def bytes_per_token(self):
         return 2 * self.kv_heads * (DIM + 1 / self.block_tokens)
 
-    def _store(self, plan, stream, k, v, slots):
+    def record(self, plan, k, v, slots):
+        """The keys and values [tokens, kv_heads, 256] of a step's tokens into their slots; -1: nowhere."""
         rows = [_rows_of(t, self.kv_heads, tuple(_TYPES), what) for t, what in ((k, "PagedCache k"), (v, "PagedCache v"))]
         _need(slots, torch.int32, "PagedCache slots")
         if k.dtype is not v.dtype or k.shape[0] != v.shape[0] or slots.numel() != k.shape[0]:
             raise ValueError("PagedCache: k, v and slots must be of as many tokens, k and v of one type")
-        _do(plan, stream, "paged_store", "saetta_paged_store", "paged_store",
-            (_TYPES[k.dtype], *rows, slots.data_ptr(), self.c(), slots.numel()), (k, v, slots, *self.tensors()))
-
-    def record(self, plan, k, v, slots):
-        """The keys and values [tokens, kv_heads, 256] of a step's tokens into their slots; -1: nowhere."""
-        self._store(plan, None, k, v, slots)
+        plan.op("paged_store", _Call("saetta_paged_store", "paged_store", (
+            _TYPES[k.dtype], *rows, _ptr(slots), self.c(), slots.numel()), (k, v, slots, *self.tensors())))
 
     def encode(self, k, v, slots, stream=None):
-        self._store(None, stream, k, v, slots)
-
-    def _gather(self, plan, stream, slots, keys, values):
-        _need(slots, torch.int32, "PagedCache slots")
-        outs = [t for t in (keys, values) if t is not None]
-        for t in outs:
-            if not (isinstance(t, torch.Tensor) and t.dtype in _TYPES):
-                raise TypeError("PagedCache: keys and values must be tensors of f32, f16 or bf16")
-            _need(t, t.dtype, "PagedCache keys and values")
-            if t.numel() < slots.numel() * self.kv_heads * DIM:
-                raise ValueError("PagedCache: keys and values do not hold the slots' rows")
-        if not outs or outs[0].dtype is not outs[-1].dtype:
-            raise ValueError("PagedCache: keys or values or both, of one type")
-        _do(plan, stream, "paged_gather", "saetta_paged_gather", "paged_gather",
-            (_TYPES[outs[0].dtype], self.c(), slots.data_ptr(), *[None if t is None else t.data_ptr() for t in (keys, values)],
-             slots.numel()), (slots, keys, values, *self.tensors()))
+        _calls.paged_store(k, v, slots, self._parts, _handle(stream))
 
     def record_dequantize(self, plan, slots, keys, values):
-        """What the slots hold, as contiguous [tokens, kv_heads, 256]; either of the two may be None."""
-        self._gather(plan, None, slots, keys, values)
+        """What the slots hold, as contiguous [tokens, kv_heads, 256] of f32, f16 or bf16; either of the two may be None."""
+        _need(slots, torch.int32, "PagedCache slots")
+        outs = [t for t in (keys, values) if t is not None]
+        if not outs or outs[0].dtype not in _TYPES:
+            raise ValueError("PagedCache: keys or values or both, of f32, f16 or bf16")
+        for t in outs:
+            _need(t, outs[0].dtype, "PagedCache keys and values")
+            if t.numel() < slots.numel() * self.kv_heads * DIM:
+                raise ValueError("PagedCache: keys and values do not hold the slots' rows")
+        plan.op("paged_gather", _Call("saetta_paged_gather", "paged_gather", (
+            _TYPES[outs[0].dtype], self.c(), _ptr(slots), *[None if t is None else _ptr(t) for t in (keys, values)], slots.numel()),
+            (slots, keys, values, *self.tensors())))
 
     def encode_dequantize(self, slots, keys, values, stream=None):
-        self._gather(None, stream, slots, keys, values)
+        _calls.paged_gather(slots, keys, values, self._parts, _handle(stream))
 
 
 class PagedTables:
@@ -734,6 +710,9 @@ class PagedTables:
         self.query_starts, self.kv_lens = torch.zeros(requests + 1, **ints), torch.zeros(requests, **ints)
         self.slots, self.positions = torch.full((tokens,), -1, **ints), torch.full((tokens,), -1, **ints)
         self.unplaced = torch.zeros(1, **ints)
+        # as the extension's calls take them
+        self._state, self._sizes = self.tensors(), (requests, max_blocks, block_tokens, blocks, tokens)
+        self._batch = (self.query_starts, self.kv_lens, self.block_table, requests, max_blocks, block_tokens)
 
     def tensors(self):
         return (self.block_table, self.held, self.free_list, self.free_count, self.query_starts, self.kv_lens, self.slots,
@@ -743,24 +722,20 @@ class PagedTables:
         return ffi.PagedBatchC(self.query_starts.data_ptr(), self.kv_lens.data_ptr(), self.block_table.data_ptr(), self.requests,
                                self.max_blocks, self.block_tokens)
 
-    def _tables(self, plan, stream, context_lens, new_lens):
+    def record(self, plan, context_lens, new_lens):
+        """A step of new_lens[r] tokens behind context_lens[r]: blocks taken or given back, slots, positions, query_starts,
+        kv_lens.  context_lens may be kv_lens: a recorded step then goes on from where the last one ended."""
         for t, what in ((context_lens, "context_lens"), (new_lens, "new_lens")):
             _need(t, torch.int32, f"PagedTables {what}")
             if t.numel() != self.requests:
                 raise ValueError(f"PagedTables: {what} must be of {self.requests} requests")
-        at = [t.data_ptr() for t in self.tensors()]
-        params = ffi.PagedTablesParamsC(self.requests, self.max_blocks, self.block_tokens, self.blocks, self.tokens)
-        _do(plan, stream, "paged_tables", "saetta_paged_tables", "paged_tables",
-            (context_lens.data_ptr(), new_lens.data_ptr(), ffi.PagedStateC(*at[:4]), ffi.PagedStepC(*at[4:]), params),
-            (context_lens, new_lens, *self.tensors()))
-
-    def record(self, plan, context_lens, new_lens):
-        """A step of new_lens[r] tokens behind context_lens[r]: blocks taken or given back, slots, positions, query_starts,
-        kv_lens.  context_lens may be kv_lens: a recorded step then goes on from where the last one ended."""
-        self._tables(plan, None, context_lens, new_lens)
+        at = [_ptr(t) for t in self.tensors()]
+        plan.op("paged_tables", _Call("saetta_paged_tables", "paged_tables", (
+            _ptr(context_lens), _ptr(new_lens), ffi.PagedStateC(*at[:4]), ffi.PagedStepC(*at[4:]), ffi.PagedTablesParamsC(*self._sizes)),
+            (context_lens, new_lens, *self.tensors())))
 
     def encode(self, context_lens, new_lens, stream=None):
-        self._tables(None, stream, context_lens, new_lens)
+        _calls.paged_tables(context_lens, new_lens, self._state, self._sizes, _handle(stream))
 
 
 class PagedAttention:
@@ -777,9 +752,9 @@ class PagedAttention:
             raise ValueError("paged attention: rows of one at least")
         self.heads, self.kv_heads, self.rows = heads, kv_heads, rows
         self.shape = (tables.requests, tables.tokens, tables.max_blocks, tables.block_tokens)
-        self.scale = 1.0 / math.sqrt(DIM)
+        self._params = (heads, kv_heads, tables.tokens, rows, 1.0 / math.sqrt(DIM))
         device = tables.block_table.device if device is None else device
-        l, p = ffi.lib(), self._params()
+        l, p = ffi.lib(), ffi.PagedAttnParamsC(*self._params)
         with torch.cuda.device(device):  # (the sizes are of the device's compute units)
             split, workspace = l.saetta_paged_split_bytes(p, tables.requests), l.saetta_paged_workspace_bytes(p, tables.requests)
         if not split or not workspace:
@@ -787,48 +762,42 @@ class PagedAttention:
         self.split = torch.empty(split, dtype=torch.uint8, device=device)
         self.workspace = torch.empty(workspace, dtype=torch.uint8, device=device)
 
-    def _params(self):
-        return ffi.PagedAttnParamsC(self.heads, self.kv_heads, self.shape[1], self.rows, self.scale)
-
-    def _check(self, tables):
+    def _check(self, tables, cache=None):
         if (tables.requests, tables.tokens, tables.max_blocks, tables.block_tokens) != self.shape:
             raise ValueError("paged attention: made for tables of another size")
-
-    def _split(self, plan, stream, tables):
-        self._check(tables)
-        _do(plan, stream, "paged_split", "saetta_paged_split", "paged_split", (tables.batch(), self._params(), self.split.data_ptr()),
-            (self.split, tables.query_starts, tables.kv_lens, tables.block_table))
+        if cache is not None and (cache.kv_heads, cache.block_tokens) != (self.kv_heads, tables.block_tokens):
+            raise ValueError("paged attention: a cache of other kv heads or blocks")
 
     def record_split(self, plan, tables):
         """Deals a step's rows and keys out, once for all layers: behind the tables, before the first layer's attention."""
-        self._split(plan, None, tables)
+        self._check(tables)
+        plan.op("paged_split", _Call("saetta_paged_split", "paged_split", (
+            tables.batch(), ffi.PagedAttnParamsC(*self._params), _ptr(self.split)),
+            (self.split, tables.query_starts, tables.kv_lens, tables.block_table)))
 
     def encode_split(self, tables, stream=None):
-        self._split(None, stream, tables)
-
-    def _attend(self, plan, stream, q, cache, tables, out, gate):
         self._check(tables)
-        if (cache.kv_heads, cache.block_tokens) != (self.kv_heads, tables.block_tokens):
-            raise ValueError("paged attention: a cache of other kv heads or blocks")
-        rows = [_rows_of(t, self.heads, _HALVES, what) for t, what in ((q, "q"), (out, "out"))]
-        gate_rows = ffi.StridedRowsC(None, 0, 0) if gate is None else _rows_of(gate, self.heads, _HALVES, "gate")
-        for t, what in ((q, "q"), (out, "out"), (gate, "gate")):
-            if t is not None and (t.dtype is not q.dtype or t.shape[0] < tables.tokens):
-                raise ValueError(f"paged attention: {what} must be of q's type and of {tables.tokens} tokens")
-        if 0 in (out.stride(0) if out.shape[0] > 1 else 1, out.stride(1) if self.heads > 1 else 1):
-            raise ValueError("paged attention: out's rows must lie apart")
-        _do(plan, stream, "paged_attention", "saetta_paged_attn", "paged_attn",
-            (_TYPES[q.dtype], rows[0], cache.c(), tables.batch(), self.split.data_ptr(), gate_rows, rows[1], self._params(),
-             self.workspace.data_ptr(), self.workspace.numel()),
-            (q, out, gate, *cache.tensors(), tables.query_starts, tables.kv_lens, tables.block_table, self.split, self.workspace))
+        _calls.paged_split(tables._batch, self._params, self.split, _handle(stream))
 
     def record(self, plan, q, cache, tables, out, gate=None):
         """q, out and gate [tokens, heads, 256] in f16 or bf16, any strides of multiples of 16 bytes: the halves of a projection's
         output as they are.  Rows past the step's last token are left as they were."""
-        self._attend(plan, None, q, cache, tables, out, gate)
+        self._check(tables, cache)
+        rows = [_rows_of(t, self.heads, _HALVES, what) for t, what in ((q, "q"), (out, "out"))]
+        gate_rows = ffi.StridedRowsC(None, 0, 0) if gate is None else _rows_of(gate, self.heads, _HALVES, "gate")
+        for t in (q, out, gate):
+            if t is not None and (t.dtype is not q.dtype or t.shape[0] < tables.tokens):
+                raise ValueError(f"paged attention: q, gate and out must be of one type and of {tables.tokens} tokens")
+        if (out.shape[0] > 1 and out.stride(0) == 0) or (self.heads > 1 and out.stride(1) == 0):
+            raise ValueError("paged attention: out's rows must lie apart")
+        plan.op("paged_attention", _Call("saetta_paged_attn", "paged_attn", (
+            _TYPES[q.dtype], rows[0], cache.c(), tables.batch(), _ptr(self.split), gate_rows, rows[1], ffi.PagedAttnParamsC(*self._params),
+            _ptr(self.workspace), self.workspace.numel()),
+            (q, out, gate, *cache.tensors(), tables.query_starts, tables.kv_lens, tables.block_table, self.split, self.workspace)))
 
     def encode(self, q, cache, tables, out, gate=None, stream=None):
-        self._attend(None, stream, q, cache, tables, out, gate)
+        self._check(tables, cache)
+        _calls.paged_attn(q, gate, out, cache._parts, tables._batch, self._params, self.split, self.workspace, _handle(stream))
 
 
 class RowBackup:
