@@ -33,6 +33,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int DIM = SAETTA_HEAD_DIM;
+#include "prefill_stream.hpp"  // scores_block, stream_block_alone, settle
 constexpr float NO_SCORE = -1e30f;               // of a key that a row does not see
 constexpr float NO_MAXIMUM = 0.25f * NO_SCORE;   // where nothing was seen: 2^(NO_SCORE - NO_MAXIMUM) is 0
 constexpr float TAU = 8.0f;                      // the reference maximum is raised only past this many powers of two
@@ -47,28 +48,32 @@ struct alignas(16) Item {
     uint32_t request, row0, tokens;  // rows of q from row0 on
     int32_t pos0;                    // position of the first of them
     uint32_t key0, key1;             // keys that are taken (up to what the last row sees)
-    uint32_t part, parts;            // of the tile's keys; parts 0: nothing to do.  The parts of a tile are items side by side
+    uint32_t slot;                   // where its sums go, if the tile's keys are taken in parts; of a tile in parts, its first part's
+    uint32_t parts;                  // of the tile
 };
 struct alignas(16) SplitHead {
-    uint32_t items, tiles;  // items dealt out; tiles in parts: their first items once more, `part` the place among the items
+    uint32_t items, tiles;  // items dealt out; tiles in parts, which are joined afterwards
     uint32_t unused[2];
 };
 
 struct Shape {
     uint32_t group, tile_tokens, tile_rows;
-    uint32_t target;  // items that fill the device
-    uint32_t most_items, most_tiles;
+    uint32_t target;  // items that the device takes at once
+    uint32_t most_items, most_tiles, most_joined, slots;
 };
 Shape shape_of(const saetta_paged_attn_params &p, uint32_t requests) {
     Shape s;
     s.group = p.heads / p.kv_heads;
     const bool few = uint64_t(p.rows) * s.group <= FEW_ROWS;
     s.tile_rows = few ? FEW_ROWS : CHUNK_ROWS;
-    s.tile_tokens = few ? (p.rows ? p.rows : 1) : CHUNK_ROWS / s.group;
+    s.tile_tokens = few ? p.rows : CHUNK_ROWS / s.group;
     const uint32_t workgroups = cu_count() * (few ? 2 : 1);
     s.target = workgroups / p.kv_heads ? workgroups / p.kv_heads : 1;
     s.most_tiles = few ? requests : p.tokens / s.tile_tokens + requests;
-    s.most_items = s.most_tiles > s.target ? s.most_tiles : s.target;
+    // With parts of total / target no more than `target` tiles have more than one, and their parts are 2 * target at most
+    s.most_items = s.most_tiles + s.target;
+    s.most_joined = s.target < s.most_tiles ? s.target : s.most_tiles;
+    s.slots = 2 * s.target;
     return s;
 }
 
@@ -76,144 +81,141 @@ struct SplitArgs {
     saetta_paged_batch batch;
     SplitHead *head;
     Item *items, *tiles;
-    uint32_t tile_tokens, target, most_items, most_joined, tokens, rows;
-    uint32_t few, granule;
+    uint32_t tile_tokens, target, most_items, most_joined, slots, tokens, rows;
+    uint32_t few, granule, least, half_tokens;
 };
 
 constexpr int SPLIT_THREADS = 1024, SPLIT_WAVES = SPLIT_THREADS / 64;
-constexpr uint32_t SPLIT_HELD = 1024;  // requests whose tiles and keys are kept in LDS
-
-__device__ __forceinline__ uint32_t wave_sum(uint32_t x) {
-#pragma unroll
-    for (int d = 32; d > 0; d /= 2) x += __shfl_xor(x, d);
-    return x;
-}
-__device__ __forceinline__ uint64_t wave_sum(uint64_t x) {
-#pragma unroll
-    for (int d = 32; d > 0; d /= 2) x += __shfl_xor(x, d);
-    return x;
-}
+constexpr uint32_t SIZES = 64;  // classes of items by what they cost
 
 // A request as the split sees it.
 struct Work {
-    uint32_t row0, tokens, tiles, keys;  // keys: what its last row sees, in whole rows of the table
+    uint32_t row0, tokens, tiles;
     int32_t pos0;
 };
 __device__ __forceinline__ Work work_of(const SplitArgs &a, uint32_t r) {
-    Work w = {0, 0, 0, 0, 0};
+    Work w = {0, 0, 0, 0};
     if (r >= a.batch.requests) return w;
     const uint32_t start = min(a.batch.query_starts[r], a.tokens), end = min(a.batch.query_starts[r + 1], a.tokens);
     const uint32_t n = end > start ? end - start : 0;
-    const uint32_t length = min(a.batch.kv_lens[r], 0x7fffffffu);
     w.row0 = start, w.tokens = a.few ? min(n, a.rows) : n;
-    w.pos0 = int32_t(length) - int32_t(n);
+    w.pos0 = int32_t(min(a.batch.kv_lens[r], 0x7fffffffu)) - int32_t(n);
     w.tiles = (w.tokens + a.tile_tokens - 1) / a.tile_tokens;
-    w.keys = min(uint32_t(max(w.pos0 + int32_t(w.tokens), 0)), a.batch.max_blocks * a.batch.block_tokens);
     return w;
 }
-__device__ __forceinline__ uint32_t parts_of(uint32_t keys, uint32_t length) { return keys > length ? (keys + length - 1) / length : 1; }
+// Tile `tile` of it, whole.
+__device__ __forceinline__ Item tile_of(const SplitArgs &a, const Work &w, uint32_t r, uint32_t tile) {
+    Item item;
+    const uint32_t first = tile * a.tile_tokens;
+    item.request = r, item.row0 = w.row0 + first, item.tokens = min(a.tile_tokens, w.tokens - first);
+    item.pos0 = w.pos0 + int32_t(first);
+    item.key0 = 0, item.key1 = min(uint32_t(max(item.pos0 + int32_t(item.tokens), 0)), a.batch.max_blocks * a.batch.block_tokens);
+    item.slot = 0, item.parts = 1;
+    return item;
+}
 
-// The keys of every tile in parts of at most `length`, the least length (in granules) for which there are at most `target` items; with as
-// many tiles as that, whole.  A request's parts are then made equal.  For a length p the items are between total / p and total / p + tiles,
-// which leaves few lengths to try: one wave bisects them, without barriers.
+// Deals the work out so that the workgroups that run at once end together.  What a key of a tile costs is one of two numbers: a chunk's tile of
+// at most half the rows keeps half the waves and takes 5 / 8 of the time.  A tile that costs more than total / target is cut into parts of that
+// and a rest; the items go out from the dearest class to the cheapest, so that who ends early takes what is small.  (One workgroup: a sum over the
+// tiles, a count of the classes, and the items themselves; the tiles by turns over its threads.  The places of the items in a class and of the
+// parts' sums follow from atomic counts, in any order: what is computed does not depend on them.)
 __global__ __launch_bounds__(SPLIT_THREADS) void paged_split_kernel(SplitArgs a) {
-    __shared__ uint32_t waves[SPLIT_WAVES], starts[SPLIT_THREADS], tiles_there, chosen;
-    __shared__ uint2 held[SPLIT_HELD];  // tiles, keys
+    __shared__ uint32_t waves[SPLIT_WAVES], starts[SPLIT_THREADS], classes[SIZES], slots_there, tiles_there;
+    __shared__ unsigned long long total;
     const uint32_t tid = threadIdx.x, requests = a.batch.requests;
-    for (uint32_t r = tid; r < min(requests, SPLIT_HELD); r += SPLIT_THREADS) {
-        const Work w = work_of(a, r);
-        held[r] = uint2{w.tiles, w.keys};
-    }
-    __syncthreads();
-    if (tid < 64) {
-        auto shape = [&](uint32_t r) {
-            if (r < SPLIT_HELD) return held[r];
-            const Work w = work_of(a, r);
-            return uint2{w.tiles, w.keys};
-        };
-        uint32_t tiles = 0, longest = 0;
-        uint64_t total = 0;
-        for (uint32_t r = tid; r < requests; r += 64) {
-            const uint2 w = shape(r);
-            tiles += w.x, longest = max(longest, w.y), total += uint64_t(w.x) * w.y;
-        }
-        tiles = wave_sum(tiles), total = wave_sum(total);
+    if (tid < SIZES) classes[tid] = 0;
+    if (tid == 0) slots_there = tiles_there = 0, total = 0;
+
+    // f(tile) for every tile; a call for each of the passes
+    bool found = false;
+    uint32_t found_tiles = 0;
+    auto for_tiles = [&](auto f) {
+        for (uint32_t r0 = 0; r0 < requests; r0 += SPLIT_THREADS) {
+            if (!found) {  // (one round of requests: the same starts in every pass)
+                const uint32_t tiles = work_of(a, r0 + tid).tiles;
+                uint32_t through = tiles;
 #pragma unroll
-        for (int d = 32; d > 0; d /= 2) longest = max(longest, uint32_t(__shfl_xor(longest, d)));
-        uint32_t high = max((longest + a.granule - 1) / a.granule, 1u);  // in granules: a length that will do
-        if (tiles < a.target) {
-            const uint64_t enough = total / (uint64_t(a.target - tiles) * a.granule) + 1, least = total / (uint64_t(a.target) * a.granule);
-            high = uint32_t(min(uint64_t(high), enough));
-            uint32_t low = uint32_t(max(min(least, uint64_t(high)), uint64_t(1)));
-            while (low < high) {
-                const uint32_t mid = (low + high) / 2;
-                uint32_t items = 0;  // (tiles * parts: with so few tiles no more than some thousands)
-                for (uint32_t r = tid; r < requests; r += 64) {
-                    const uint2 w = shape(r);
-                    items += w.x * parts_of(w.y, mid * a.granule);
+                for (int d = 1; d < 64; d *= 2) {
+                    const uint32_t other = __shfl_up(through, d);
+                    if ((tid & 63) >= uint32_t(d)) through += other;
                 }
-                if (wave_sum(items) <= a.target) high = mid;
-                else low = mid + 1;
+                __syncthreads();
+                if ((tid & 63) == 63) waves[tid >> 6] = through;
+                __syncthreads();
+                uint32_t base = 0, all = 0;
+#pragma unroll
+                for (uint32_t w = 0; w < SPLIT_WAVES; w++) {
+                    if (w < (tid >> 6)) base += waves[w];
+                    all += waves[w];
+                }
+                starts[tid] = base + through - tiles;
+                __syncthreads();
+                found = requests <= SPLIT_THREADS, found_tiles = all;
+            }
+            const uint32_t n = min(uint32_t(SPLIT_THREADS), requests - r0);
+            for (uint32_t k = tid; k < found_tiles; k += SPLIT_THREADS) {
+                uint32_t i = 0, left = n;  // the last request whose tiles start at k or before
+                while (left > 1) {
+                    const uint32_t half = left / 2;
+                    if (starts[i + half] <= k) i += half, left -= half;
+                    else left = half;
+                }
+                f(tile_of(a, work_of(a, r0 + i), r0 + i, k - starts[i]));
             }
         }
-        if (tid == 0) chosen = high, tiles_there = 0;
-    }
-    __syncthreads();
-    const uint32_t length = chosen * a.granule;
+    };
+    auto price = [&](const Item &tile) { return tile.tokens <= a.half_tokens ? 5u : 8u; };
 
-    uint32_t before = 0;
-    for (uint32_t r0 = 0; r0 < requests; r0 += SPLIT_THREADS) {
-        const Work mine = work_of(a, r0 + tid);
-        const uint32_t items = mine.tiles * parts_of(mine.keys, length);
-        // prefix sum over the workgroup
-        uint32_t through = items;
+    unsigned long long sum = 0;
+    for_tiles([&](const Item &tile) { sum += static_cast<unsigned long long>(tile.key1) * price(tile); });
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) sum += __shfl_xor(sum, d);
+    if ((tid & 63) == 0 && sum) atomicAdd(&total, sum);
+    __syncthreads();
+    // what a part costs at most, and its keys
+    const unsigned long long fair = max(total / a.target + 1, static_cast<unsigned long long>(a.least) * 8);
+    auto length_of = [&](const Item &tile) {
+        const unsigned long long keys = fair / price(tile) + a.granule;
+        return uint32_t(keys > 0x7fffffffu ? 0x7fffffffu : keys) / a.granule * a.granule;
+    };
+    const unsigned long long dearest = fair + 8ull * a.granule;
+    auto class_of = [&](uint32_t keys, uint32_t price) { return SIZES - 1 - uint32_t(min(static_cast<unsigned long long>(keys) * price * SIZES / dearest, SIZES - 1ull)); };
+    for_tiles([&](const Item &tile) {
+        const uint32_t length = length_of(tile), whole = tile.key1 / length, rest = tile.key1 - whole * length;
+        if (whole) atomicAdd(&classes[class_of(length, price(tile))], whole);
+        if (rest || !whole) atomicAdd(&classes[class_of(rest, price(tile))], 1u);
+    });
+    __syncthreads();
+    if (tid < 64) {  // where each class begins
+        static_assert(SIZES == 64, "a lane a class");
+        const uint32_t n = classes[tid];
+        uint32_t through = n;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
             const uint32_t other = __shfl_up(through, d);
-            if ((tid & 63) >= uint32_t(d)) through += other;
+            if (tid >= uint32_t(d)) through += other;
         }
-        if ((tid & 63) == 63) waves[tid >> 6] = through;
-        __syncthreads();
-        uint32_t base = 0, all = 0;
-#pragma unroll
-        for (uint32_t w = 0; w < SPLIT_WAVES; w++) {
-            if (w < (tid >> 6)) base += waves[w];
-            all += waves[w];
-        }
-        starts[tid] = base + through - items;
-        __syncthreads();
-        for (uint32_t k = tid; k < all; k += SPLIT_THREADS) {
-            uint32_t i = 0, n = SPLIT_THREADS;  // the last request whose items start at k or before
-            while (n > 1) {
-                const uint32_t half = n / 2;
-                if (starts[i + half] <= k) i += half, n -= half;
-                else n = half;
-            }
-            const Work w = work_of(a, r0 + i);
-            const uint32_t parts = parts_of(w.keys, length), at = k - starts[i];
-            const uint32_t even = (w.keys + parts - 1) / parts, each = max((even + a.granule - 1) / a.granule * a.granule, a.granule);
-            const uint32_t tile = w.tiles - 1 - at / parts;  // the tiles with the most keys first
-            Item item;
-            item.request = r0 + i, item.part = at % parts;
-            item.row0 = w.row0 + tile * a.tile_tokens, item.tokens = min(a.tile_tokens, w.tokens - tile * a.tile_tokens);
-            item.pos0 = w.pos0 + int32_t(tile * a.tile_tokens);
-            const uint32_t keys = min(uint32_t(max(item.pos0 + int32_t(item.tokens), 0)), w.keys);
-            item.parts = parts_of(keys, each);
-            item.key0 = item.part * each, item.key1 = min(item.key0 + each, keys);
-            if (item.part >= item.parts) item.parts = 0;
-            const uint32_t where = before + k;
-            if (where >= a.most_items) continue;  // (never: most_items has room for every split that this makes)
-            a.items[where] = item;
-            if (item.part == 0 && item.parts > 1) {
-                const uint32_t t = atomicAdd(&tiles_there, 1u);  // (their order does not matter: each is joined by itself)
-                item.part = where;
-                if (t < a.most_joined) a.tiles[t] = item;
-            }
-        }
-        before += all;
-        __syncthreads();
+        classes[tid] = through - n;
+        if (tid == 63) a.head->items = min(through, a.most_items);
     }
-    if (tid == 0) *a.head = {min(before, a.most_items), min(tiles_there, a.most_joined), {0, 0}};
+    __syncthreads();
+    for_tiles([&](Item tile) {
+        const uint32_t length = length_of(tile), end = tile.key1;
+        tile.parts = end > length ? (end + length - 1) / length : 1;
+        if (tile.parts > 1) {
+            tile.slot = atomicAdd(&slots_there, tile.parts);
+            const uint32_t t = atomicAdd(&tiles_there, 1u);
+            if (t < a.most_joined) a.tiles[t] = tile;
+        }
+        for (uint32_t p = 0; p < tile.parts; p++) {
+            Item item = tile;
+            item.key0 = p * length, item.key1 = min(end, item.key0 + length), item.slot = tile.slot + p;
+            const uint32_t where = atomicAdd(&classes[class_of(item.key1 - item.key0, price(tile))], 1u);
+            if (where < a.most_items) a.items[where] = item;
+        }
+    });
+    __syncthreads();
+    if (tid == 0) a.head->tiles = min(tiles_there, a.most_joined);
 }
 
 // ---- the attention kernels ----------------------------------------------------------------------------------------
@@ -224,9 +226,9 @@ struct AttnArgs {
     const int32_t *block_table;
     const SplitHead *head;
     const Item *items;
-    float *part_o;   // [item][kv head][tile rows][256], relative to M
-    float *part_ml;  // [item][kv head][tile rows][M, sum]
-    uint32_t requests, max_blocks, tokens, group, group_shift, block_shift, target, tile_tokens;
+    float *part_o;   // [slot][kv head][tile rows][256], relative to M
+    float *part_ml;  // [slot][kv head][tile rows][M, sum]
+    uint32_t requests, max_blocks, tokens, group, group_shift, block_shift, slots, tile_tokens;
     float scale;
 };
 
@@ -268,27 +270,29 @@ struct Unit {
     uint32_t block;     // row of [blocks][kv_heads]; of the first block where there is none
     uint32_t scales;    // 127 + ek | (127 + ev) << 8 | there << 16
 };
-constexpr uint32_t WINDOW = 512;  // units whose places a workgroup keeps in LDS
-
-__device__ __forceinline__ void find_units(const AttnArgs &a, Unit *units, uint32_t request, uint32_t head, uint32_t first, uint32_t end, uint32_t threads) {
+// Units that a workgroup keeps in LDS: unit u at u % WINDOW.  Units from `first` on, `count` of them; from `end` on there are none.
+constexpr uint32_t WINDOW = 512;
+__device__ __forceinline__ void find_units(const AttnArgs &a, Unit *units, uint32_t request, uint32_t head, uint32_t first, uint32_t count, uint32_t end) {
     const uint32_t shift = a.block_shift - 4;
-    for (uint32_t u = threadIdx.x; u < WINDOW && first + u < end; u += threads) {
-        const uint32_t entry = (first + u) >> shift;
-        uint32_t block = entry < a.max_blocks ? uint32_t(a.block_table[size_t(request) * a.max_blocks + entry]) : ~0u;
+    for (uint32_t i = threadIdx.x; i < count; i += blockDim.x) {
+        const uint32_t u = first + i, entry = u >> shift;
+        uint32_t block = ~0u;
+        if (u < end && entry < a.max_blocks) block = uint32_t(a.block_table[size_t(request) * a.max_blocks + entry]);
         const bool there = block < a.cache.blocks;
-        if (!there) block = 0;
-        const uint32_t row = block * a.cache.kv_heads + head;
-        units[u] = {row, uint32_t(a.cache.key_scales[row]) | uint32_t(a.cache.value_scales[row]) << 8 | uint32_t(there) << 16};
+        const uint32_t row = (there ? block : 0) * a.cache.kv_heads + head;
+        units[u % WINDOW] = {row, uint32_t(a.cache.key_scales[row]) | uint32_t(a.cache.value_scales[row]) << 8 | uint32_t(there) << 16};
     }
 }
 // (exponents as the store writes them: what else a byte says would make scores no numbers)
 __device__ __forceinline__ float key_scale(uint32_t scales) { return power_of_two(min(max(int(scales & 0xff) - 127, LOWEST_EXPONENT), HIGHEST_EXPONENT)); }
 __device__ __forceinline__ int value_exponent(uint32_t scales) { return min(max(int(scales >> 8 & 0xff) - 127, LOWEST_EXPONENT), HIGHEST_EXPONENT); }
 
-// An item that the split has made for these buffers.  (A split of other parameters is not followed out of them.)
-__device__ __forceinline__ bool item_ok(const AttnArgs &a, const Item &item, uint32_t index) {
-    return item.parts > 0 && item.request < a.requests && item.tokens > 0 && item.tokens <= a.tile_tokens && item.row0 <= a.tokens && item.tokens <= a.tokens - item.row0 &&
-           item.part < item.parts && (item.parts == 1 || index < a.target) && item.key1 <= a.max_blocks << a.block_shift;
+// An item that the split has made for these buffers.  (A split of other parameters is not followed out of them.)  (No branches: the
+// loads go out together.)
+__device__ __forceinline__ bool item_ok(const AttnArgs &a, const Item &item, uint32_t slots) {
+    return int(item.request < a.requests) & int(item.tokens > 0) & int(item.tokens <= a.tile_tokens) & int(item.row0 <= a.tokens) &
+           int(item.tokens <= a.tokens - min(item.row0, a.tokens)) & int(item.key1 <= a.max_blocks << a.block_shift) &
+           int((int(item.parts == 1) | (int(item.slot < a.slots) & int(slots <= a.slots - min(item.slot, a.slots)))) != 0);
 }
 
 // Bytes of a dword of four tokens' values that are NaN, as 0x80 in each.
@@ -338,7 +342,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(AttnArgs a
     const uint32_t index = blockIdx.x / a.cache.kv_heads, kv = blockIdx.x % a.cache.kv_heads;
     const uint32_t items = a.head->items;
     const Item item = a.items[index];
-    if (!(int(index < items) & int(item_ok(a, item, index)))) return;
+    if (!(int(index < items) & int(item_ok(a, item, 1)))) return;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t col = lane & 15, quarter = lane >> 4;
     const uint32_t rows = item.tokens << a.group_shift;  // of the tile that are there
@@ -492,7 +496,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(AttnArgs a
         for (int i = 0; i < 4; i++)
             if (nan_from[dim + i] != ~0u && int32_t(nan_from[dim + i]) < item.pos0 + int32_t(tok) + 1) o[i] = __builtin_nanf("");
         if (item.parts > 1) {
-            const size_t slot = (size_t(index) * a.cache.kv_heads + kv) * FEW_ROWS + r;
+            const size_t slot = (size_t(item.slot) * a.cache.kv_heads + kv) * FEW_ROWS + r;
             *reinterpret_cast<floatx4 *>(a.part_o + slot * DIM + dim) = floatx4{o[0], o[1], o[2], o[3]};
             if (lane == 0) *reinterpret_cast<float2 *>(a.part_ml + slot * 2) = float2{top, sum};
         } else {
@@ -504,35 +508,50 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(AttnArgs a
     }
 }
 
-// Chunks: a workgroup of 8 waves takes 256 rows (256 / group tokens of the q heads of a kv head), 32 a wave, over an item's keys, 32 a step.  Every thread
-// converts 16 codes of keys and 16 of values of the next step and puts them into LDS in the order of the operands, once for all 8 waves.
-constexpr uint32_t PART_BYTES = STEP_KEYS * DIM * 2;  // a step's keys, or values, as halves
+// Chunks: a workgroup of 8 waves takes 256 rows (256 / group tokens of the q heads of a kv head), 32 a wave, over an item's keys, 32 a
+// step.  The codes travel global -> LDS, AHEAD steps before they are wanted; the wave that asked for a kilobyte of keys and one of values
+// makes halves of them, in the order of the operands, once for all eight waves.  A wave's step is a softmax and one stream of products, O^T +=
+// V^T P^T of the step and S^T = K Q^T of the next; the two waves of a SIMD (w and w + 4) take them in opposite order, one's softmax and
+// conversions under the other's products:
+//   waves 0..3:  softmax(s)                | O(s) + S(s+1)
+//   waves 4..7:  O(s) + S(s+1)             | softmax(s+1)
+// Step s reads V(s) and K(s+1) as halves and makes V(s+1) and K(s+2), in the places of V(s-1) and K(s): one barrier a step.
+constexpr uint32_t CODE_BYTES = STEP_KEYS * DIM, HALF_BYTES = 2 * CODE_BYTES;  // a step's keys, or values
+constexpr uint32_t AHEAD = 3, PLACES = 4;
+constexpr uint32_t K_HALVES = 0, V_HALVES = 2 * HALF_BYTES, K_CODES = 4 * HALF_BYTES, V_CODES = K_CODES + PLACES * CODE_BYTES;
+constexpr uint32_t CHUNK_LDS = V_CODES + PLACES * CODE_BYTES;
 template <int TYPE>
 __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnArgs a) {
     typedef typename Row<TYPE>::value V;
-    extern __shared__ __attribute__((aligned(1024))) unsigned char tiles[];  // keys, keys, values, values
+    extern __shared__ __attribute__((aligned(1024))) unsigned char tiles[];
     __shared__ Unit units[WINDOW];
     __shared__ uint32_t nan_from[DIM];
+    constexpr bool BRAIN = TYPE == SAETTA_BF16;
     const uint32_t index = blockIdx.x / a.cache.kv_heads, kv = blockIdx.x % a.cache.kv_heads;
     const uint32_t items = a.head->items;
     const Item item = a.items[index];
-    if (!(int(index < items) & int(item_ok(a, item, index)))) return;
+    if (!(int(index < items) & int(item_ok(a, item, 1)))) return;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t col = lane & 31, hf = lane >> 5;
     const uint32_t rows = item.tokens << a.group_shift;
     for (uint32_t i = tid; i < DIM; i += 64 * CHUNK_WAVES) nan_from[i] = ~0u;
+    const uint32_t unit0 = item.key0 / UNIT_TOKENS, end_unit = (item.key1 + UNIT_TOKENS - 1) / UNIT_TOKENS;
+    const uint32_t steps = end_unit > unit0 ? (end_unit - unit0 + 1) / 2 : 0;
+    find_units(a, units, item.request, kv, unit0, WINDOW, end_unit);
 
-    const uint32_t my_row = wave * 32 + col, row = min(my_row, rows - 1), token = row >> a.group_shift, head = kv * a.group + (row & (a.group - 1));
-    const V *qp = static_cast<const V *>(a.q.data) + (uint64_t(item.row0) + token) * a.q.token_stride + head * a.q.head_stride;
-    u32x4 q[16];
+    half8 q[16];
+    int32_t sees;
+    {
+        const uint32_t row = min(wave * 32 + (lane & 31), rows - 1), token = row >> a.group_shift, head = kv * a.group + (row & (a.group - 1));
+        sees = item.pos0 + int32_t(token) + 1;
+        const V *qp = static_cast<const V *>(a.q.data) + (uint64_t(item.row0) + token) * a.q.token_stride + head * a.q.head_stride + (lane >> 5) * 8;
 #pragma unroll
-    for (int i = 0; i < 16; i++) q[i] = *reinterpret_cast<const u32x4 *>(qp + i * 16 + hf * 8);
+        for (int i = 0; i < 16; i++) q[i] = *reinterpret_cast<const half8 *>(qp + i * 16);
+    }
     const float c = a.scale * 1.4426950408889634f;
-    const int32_t sees = item.pos0 + int32_t(token) + 1;
     const uint32_t all_see = uint32_t(max(item.pos0 + 1, 0));
     // what the wave's first and last rows see
     const uint32_t first_row = min(wave * 32, rows - 1), last_row = min(wave * 32 + 31, rows - 1);
-    const uint32_t wave_all = uint32_t(max(item.pos0 + int32_t(first_row >> a.group_shift) + 1, 0));
+    const uint32_t wave_all = min(uint32_t(max(item.pos0 + int32_t(first_row >> a.group_shift) + 1, 0)), item.key1);
     const uint32_t wave_end = wave * 32 < rows ? min(uint32_t(max(item.pos0 + int32_t(last_row >> a.group_shift) + 1, 0)), item.key1) : 0;
 
     floatx16 acc[8];
@@ -544,96 +563,157 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
 
     const size_t block_bytes = size_t(DIM) << a.block_shift;
     const uint32_t unit_mask = (1u << (a.block_shift - 4)) - 1;
-    const uint32_t end_unit = (item.key1 + UNIT_TOKENS - 1) / UNIT_TOKENS;
-    for (uint32_t first = item.key0 / UNIT_TOKENS; first < end_unit; first += WINDOW) {
-        __syncthreads();
-        find_units(a, units, item.request, kv, first, end_unit, 64 * CHUNK_WAVES);
-        __syncthreads();
-        const uint32_t in_window = min(WINDOW, end_unit - first), steps = (in_window + 1) / 2;
-        u32x4 kc, vc;  // codes on their way: 16 bytes of a unit, keys and values
-        const uint32_t mine = tid >> 8, piece = tid & 255;
-        auto fetch = [&](uint32_t step) {
-            const uint32_t u = min(2 * step + mine, in_window - 1);
-            const size_t at = units[u].block * block_bytes + ((first + u) & unit_mask) * UNIT_BYTES + piece * 16;
-            kc = *reinterpret_cast<const u32x4 *>(a.cache.keys + at);
-            vc = *reinterpret_cast<const u32x4 *>(a.cache.values + at);
-        };
-        auto put = [&](uint32_t step) {
-            unsigned char *kt = tiles + (step & 1) * PART_BYTES, *vt = tiles + (2 + (step & 1)) * PART_BYTES;
-            const uint32_t t = piece & 15, quarter = piece >> 4 & 3, j = piece >> 6;
-            // keys: token t, dims 64 j + 16 quarter .. + 15: both halves of fragment 4 j + quarter
-            unsigned char *kd = kt + (4 * j + quarter) * 1024 + (mine * 16 + t) * 16;
-            *reinterpret_cast<u32x4 *>(kd) = operands_of<TYPE>(kc.x, kc.y);
-            *reinterpret_cast<u32x4 *>(kd + 512) = operands_of<TYPE>(kc.z, kc.w);
-            // values: tokens 4 quarter .. + 3 of dims 16 (4 j + i) + t
-            const uint32_t u = 2 * step + mine, key = (first + u) * UNIT_TOKENS;
-            if (key + UNIT_TOKENS > min(all_see, item.key1) || u >= in_window || !(units[min(u, in_window - 1)].scales & 0x10000)) {
-                const uint32_t limit = u < in_window && (units[u].scales & 0x10000) ? item.key1 : 0;
+    const uint32_t lds0 = uint32_t(reinterpret_cast<uintptr_t>(tiles));
+    // The lane, for what is worked out from it where it is used: kept over the loop it would be in registers that the queries want.
+    auto here = [&] {
+        uint32_t at = lane;
+        asm volatile("" : "+v"(at));
+        return at;
+    };
+    // the wave's kilobyte of a step: 64 dims (part) of the unit `mine`
+    const uint32_t mine = wave >> 2, part = wave & 3;
+    auto copy = [&](const uint8_t *codes, uint32_t step, uint32_t place) {
+        const uint32_t u = unit0 + 2 * step + mine;
+        const uint32_t row = __builtin_amdgcn_readfirstlane(units[u % WINDOW].block);
+        const uint64_t src = reinterpret_cast<uint64_t>(codes) + row * block_bytes + (u & unit_mask) * UNIT_BYTES + part * 1024;
+        asm volatile(
+            "s_mov_b32 m0, %[dst]\n"
+            "s_nop 0\n"
+            "global_load_lds_dwordx4 %[off], %[src]\n"
+            :
+            : [off] "v"(here() * 16), [src] "s"(src), [dst] "s"(lds0 + place + (step % PLACES) * CODE_BYTES + wave * 1024)
+            : "memory", "m0");
+    };
+    auto copy_keys = [&](uint32_t step) { copy(a.cache.keys, step, K_CODES); };
+    auto copy_values = [&](uint32_t step) { copy(a.cache.values, step, V_CODES); };
+    auto make_keys = [&](uint32_t step) {  // token t, dims 64 part + 16 quarter .. + 15: both halves of fragment 4 part + quarter
+        const uint32_t at = here(), t = at & 15, quarter = at >> 4;
+        const u32x4 x = *reinterpret_cast<const u32x4 *>(tiles + K_CODES + (step % PLACES) * CODE_BYTES + wave * 1024 + at * 16);
+        unsigned char *to = tiles + K_HALVES + (step & 1) * HALF_BYTES + (4 * part + quarter) * 1024 + (mine * 16 + t) * 16;
+        *reinterpret_cast<u32x4 *>(to) = operands_of<TYPE>(x.x, x.y);
+        *reinterpret_cast<u32x4 *>(to + 512) = operands_of<TYPE>(x.z, x.w);
+    };
+    auto make_values = [&](uint32_t step) {  // tokens 4 quarter .. + 3 of dims 16 (4 part + i) + t
+        const uint32_t at = here(), t = at & 15, quarter = at >> 4;
+        u32x4 x = *reinterpret_cast<const u32x4 *>(tiles + V_CODES + (step % PLACES) * CODE_BYTES + wave * 1024 + at * 16);
+        const uint32_t u = unit0 + 2 * step + mine, key = u * UNIT_TOKENS;
+        const bool there = __builtin_amdgcn_readfirstlane(units[u % WINDOW].scales) & 0x10000;
+        if (key + UNIT_TOKENS > min(all_see, item.key1) || !there) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) vc[i] = clean_values(vc[i], key + 4 * quarter, limit, all_see, (4 * j + i) * 16 + t, nan_from);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint32_t dim = (4 * j + i) * 16 + t;
-                *reinterpret_cast<u32x2 *>(vt + (2 * (dim >> 5) + mine) * 1024 + (quarter & 1) * 512 + (dim & 31) * 16 + (quarter >> 1) * 8) = halves_of(vc[i]);
-            }
-        };
-        fetch(0);
-        put(0);
-        for (uint32_t step = 0; step < steps; step++) {
-            if (step + 1 < steps) fetch(step + 1);
-            __syncthreads();  // this step's keys and values are in LDS, and the last step's have been read
-            const uint32_t key = (first + 2 * step) * UNIT_TOKENS;
-            if (key < wave_end) {
-                const unsigned char *kt = tiles + (step & 1) * PART_BYTES + lane * 16, *vt = tiles + (2 + (step & 1)) * PART_BYTES + lane * 16;
-                floatx16 s;
-#pragma unroll
-                for (int r = 0; r < 16; r++) s[r] = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 16; i++) s = product32<TYPE>(*reinterpret_cast<const u32x4 *>(kt + i * 1024), q[i], s);
-                const uint32_t scales[2] = {units[2 * step].scales, units[min(2 * step + 1, in_window - 1)].scales};
-                float ck[2], sum[2] = {0.0f, 0.0f}, top = NO_SCORE;
-                int ev[2];
-#pragma unroll
-                for (int i = 0; i < 2; i++) ck[i] = c * key_scale(scales[i]), ev[i] = value_exponent(scales[i]);
-#pragma unroll
-                for (int r = 0; r < 16; r++) s[r] = fmaf(s[r], ck[r >> 3], float(ev[r >> 3]));
-                if (key + STEP_KEYS > min(wave_all, item.key1) || !(scales[0] & scales[1] & 0x10000)) {
-#pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        const uint32_t t = key + 4 * hf + (r & 3) + 8 * (r >> 2);
-                        s[r] = (scales[r >> 3] & 0x10000) && t < item.key1 && int32_t(t) < sees ? s[r] : NO_SCORE;
-                    }
-                }
-#pragma unroll
-                for (int r = 0; r < 16; r++) top = fmaxf(top, s[r]);
-                top = across_rows<32, 64>(top, MaxOp());
-                if (__any(top > m + TAU)) {
-                    const float next = top > m + TAU ? top : m, down = __builtin_amdgcn_exp2f(m - next);
-                    m = next, l *= down;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) acc[i] *= down;
-                }
-#pragma unroll
-                for (int r = 0; r < 16; r++) s[r] = __builtin_amdgcn_exp2f(s[r] - m), sum[r >> 3] += s[r];
-                l = fmaf(sum[0], power_of_two(-ev[0]), fmaf(sum[1], power_of_two(-ev[1]), l));
-#pragma unroll
-                for (int sp = 0; sp < 2; sp++) {
-                    const u32x4 w = {pack_half2(s[8 * sp], s[8 * sp + 1]), pack_half2(s[8 * sp + 2], s[8 * sp + 3]),
-                                     pack_half2(s[8 * sp + 4], s[8 * sp + 5]), pack_half2(s[8 * sp + 6], s[8 * sp + 7])};
-#pragma unroll
-                    for (int i = 0; i < 8; i++) acc[i] = product32<SAETTA_F16>(*reinterpret_cast<const u32x4 *>(vt + (2 * i + sp) * 1024), w, acc[i]);
-                }
-            }
-            if (step + 1 < steps) put(step + 1);
+            for (int i = 0; i < 4; i++) x[i] = clean_values(x[i], key + 4 * quarter, there ? item.key1 : 0, all_see, (4 * part + i) * 16 + t, nan_from);
         }
+        unsigned char *to = tiles + V_HALVES + (step & 1) * HALF_BYTES + mine * 1024 + (quarter & 1) * 512 + (quarter >> 1) * 8;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t dim = (4 * part + i) * 16 + t;
+            *reinterpret_cast<u32x2 *>(to + 2 * (dim >> 5) * 1024 + (dim & 31) * 16) = halves_of(x[i]);
+        }
+    };
+    // Probabilities of a step from its scores, as operands.
+    auto softmax = [&](floatx16 &s, uint32_t step, half8 (&p)[2]) {
+        const uint32_t u = unit0 + 2 * step, key = u * UNIT_TOKENS;
+        const uint32_t scales[2] = {uint32_t(__builtin_amdgcn_readfirstlane(units[u % WINDOW].scales)), uint32_t(__builtin_amdgcn_readfirstlane(units[(u + 1) % WINDOW].scales))};
+        float ck[2], sum[2] = {0.0f, 0.0f}, top = NO_SCORE;
+        int ev[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) ck[i] = c * key_scale(scales[i]), ev[i] = value_exponent(scales[i]);
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] = fmaf(s[r], ck[r >> 3], float(ev[r >> 3]));
+        if (key + STEP_KEYS > wave_all || !(scales[0] & scales[1] & 0x10000)) {
+            // keys of the step that the row sees, less the lane half's four; none of a unit that is not there
+            const int n = min(sees, int(item.key1)) - int(key) - 4 * int(here() >> 5);
+            const int seen[2] = {scales[0] & 0x10000 ? n : -1, scales[1] & 0x10000 ? n : -1};
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] = int((r & 3) + 8 * (r >> 2)) < (r < 8 ? seen[0] : seen[1]) ? s[r] : NO_SCORE;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; r++) top = fmaxf(top, s[r]);
+        top = across_rows<32, 64>(top, MaxOp());
+        if (__any(top > m + TAU)) {
+            const float next = top > m + TAU ? top : m, down = __builtin_amdgcn_exp2f(m - next);
+            m = next, l *= down;
+#pragma unroll
+            for (int i = 0; i < 8; i++) acc[i] *= down;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] = __builtin_amdgcn_exp2f(s[r] - m), sum[r >> 3] += s[r];
+        l = fmaf(sum[0], power_of_two(-ev[0]), fmaf(sum[1], power_of_two(-ev[1]), l));
+#pragma unroll
+        for (int sp = 0; sp < 2; sp++) {
+            const u32x4 w = {pack_half2(s[8 * sp], s[8 * sp + 1]), pack_half2(s[8 * sp + 2], s[8 * sp + 3]),
+                             pack_half2(s[8 * sp + 4], s[8 * sp + 5]), pack_half2(s[8 * sp + 6], s[8 * sp + 7])};
+            p[sp] = __builtin_bit_cast(half8, w);
+        }
+    };
+    auto key_at = [&](uint32_t step) { return (unit0 + 2 * step) * UNIT_TOKENS; };
+    auto k_halves = [&](uint32_t step) { return lds0 + K_HALVES + (step & 1) * HALF_BYTES + here() * 16; };
+    auto v_halves = [&](uint32_t step) { return lds0 + V_HALVES + (step & 1) * HALF_BYTES + here() * 16; };
+
+    if (steps) {
+        __syncthreads();  // the units are there
+        // K(0), K(1), V(0), then what the steps before the first would have asked for
+        copy_keys(0), copy_keys(1), copy_values(0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        make_keys(0), make_keys(1), make_values(0);
+        static_assert(PLACES == AHEAD + 1, "a place is free again when the step after next asks for it");
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; i++) copy_values(1 + i), copy_keys(2 + i);
+        __syncthreads();
+        static_assert(AHEAD == 3, "the copies of three steps are on their way: six of a wave");
+        auto begin = [&](uint32_t step) {
+            // half of the window ahead, before a step comes near it
+            if (step % (WINDOW / 4) == 0 && step) find_units(a, units, item.request, kv, unit0 + 2 * step + WINDOW / 2, WINDOW / 2, end_unit);
+            copy_values(step + 1 + AHEAD), copy_keys(step + 2 + AHEAD);
+        };
+        auto make = [&](uint32_t step) {
+            asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+            make_values(step + 1), make_keys(step + 2);
+        };
+        if (wave < 4) {
+            floatx16 s;
+            if (key_at(0) < wave_end) scores_block<BRAIN>(s, q, k_halves(0));
+            __syncthreads();  // K(0) has been read
+            for (uint32_t step = 0; step < steps; step++) {
+                begin(step);
+                half8 p[2];
+                const bool works = key_at(step) < wave_end;
+                if (works) softmax(s, step, p);
+                make(step);
+                if (works) stream_block_alone<BRAIN>(s, acc, q, p, k_halves(step + 1), v_halves(step));
+                __syncthreads();
+            }
+        } else {
+            half8 p[2] = {};
+            if (key_at(0) < wave_end) {
+                floatx16 s;
+                scores_block<BRAIN>(s, q, k_halves(0));
+                softmax(s, 0, p);
+            }
+            __syncthreads();
+            for (uint32_t step = 0; step < steps; step++) {
+                begin(step);
+                if (key_at(step) < wave_end) {
+                    // (its products go first: its softmax then finds the other wave's to run under)
+                    floatx16 s;
+                    __builtin_amdgcn_s_setprio(2);
+                    stream_block_alone<BRAIN>(s, acc, q, p, k_halves(step + 1), v_halves(step));
+                    __builtin_amdgcn_s_setprio(0);
+                    if (key_at(step + 1) < wave_end) softmax(s, step + 1, p);
+                }
+                make(step);
+                __syncthreads();
+            }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        settle(acc);
     }
 
     __syncthreads();  // nan_from is whole
     l = across_rows<32, 64>(l, SumOp());
+    const uint32_t at = here(), hf = at >> 5, my_row = wave * 32 + (at & 31), token = my_row >> a.group_shift, head = kv * a.group + (my_row & (a.group - 1));
     if (my_row >= rows) return;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const size_t slot = (size_t(index) * a.cache.kv_heads + kv) * CHUNK_ROWS + my_row;
+    const size_t slot = (size_t(item.parts > 1 ? item.slot : 0) * a.cache.kv_heads + kv) * CHUNK_ROWS + my_row;
 #pragma unroll
     for (int i = 0; i < 8; i++)
 #pragma unroll
@@ -666,14 +746,12 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, const Item
     typedef typename Row<TYPE>::value V;
     constexpr uint32_t TILE = FEW ? FEW_ROWS : CHUNK_ROWS, BY = FEW ? 4 : 1;
     const uint32_t there = a.head->tiles, kv = blockIdx.z;
-    Item item = tiles[blockIdx.x];
-    const uint32_t index = item.part;
-    item.part = 0;
-    if (!(int(blockIdx.x < there) & int(index < a.target) & int(item_ok(a, item, index)) & int(item.parts <= a.target - min(index, a.target)))) return;
+    const Item item = tiles[blockIdx.x];
+    if (!(int(blockIdx.x < there) & int(item.parts > 1) & int(item_ok(a, item, item.parts)))) return;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t r = FEW ? blockIdx.y : blockIdx.y * 4 + wave;
     if (r >= item.tokens << a.group_shift) return;  // (FEW: the whole workgroup)
-    const size_t stride = size_t(a.cache.kv_heads) * TILE, slot = (size_t(index) * a.cache.kv_heads + kv) * TILE + r;
+    const size_t stride = size_t(a.cache.kv_heads) * TILE, slot = (size_t(item.slot) * a.cache.kv_heads + kv) * TILE + r;
     const uint64_t row = uint64_t(item.row0) + (r >> a.group_shift);
     const uint32_t head = kv * a.group + (r & (a.group - 1)), dim = lane * 4;
     float gate[4];
@@ -749,18 +827,15 @@ int check_batch(const saetta_paged_batch &b, const char *what) {
     SAETTA_REQUIRE(b.max_blocks > 0 && uint64_t(b.max_blocks) * b.block_tokens < (1ull << 31), SAETTA_E_SHAPE, "%s: rows of %u blocks", what, b.max_blocks);
     return SAETTA_OK;
 }
-// Tiles in parts that there can be: each has two at least, all among the first `target` items.
-uint32_t joined_tiles(const Shape &s) { return s.target / 2 < s.most_tiles ? s.target / 2 : s.most_tiles; }
 size_t items_offset() { return sizeof(SplitHead); }
 size_t tiles_offset(const Shape &s) { return items_offset() + sizeof(Item) * s.most_items; }
 
-constexpr uint32_t CHUNK_LDS = 4 * PART_BYTES;
 uint32_t shift_of(uint32_t n) { return uint32_t(__builtin_ctz(n)); }
 
 template <int TYPE>
 void launch_attn(hipStream_t stream, const AttnArgs &a, const Shape &s, const saetta_paged_attn_params &p, const Item *tiles) {
     const dim3 grid(s.most_items * p.kv_heads);
-    const uint32_t joined = joined_tiles(s);
+    const uint32_t joined = s.most_joined;
     if (s.tile_rows == FEW_ROWS) {
         launch(paged_few_kernel<TYPE>, grid, dim3(64 * FEW_WAVES), 0, stream, a);
         if (joined) launch(paged_merge_kernel<TYPE, true>, dim3(joined, p.rows * s.group, p.kv_heads), dim3(256), 0, stream, a, tiles);
@@ -787,13 +862,13 @@ using namespace saetta;
 extern "C" size_t saetta_paged_split_bytes(saetta_paged_attn_params p, uint32_t requests) {
     if (check_attn(p, requests, "paged_split_bytes")) return 0;
     const Shape s = shape_of(p, requests);
-    return tiles_offset(s) + sizeof(Item) * size_t(joined_tiles(s));
+    return tiles_offset(s) + sizeof(Item) * size_t(s.most_joined);
 }
 
 extern "C" size_t saetta_paged_workspace_bytes(saetta_paged_attn_params p, uint32_t requests) {
     if (check_attn(p, requests, "paged_workspace_bytes")) return 0;
     const Shape s = shape_of(p, requests);
-    return size_t(s.target) * p.kv_heads * s.tile_rows * (DIM + 2) * sizeof(float);
+    return size_t(s.slots) * p.kv_heads * s.tile_rows * (DIM + 2) * sizeof(float);
 }
 
 extern "C" int saetta_paged_split(saetta_stream_t stream, saetta_paged_batch batch, saetta_paged_attn_params p, void *split) {
@@ -806,7 +881,8 @@ extern "C" int saetta_paged_split(saetta_stream_t stream, saetta_paged_batch bat
     unsigned char *at = static_cast<unsigned char *>(split);
     const bool few = s.tile_rows == FEW_ROWS;
     const SplitArgs a = {batch, reinterpret_cast<SplitHead *>(at), reinterpret_cast<Item *>(at + items_offset()), reinterpret_cast<Item *>(at + tiles_offset(s)),
-                         s.tile_tokens, s.target, s.most_items, joined_tiles(s), p.tokens, p.rows, few, few ? STEP_KEYS * FEW_WAVES : 256u};
+                         s.tile_tokens, s.target, s.most_items, s.most_joined, s.slots, p.tokens, p.rows,
+                         few, few ? STEP_KEYS * FEW_WAVES : STEP_KEYS, few ? STEP_KEYS * FEW_WAVES : 256u, few ? 0u : s.tile_tokens / 2};
     launch(paged_split_kernel, dim3(1), dim3(SPLIT_THREADS), 0, as_stream(stream), a);
     return launch_status("paged_split");
 }
@@ -832,8 +908,8 @@ extern "C" int saetta_paged_attn(saetta_stream_t stream, int type, saetta_stride
     const unsigned char *at = static_cast<const unsigned char *>(split);
     float *part_o = static_cast<float *>(workspace);
     const AttnArgs a = {q, gate, out, cache, batch.block_table, reinterpret_cast<const SplitHead *>(at), reinterpret_cast<const Item *>(at + items_offset()),
-                        part_o, part_o + size_t(s.target) * p.kv_heads * s.tile_rows * DIM, batch.requests, batch.max_blocks, p.tokens,
-                        s.group, shift_of(s.group), shift_of(cache.block_tokens), s.target, s.tile_tokens, p.scale};
+                        part_o, part_o + size_t(s.slots) * p.kv_heads * s.tile_rows * DIM, batch.requests, batch.max_blocks, p.tokens,
+                        s.group, shift_of(s.group), shift_of(cache.block_tokens), s.slots, s.tile_tokens, p.scale};
     const Item *tiles = reinterpret_cast<const Item *>(at + tiles_offset(s));
     if (type == SAETTA_F16) launch_attn<SAETTA_F16>(as_stream(stream), a, s, p, tiles);
     else launch_attn<SAETTA_BF16>(as_stream(stream), a, s, p, tiles);
