@@ -9,7 +9,7 @@
 // f16, half a step 2^-12 of it, as operand of the second product: the sums are f32).
 //
 // The three kernels: paged_split_kernel deals rows and keys out as items from the lengths; the attention kernel, one
-// workgroup to an item and kv head, paged_few_kernel for tiles of up to 16 rows and paged_chunk_kernel for tiles of
+// workgroup to an item and kv head, paged_few_kernel for tiles of up to 64 rows and paged_chunk_kernel for tiles of
 // 256; paged_merge_kernel where a tile's keys were taken in parts.
 //
 // Both attention kernels compute S^T = K Q^T and O^T += V^T P^T: a lane owns one query row (column), the running
@@ -38,7 +38,7 @@ constexpr float NO_SCORE = -1e30f;               // of a key that a row does not
 constexpr float NO_MAXIMUM = 0.25f * NO_SCORE;   // where nothing was seen: 2^(NO_SCORE - NO_MAXIMUM) is 0
 constexpr float TAU = 8.0f;                      // the reference maximum is raised only past this many powers of two
 constexpr uint32_t STEP_KEYS = 32;               // keys of a step: two units
-constexpr uint32_t FEW_ROWS = 16, CHUNK_ROWS = 256;
+constexpr uint32_t FEW_ROWS = 16, CHUNK_ROWS = 256;  // FEW_ROWS: of a group of columns; a tile of few rows has 1, 2 or 4 groups
 constexpr int FEW_WAVES = 4, CHUNK_WAVES = 8;
 
 // ---- what is dealt out -------------------------------------------------------------------------------------------
@@ -58,16 +58,19 @@ struct alignas(16) SplitHead {
 
 struct Shape {
     uint32_t group, tile_tokens, tile_rows;
+    uint32_t columns;  // groups of FEW_ROWS rows of the kernel for few rows; 0: chunks
     uint32_t target;  // items that the device takes at once
     uint32_t most_items, most_tiles, most_joined, slots;
 };
 Shape shape_of(const saetta_paged_attn_params &p, uint32_t requests) {
     Shape s;
     s.group = p.heads / p.kv_heads;
-    const bool few = uint64_t(p.rows) * s.group <= FEW_ROWS;
-    s.tile_rows = few ? FEW_ROWS : CHUNK_ROWS;
+    const uint64_t rows = uint64_t(p.rows) * s.group;
+    s.columns = rows <= FEW_ROWS ? 1 : rows <= 2 * FEW_ROWS ? 2 : rows <= 4 * FEW_ROWS ? 4 : 0;
+    const bool few = s.columns > 0;
+    s.tile_rows = few ? s.columns * FEW_ROWS : CHUNK_ROWS;
     s.tile_tokens = few ? p.rows : CHUNK_ROWS / s.group;
-    const uint32_t workgroups = cu_count() * (few ? 2 : 1);
+    const uint32_t workgroups = cu_count() * (s.columns == 1 ? 2 : 1);
     s.target = workgroups / p.kv_heads ? workgroups / p.kv_heads : 1;
     s.most_tiles = few ? requests : p.tokens / s.tile_tokens + requests;
     // With parts of total / target no more than `target` tiles have more than one, and their parts are 2 * target at most
@@ -114,60 +117,80 @@ __device__ __forceinline__ Item tile_of(const SplitArgs &a, const Work &w, uint3
     return item;
 }
 
+// x summed over the threads before this one; `all`: over all of them.  (All threads; `waves` is free again on return.)
+__device__ __forceinline__ uint32_t before_this(uint32_t x, uint32_t *waves, uint32_t &all) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t through = x;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const uint32_t other = __shfl_up(through, d);
+        if (lane >= uint32_t(d)) through += other;
+    }
+    if (lane == 63) waves[wave] = through;
+    __syncthreads();
+    uint32_t before = 0;
+    all = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < SPLIT_WAVES; w++) {
+        if (w < wave) before += waves[w];
+        all += waves[w];
+    }
+    __syncthreads();
+    return before + through - x;
+}
+// The last of `starts` (rising, starts[0] <= x) that is no more than x.
+__device__ __forceinline__ uint32_t last_at_most(const uint32_t *starts, uint32_t n, uint32_t x) {
+    uint32_t low = 0;
+    while (n > 1) {
+        const uint32_t half = n / 2;
+        if (starts[low + half] <= x) low += half, n -= half;
+        else n = half;
+    }
+    return low;
+}
+
 // Deals the work out so that the workgroups that run at once end together.  What a key of a tile costs is one of two numbers: a chunk's tile of
 // at most half the rows keeps half the waves and takes 5 / 8 of the time.  A tile that costs more than total / target is cut into parts of that
 // and a rest; the items go out from the dearest class to the cheapest, so that who ends early takes what is small.  (One workgroup: a sum over the
 // tiles, a count of the classes, and the items themselves; the tiles by turns over its threads.  The places of the items in a class and of the
 // parts' sums follow from atomic counts, in any order: what is computed does not depend on them.)
 __global__ __launch_bounds__(SPLIT_THREADS) void paged_split_kernel(SplitArgs a) {
-    __shared__ uint32_t waves[SPLIT_WAVES], starts[SPLIT_THREADS], classes[SIZES], slots_there, tiles_there;
+    __shared__ uint32_t waves[SPLIT_WAVES], starts[SPLIT_THREADS], ends[SPLIT_THREADS], classes[SIZES], slots_there, tiles_there;
     __shared__ unsigned long long total;
+    __shared__ Item cut[SPLIT_THREADS];
     const uint32_t tid = threadIdx.x, requests = a.batch.requests;
     if (tid < SIZES) classes[tid] = 0;
     if (tid == 0) slots_there = tiles_there = 0, total = 0;
+    __syncthreads();
 
-    // f(tile) for every tile; a call for each of the passes
+    // Requests by rounds of as many as there are threads, their tiles by rounds too: f(a tile of this thread's, or one of no tokens), all threads
+    // alike.  Where one round holds all (as a rule) the tile is found once.
     bool found = false;
-    uint32_t found_tiles = 0;
+    Item mine;
     auto for_tiles = [&](auto f) {
+        if (found) return f(mine);
         for (uint32_t r0 = 0; r0 < requests; r0 += SPLIT_THREADS) {
-            if (!found) {  // (one round of requests: the same starts in every pass)
-                const uint32_t tiles = work_of(a, r0 + tid).tiles;
-                uint32_t through = tiles;
-#pragma unroll
-                for (int d = 1; d < 64; d *= 2) {
-                    const uint32_t other = __shfl_up(through, d);
-                    if ((tid & 63) >= uint32_t(d)) through += other;
+            uint32_t all;
+            const uint32_t tiles = work_of(a, r0 + tid).tiles, before = before_this(tiles, waves, all), n = min(uint32_t(SPLIT_THREADS), requests - r0);
+            starts[tid] = before;
+            __syncthreads();
+            for (uint32_t k0 = 0; k0 < all; k0 += SPLIT_THREADS) {
+                const uint32_t k = k0 + tid;
+                mine.tokens = 0;
+                if (k < all) {
+                    const uint32_t i = last_at_most(starts, n, k);
+                    mine = tile_of(a, work_of(a, r0 + i), r0 + i, k - starts[i]);
                 }
-                __syncthreads();
-                if ((tid & 63) == 63) waves[tid >> 6] = through;
-                __syncthreads();
-                uint32_t base = 0, all = 0;
-#pragma unroll
-                for (uint32_t w = 0; w < SPLIT_WAVES; w++) {
-                    if (w < (tid >> 6)) base += waves[w];
-                    all += waves[w];
-                }
-                starts[tid] = base + through - tiles;
-                __syncthreads();
-                found = requests <= SPLIT_THREADS, found_tiles = all;
+                f(mine);
             }
-            const uint32_t n = min(uint32_t(SPLIT_THREADS), requests - r0);
-            for (uint32_t k = tid; k < found_tiles; k += SPLIT_THREADS) {
-                uint32_t i = 0, left = n;  // the last request whose tiles start at k or before
-                while (left > 1) {
-                    const uint32_t half = left / 2;
-                    if (starts[i + half] <= k) i += half, left -= half;
-                    else left = half;
-                }
-                f(tile_of(a, work_of(a, r0 + i), r0 + i, k - starts[i]));
-            }
+            found = requests <= SPLIT_THREADS && all <= SPLIT_THREADS;
+            __syncthreads();  // `starts` may be written again
         }
     };
     auto price = [&](const Item &tile) { return tile.tokens <= a.half_tokens ? 5u : 8u; };
 
     unsigned long long sum = 0;
-    for_tiles([&](const Item &tile) { sum += static_cast<unsigned long long>(tile.key1) * price(tile); });
+    for_tiles([&](const Item &tile) { sum += tile.tokens ? static_cast<unsigned long long>(tile.key1) * price(tile) : 0; });
 #pragma unroll
     for (int d = 32; d > 0; d /= 2) sum += __shfl_xor(sum, d);
     if ((tid & 63) == 0 && sum) atomicAdd(&total, sum);
@@ -178,9 +201,10 @@ __global__ __launch_bounds__(SPLIT_THREADS) void paged_split_kernel(SplitArgs a)
         const unsigned long long keys = fair / price(tile) + a.granule;
         return uint32_t(keys > 0x7fffffffu ? 0x7fffffffu : keys) / a.granule * a.granule;
     };
-    const unsigned long long dearest = fair + 8ull * a.granule;
-    auto class_of = [&](uint32_t keys, uint32_t price) { return SIZES - 1 - uint32_t(min(static_cast<unsigned long long>(keys) * price * SIZES / dearest, SIZES - 1ull)); };
+    const float per_class = float(SIZES) / float(fair + 8ull * a.granule);
+    auto class_of = [&](uint32_t keys, uint32_t price) { return SIZES - 1 - min(uint32_t(float(keys) * float(price) * per_class), SIZES - 1); };
     for_tiles([&](const Item &tile) {
+        if (!tile.tokens) return;
         const uint32_t length = length_of(tile), whole = tile.key1 / length, rest = tile.key1 - whole * length;
         if (whole) atomicAdd(&classes[class_of(length, price(tile))], whole);
         if (rest || !whole) atomicAdd(&classes[class_of(rest, price(tile))], 1u);
@@ -199,22 +223,29 @@ __global__ __launch_bounds__(SPLIT_THREADS) void paged_split_kernel(SplitArgs a)
         if (tid == 63) a.head->items = min(through, a.most_items);
     }
     __syncthreads();
+    // the items: a round's tiles in LDS, their parts over all threads
     for_tiles([&](Item tile) {
-        const uint32_t length = length_of(tile), end = tile.key1;
-        tile.parts = end > length ? (end + length - 1) / length : 1;
+        const uint32_t length = tile.tokens ? length_of(tile) : 1;
+        tile.parts = !tile.tokens ? 0 : tile.key1 > length ? (tile.key1 + length - 1) / length : 1;
         if (tile.parts > 1) {
             tile.slot = atomicAdd(&slots_there, tile.parts);
             const uint32_t t = atomicAdd(&tiles_there, 1u);
             if (t < a.most_joined) a.tiles[t] = tile;
         }
-        for (uint32_t p = 0; p < tile.parts; p++) {
-            Item item = tile;
-            item.key0 = p * length, item.key1 = min(end, item.key0 + length), item.slot = tile.slot + p;
-            const uint32_t where = atomicAdd(&classes[class_of(item.key1 - item.key0, price(tile))], 1u);
+        uint32_t all;
+        ends[tid] = before_this(tile.parts, waves, all);
+        cut[tid] = tile;
+        __syncthreads();
+        for (uint32_t k = tid; k < all; k += SPLIT_THREADS) {
+            const uint32_t i = last_at_most(ends, SPLIT_THREADS, k);
+            Item item = cut[i];
+            const uint32_t each = length_of(item), p = k - ends[i];
+            item.key0 = p * each, item.key1 = min(item.key1, item.key0 + each), item.slot += p;
+            const uint32_t where = atomicAdd(&classes[class_of(item.key1 - item.key0, price(item))], 1u);
             if (where < a.most_items) a.items[where] = item;
         }
+        __syncthreads();
     });
-    __syncthreads();
     if (tid == 0) a.head->tiles = min(tiles_there, a.most_joined);
 }
 
@@ -270,18 +301,17 @@ struct Unit {
     uint32_t block;     // row of [blocks][kv_heads]; of the first block where there is none
     uint32_t scales;    // 127 + ek | (127 + ev) << 8 | there << 16
 };
-// Units that a workgroup keeps in LDS: unit u at u % WINDOW.  Units from `first` on, `count` of them; from `end` on there are none.
+// Units that a workgroup keeps in LDS: unit u at u % WINDOW.  From `end` on there are none.
 constexpr uint32_t WINDOW = 512;
-__device__ __forceinline__ void find_units(const AttnArgs &a, Unit *units, uint32_t request, uint32_t head, uint32_t first, uint32_t count, uint32_t end) {
-    const uint32_t shift = a.block_shift - 4;
-    for (uint32_t i = threadIdx.x; i < count; i += blockDim.x) {
-        const uint32_t u = first + i, entry = u >> shift;
-        uint32_t block = ~0u;
-        if (u < end && entry < a.max_blocks) block = uint32_t(a.block_table[size_t(request) * a.max_blocks + entry]);
-        const bool there = block < a.cache.blocks;
-        const uint32_t row = (there ? block : 0) * a.cache.kv_heads + head;
-        units[u % WINDOW] = {row, uint32_t(a.cache.key_scales[row]) | uint32_t(a.cache.value_scales[row]) << 8 | uint32_t(there) << 16};
-    }
+__device__ __forceinline__ Unit find_unit(const AttnArgs &a, uint32_t request, uint32_t head, uint32_t u, uint32_t end) {
+    const uint32_t entry = u >> (a.block_shift - 4);
+    uint32_t block = ~0u;
+    if (u < end && entry < a.max_blocks) block = uint32_t(a.block_table[size_t(request) * a.max_blocks + entry]);
+    const bool there = block < a.cache.blocks;
+    return {(there ? block : 0) * a.cache.kv_heads + head, uint32_t(there) << 16};
+}
+__device__ __forceinline__ uint32_t find_scales(const AttnArgs &a, const Unit &u) {
+    return u.scales | uint32_t(a.cache.key_scales[u.block]) | uint32_t(a.cache.value_scales[u.block]) << 8;
 }
 // (exponents as the store writes them: what else a byte says would make scores no numbers)
 __device__ __forceinline__ float key_scale(uint32_t scales) { return power_of_two(min(max(int(scales & 0xff) - 127, LOWEST_EXPONENT), HIGHEST_EXPONENT)); }
@@ -328,14 +358,21 @@ __device__ __forceinline__ void put_row(const AttnArgs &a, uint64_t row, uint32_
 
 // Few rows: a workgroup of 4 waves walks an item's keys, every wave 32 of 128 at a time, straight from memory into registers, the
 // keys of its next step on their way while this one's values are worked on, and the other way round.  Bound by memory: 16 KB a step of a
-// wave, against 64 + 64 conversions of two codes and 16 + 16 products.  Row l % 16 of the tile is lane l's; the waves' sums are joined in LDS.
-// A wave looks up the places of the units of its next 32 steps by itself, a unit a lane: no barrier in the walk, and the scales, which only the
-// scores want, come behind the first codes.
+// wave, against 64 + 64 conversions of two codes and, a group of 16 rows (COLUMNS of them), 16 + 16 products.  Row l % 16 of a group is lane
+// l's; the waves' sums are joined in LDS, a group after the other.  A wave looks up the places of the units of its next 32 steps by itself, a
+// unit a lane: no barrier in the walk, and the scales, which only the scores want, come behind the first codes.
+// One group is two workgroups to a CU; two have the registers of a SIMD to themselves; of four, two teams of four waves take two each over the
+// same keys, whose codes the second team finds in the caches.  (The kernel for chunks, where most of a tile is empty, takes 102 to 108 us for 64 drafts of 3
+// to 8 rows at 4000 tokens, this one 46 to @@; four groups to a wave are more registers than there are: 353.)
+constexpr int few_threads(int columns) { return 64 * FEW_WAVES * (columns == 4 ? 2 : 1); }
 constexpr uint32_t FEW_STEPS = 32;     // steps that a wave looks up at a time
 constexpr int FEW_STRIDE = DIM + 4;    // floats of a row in LDS: neighbouring rows on other banks
-template <int TYPE>
-__global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(AttnArgs a) {
+template <int TYPE, int TILE_COLUMNS>
+__global__ __launch_bounds__(few_threads(TILE_COLUMNS), TILE_COLUMNS == 2 ? 1 : 2) void paged_few_kernel(AttnArgs a) {
     typedef typename Row<TYPE>::value V;
+    constexpr uint32_t TILE = TILE_COLUMNS * FEW_ROWS;
+    constexpr int TEAMS = TILE_COLUMNS == 4 ? 2 : 1, COLUMNS = TILE_COLUMNS / TEAMS;  // groups of a wave
+    constexpr uint32_t WAVES = TEAMS * FEW_WAVES;
     __shared__ __attribute__((aligned(16))) float sums[FEW_WAVES][FEW_ROWS][FEW_STRIDE];
     __shared__ float ml[FEW_WAVES][FEW_ROWS][2];
     __shared__ uint32_t nan_from[DIM];
@@ -345,13 +382,14 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(AttnArgs a
     if (!(int(index < items) & int(item_ok(a, item, 1)))) return;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t col = lane & 15, quarter = lane >> 4;
+    const uint32_t team = wave / FEW_WAVES, turn = wave % FEW_WAVES;  // the wave's groups; its keys
     const uint32_t rows = item.tokens << a.group_shift;  // of the tile that are there
-    for (uint32_t i = tid; i < DIM; i += 64 * FEW_WAVES) nan_from[i] = ~0u;
+    for (uint32_t i = tid; i < DIM; i += 64 * WAVES) nan_from[i] = ~0u;
 
     const size_t block_bytes = size_t(DIM) << a.block_shift;
     const uint32_t unit_shift = a.block_shift - 4, unit_mask = (1u << unit_shift) - 1;
     const uint32_t end_unit = (item.key1 + UNIT_TOKENS - 1) / UNIT_TOKENS;
-    uint32_t first = item.key0 / UNIT_TOKENS + 2 * wave;  // the wave's first unit; its steps are 2 * FEW_WAVES units apart
+    uint32_t first = item.key0 / UNIT_TOKENS + 2 * turn;  // the wave's first unit; its steps are 2 * FEW_WAVES units apart
     // Lane 2 i + j: unit j of step i, its row of [blocks][kv heads] (of block 0 where there is none) and whether there is one.
     uint32_t place = 0, scales = 0;
     auto look_up = [&] {
@@ -381,85 +419,126 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(AttnArgs a
         look_up_scales();
     }
 
-    const uint32_t row = min(col, rows - 1), token = row >> a.group_shift, head = kv * a.group + (row & (a.group - 1));
-    const V *qp = static_cast<const V *>(a.q.data) + (uint64_t(item.row0) + token) * a.q.token_stride + head * a.q.head_stride;
-    u32x4 q[8];  // [64 dims][8 of 16]
+    // The queries: [group][64 dims][8 of 16].  Of two teams they stay in LDS: two waves share the registers of a SIMD.
+    constexpr bool IN_LDS = TEAMS > 1;
+    u32x4 q[IN_LDS ? 1 : COLUMNS][8];
+    __shared__ u32x4 q_lds[IN_LDS ? TILE_COLUMNS : 1][IN_LDS ? 8 : 1][IN_LDS ? 64 : 1];
+    int32_t sees[COLUMNS];  // keys of this lane's rows
+    auto row_of = [&](uint32_t g) { return min(g * FEW_ROWS + col, rows - 1); };
+    auto q_of = [&](uint32_t g, int i) {
+        const uint32_t row = row_of(g), token = row >> a.group_shift, head = kv * a.group + (row & (a.group - 1));
+        const V *qp = static_cast<const V *>(a.q.data) + (uint64_t(item.row0) + token) * a.q.token_stride + head * a.q.head_stride;
+        return *reinterpret_cast<const u32x4 *>(qp + (i >> 1) * 64 + quarter * 16 + (i & 1) * 8);
+    };
 #pragma unroll
-    for (int i = 0; i < 8; i++) q[i] = *reinterpret_cast<const u32x4 *>(qp + (i >> 1) * 64 + quarter * 16 + (i & 1) * 8);
+    for (int g = 0; g < COLUMNS; g++) sees[g] = item.pos0 + int32_t(row_of(team * COLUMNS + g) >> a.group_shift) + 1;
+    if constexpr (IN_LDS) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) q_lds[wave >> 1][(wave & 1) * 4 + i][lane] = q_of(wave >> 1, (wave & 1) * 4 + i);
+    } else {
+#pragma unroll
+        for (int g = 0; g < COLUMNS; g++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) q[g][i] = q_of(g, i);
+    }
+    auto query = [&](int g, int i) {
+        if constexpr (IN_LDS) return q_lds[team * COLUMNS + g][i][lane];
+        else return q[g][i];
+    };
     if (steps) fetch(a.cache.values, 0, v);
     const float c = a.scale * 1.4426950408889634f;
-    const int32_t sees = item.pos0 + int32_t(token) + 1;  // keys of this row
     const uint32_t all_see = uint32_t(max(item.pos0 + 1, 0));  // of the first row, and so of all
 
-    floatx4 acc[16];
+    floatx4 acc[COLUMNS][16];
+    float m[COLUMNS], l[COLUMNS];
 #pragma unroll
-    for (int i = 0; i < 16; i++) acc[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    float m = NO_MAXIMUM, l = 0.0f;
-    __syncthreads();  // nan_from is clear
+    for (int g = 0; g < COLUMNS; g++) {
+        m[g] = NO_MAXIMUM, l[g] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) acc[g][i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    __syncthreads();  // nan_from is clear, the queries are in LDS
 
     while (steps) {
         const uint32_t here = min(steps, FEW_STEPS);
         for (uint32_t step = 0; step < here; step++) {
             const uint32_t key = (first + step * (2 * FEW_WAVES)) * UNIT_TOKENS;
-            floatx4 s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+            floatx4 s[COLUMNS][2];
+#pragma unroll
+            for (int g = 0; g < COLUMNS; g++) s[g][0] = s[g][1] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int j = 0; j < 4; j++) {
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    s[i] = product16<TYPE>(operands_of<TYPE>(k[i][j].x, k[i][j].y), q[2 * j], s[i]);
-                    s[i] = product16<TYPE>(operands_of<TYPE>(k[i][j].z, k[i][j].w), q[2 * j + 1], s[i]);
+                    const u32x4 low = operands_of<TYPE>(k[i][j].x, k[i][j].y), high = operands_of<TYPE>(k[i][j].z, k[i][j].w);
+#pragma unroll
+                    for (int g = 0; g < COLUMNS; g++) s[g][i] = product16<TYPE>(low, query(g, 2 * j), s[g][i]);
+#pragma unroll
+                    for (int g = 0; g < COLUMNS; g++) s[g][i] = product16<TYPE>(high, query(g, 2 * j + 1), s[g][i]);
                 }
             }
             if (step + 1 < here) fetch(a.cache.keys, step + 1, k);
             const uint32_t scale[2] = {uint32_t(__builtin_amdgcn_readlane(scales, 2 * step)), uint32_t(__builtin_amdgcn_readlane(scales, 2 * step + 1))};
             const int ev[2] = {value_exponent(scale[0]), value_exponent(scale[1])};
             const float ck[2] = {c * key_scale(scale[0]), c * key_scale(scale[1])};
-            float p[2][4], top = NO_SCORE;
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) p[i][r] = fmaf(s[i][r], ck[i], float(ev[i]));
-            if (key + STEP_KEYS > min(all_see, item.key1) || !(scale[0] & scale[1] & 0x10000)) {
+            const bool masked = key + STEP_KEYS > min(all_see, item.key1) || !(scale[0] & scale[1] & 0x10000);
+            // (what follows from the lane is worked out where it is used: kept over the loop it would be in registers that the sums want)
+            uint32_t at = lane;
+            if (masked) {
+                asm volatile("" : "+v"(at));
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    const bool there = scale[i] & 0x10000;
-                    const uint32_t from = key + i * UNIT_TOKENS + quarter * 4;
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const uint32_t t = from + r;
-                        p[i][r] = there && t < item.key1 && int32_t(t) < sees ? p[i][r] : NO_SCORE;
-                    }
-                    const uint32_t limit = there ? item.key1 : 0;
+                    const uint32_t from = key + i * UNIT_TOKENS + (at >> 4) * 4, limit = scale[i] & 0x10000 ? item.key1 : 0;
 #pragma unroll
                     for (int j = 0; j < 4; j++)
 #pragma unroll
-                        for (int t = 0; t < 4; t++) v[i][j][t] = clean_values(v[i][j][t], from, limit, all_see, (4 * j + t) * 16 + col, nan_from);
+                        for (int t = 0; t < 4; t++) v[i][j][t] = clean_values(v[i][j][t], from, limit, all_see, (4 * j + t) * 16 + (at & 15), nan_from);
                 }
             }
+            u32x4 w[COLUMNS];
 #pragma unroll
-            for (int i = 0; i < 2; i++)
+            for (int g = 0; g < COLUMNS; g++) {
+                float p[2][4], top = NO_SCORE;
 #pragma unroll
-                for (int r = 0; r < 4; r++) top = fmaxf(top, p[i][r]);
-            top = across_rows<16, 64>(top, MaxOp());
-            if (__any(top > m + TAU)) {
-                const float next = top > m + TAU ? top : m, down = __builtin_amdgcn_exp2f(m - next);
-                m = next, l *= down;
+                for (int i = 0; i < 2; i++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) acc[i] *= down;
+                    for (int r = 0; r < 4; r++) p[i][r] = fmaf(s[g][i][r], ck[i], float(ev[i]));
+                if (masked) {
+                    // keys of the step that the row sees, less the quarter's four; none of a unit that is not there
+                    const int n = min(sees[g], int(item.key1)) - int(key + (at >> 4) * 4);
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const int seen = scale[i] & 0x10000 ? n - i * int(UNIT_TOKENS) : -1;
+#pragma unroll
+                        for (int r = 0; r < 4; r++) p[i][r] = r < seen ? p[i][r] : NO_SCORE;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) top = fmaxf(top, p[i][r]);
+                top = across_rows<16, 64>(top, MaxOp());
+                if (__any(top > m[g] + TAU)) {
+                    const float next = top > m[g] + TAU ? top : m[g], down = __builtin_amdgcn_exp2f(m[g] - next);
+                    m[g] = next, l[g] *= down;
+#pragma unroll
+                    for (int i = 0; i < 16; i++) acc[g][i] *= down;
+                }
+                float part[2] = {0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) p[i][r] = __builtin_amdgcn_exp2f(p[i][r] - m[g]), part[i] += p[i][r];
+                l[g] = fmaf(part[0], power_of_two(-ev[0]), fmaf(part[1], power_of_two(-ev[1]), l[g]));
+                w[g] = u32x4{pack_half2(p[0][0], p[0][1]), pack_half2(p[0][2], p[0][3]), pack_half2(p[1][0], p[1][1]), pack_half2(p[1][2], p[1][3])};
             }
-            float part[2] = {0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) p[i][r] = __builtin_amdgcn_exp2f(p[i][r] - m), part[i] += p[i][r];
-            l = fmaf(part[0], power_of_two(-ev[0]), fmaf(part[1], power_of_two(-ev[1]), l));
-            const u32x4 w = {pack_half2(p[0][0], p[0][1]), pack_half2(p[0][2], p[0][3]), pack_half2(p[1][0], p[1][1]), pack_half2(p[1][2], p[1][3])};
 #pragma unroll
             for (int j = 0; j < 4; j++)
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
                     const u32x2 v0 = halves_of(v[0][j][t]), v1 = halves_of(v[1][j][t]);
-                    acc[4 * j + t] = product16<SAETTA_F16>(u32x4{v0.x, v0.y, v1.x, v1.y}, w, acc[4 * j + t]);
+#pragma unroll
+                    for (int g = 0; g < COLUMNS; g++) acc[g][4 * j + t] = product16<SAETTA_F16>(u32x4{v0.x, v0.y, v1.x, v1.y}, w[g], acc[g][4 * j + t]);
                 }
             if (step + 1 < here) fetch(a.cache.values, step + 1, v);
         }
@@ -473,37 +552,46 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(AttnArgs a
         }
     }
 
-    l = across_rows<16, 64>(l, SumOp());
 #pragma unroll
-    for (int i = 0; i < 16; i++) *reinterpret_cast<floatx4 *>(&sums[wave][col][i * 16 + quarter * 4]) = acc[i];
-    if (quarter == 0) ml[wave][col][0] = m, ml[wave][col][1] = l;
-    __syncthreads();
-    for (uint32_t r = wave; r < rows; r += FEW_WAVES) {
-        float top = NO_MAXIMUM, sum = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int w = 0; w < FEW_WAVES; w++) top = fmaxf(top, ml[w][r][0]);
-        const uint32_t dim = lane * 4;
-#pragma unroll
-        for (int w = 0; w < FEW_WAVES; w++) {
-            const float f = __builtin_amdgcn_exp2f(ml[w][r][0] - top);
-            sum = fmaf(ml[w][r][1], f, sum);
-            const floatx4 x = *reinterpret_cast<const floatx4 *>(&sums[w][r][dim]);
-#pragma unroll
-            for (int i = 0; i < 4; i++) o[i] = fmaf(x[i], f, o[i]);
+    for (int g = 0; g < TILE_COLUMNS; g++) {
+        if (g > 0) {
+            if (g * FEW_ROWS >= rows) return;
+            __syncthreads();  // the last group's sums have been read
         }
-        const uint32_t tok = r >> a.group_shift;
+        if (team == uint32_t(g / COLUMNS)) {
+            const float sum_all = across_rows<16, 64>(l[g % COLUMNS], SumOp());
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (nan_from[dim + i] != ~0u && int32_t(nan_from[dim + i]) < item.pos0 + int32_t(tok) + 1) o[i] = __builtin_nanf("");
-        if (item.parts > 1) {
-            const size_t slot = (size_t(item.slot) * a.cache.kv_heads + kv) * FEW_ROWS + r;
-            *reinterpret_cast<floatx4 *>(a.part_o + slot * DIM + dim) = floatx4{o[0], o[1], o[2], o[3]};
-            if (lane == 0) *reinterpret_cast<float2 *>(a.part_ml + slot * 2) = float2{top, sum};
-        } else {
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            for (int i = 0; i < 16; i++) *reinterpret_cast<floatx4 *>(&sums[turn][col][i * 16 + quarter * 4]) = acc[g % COLUMNS][i];
+            if (quarter == 0) ml[turn][col][0] = m[g % COLUMNS], ml[turn][col][1] = sum_all;
+        }
+        __syncthreads();
+        for (uint32_t i = wave; i < min(rows - g * FEW_ROWS, FEW_ROWS); i += WAVES) {
+            const uint32_t r = g * FEW_ROWS + i, dim = lane * 4;
+            float top = NO_MAXIMUM, sum = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < 4; i++) o[i] *= inv;
-            put_row<TYPE>(a, uint64_t(item.row0) + tok, kv * a.group + (r & (a.group - 1)), dim, o);
+            for (int w = 0; w < FEW_WAVES; w++) top = fmaxf(top, ml[w][i][0]);
+#pragma unroll
+            for (int w = 0; w < FEW_WAVES; w++) {
+                const float f = __builtin_amdgcn_exp2f(ml[w][i][0] - top);
+                sum = fmaf(ml[w][i][1], f, sum);
+                const floatx4 x = *reinterpret_cast<const floatx4 *>(&sums[w][i][dim]);
+#pragma unroll
+                for (int d = 0; d < 4; d++) o[d] = fmaf(x[d], f, o[d]);
+            }
+            const uint32_t token = r >> a.group_shift;
+#pragma unroll
+            for (int d = 0; d < 4; d++)
+                if (nan_from[dim + d] != ~0u && int32_t(nan_from[dim + d]) < item.pos0 + int32_t(token) + 1) o[d] = __builtin_nanf("");
+            if (item.parts > 1) {
+                const size_t slot = (size_t(item.slot) * a.cache.kv_heads + kv) * TILE + r;
+                *reinterpret_cast<floatx4 *>(a.part_o + slot * DIM + dim) = floatx4{o[0], o[1], o[2], o[3]};
+                if (lane == 0) *reinterpret_cast<float2 *>(a.part_ml + slot * 2) = float2{top, sum};
+            } else {
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+                for (int d = 0; d < 4; d++) o[d] *= inv;
+                put_row<TYPE>(a, uint64_t(item.row0) + token, kv * a.group + (r & (a.group - 1)), dim, o);
+            }
         }
     }
 }
@@ -519,13 +607,15 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void paged_few_kernel(AttnArgs a
 constexpr uint32_t CODE_BYTES = STEP_KEYS * DIM, HALF_BYTES = 2 * CODE_BYTES;  // a step's keys, or values
 constexpr uint32_t AHEAD = 3, PLACES = 4;
 constexpr uint32_t K_HALVES = 0, V_HALVES = 2 * HALF_BYTES, K_CODES = 4 * HALF_BYTES, V_CODES = K_CODES + PLACES * CODE_BYTES;
-constexpr uint32_t CHUNK_LDS = V_CODES + PLACES * CODE_BYTES;
+constexpr uint32_t OUT_STRIDE = 128 + 4;  // floats of half a row on its way out, and the row's sum
+constexpr uint32_t OUT_BYTES = CHUNK_ROWS * OUT_STRIDE * 4;
+constexpr uint32_t CHUNK_LDS = OUT_BYTES > V_CODES + PLACES * CODE_BYTES ? OUT_BYTES : V_CODES + PLACES * CODE_BYTES;
 template <int TYPE>
 __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnArgs a) {
     typedef typename Row<TYPE>::value V;
     extern __shared__ __attribute__((aligned(1024))) unsigned char tiles[];
     __shared__ Unit units[WINDOW];
-    __shared__ uint32_t nan_from[DIM];
+    __shared__ __attribute__((aligned(16))) uint32_t nan_from[DIM];
     constexpr bool BRAIN = TYPE == SAETTA_BF16;
     const uint32_t index = blockIdx.x / a.cache.kv_heads, kv = blockIdx.x % a.cache.kv_heads;
     const uint32_t items = a.head->items;
@@ -536,17 +626,20 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
     for (uint32_t i = tid; i < DIM; i += 64 * CHUNK_WAVES) nan_from[i] = ~0u;
     const uint32_t unit0 = item.key0 / UNIT_TOKENS, end_unit = (item.key1 + UNIT_TOKENS - 1) / UNIT_TOKENS;
     const uint32_t steps = end_unit > unit0 ? (end_unit - unit0 + 1) / 2 : 0;
-    find_units(a, units, item.request, kv, unit0, WINDOW, end_unit);
+    static_assert(WINDOW == 64 * CHUNK_WAVES, "a thread a unit");
+    Unit unit = find_unit(a, item.request, kv, unit0 + tid, end_unit);
+    units[(unit0 + tid) % WINDOW] = unit;
+    __syncthreads();  // where the codes are is known; how they are scaled comes with them
 
     half8 q[16];
     int32_t sees;
-    {
+    auto get_queries = [&] {
         const uint32_t row = min(wave * 32 + (lane & 31), rows - 1), token = row >> a.group_shift, head = kv * a.group + (row & (a.group - 1));
         sees = item.pos0 + int32_t(token) + 1;
         const V *qp = static_cast<const V *>(a.q.data) + (uint64_t(item.row0) + token) * a.q.token_stride + head * a.q.head_stride + (lane >> 5) * 8;
 #pragma unroll
         for (int i = 0; i < 16; i++) q[i] = *reinterpret_cast<const half8 *>(qp + i * 16);
-    }
+    };
     const float c = a.scale * 1.4426950408889634f;
     const uint32_t all_see = uint32_t(max(item.pos0 + 1, 0));
     // what the wave's first and last rows see
@@ -650,10 +743,12 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
     auto v_halves = [&](uint32_t step) { return lds0 + V_HALVES + (step & 1) * HALF_BYTES + here() * 16; };
 
     if (steps) {
-        __syncthreads();  // the units are there
         // K(0), K(1), V(0), then what the steps before the first would have asked for
         copy_keys(0), copy_keys(1), copy_values(0);
+        get_queries();
+        units[(unit0 + tid) % WINDOW].scales = find_scales(a, unit);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();  // the scales are there
         make_keys(0), make_keys(1), make_values(0);
         static_assert(PLACES == AHEAD + 1, "a place is free again when the step after next asks for it");
 #pragma unroll
@@ -662,7 +757,12 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
         static_assert(AHEAD == 3, "the copies of three steps are on their way: six of a wave");
         auto begin = [&](uint32_t step) {
             // half of the window ahead, before a step comes near it
-            if (step % (WINDOW / 4) == 0 && step) find_units(a, units, item.request, kv, unit0 + 2 * step + WINDOW / 2, WINDOW / 2, end_unit);
+            if (step % (WINDOW / 4) == 0 && step && tid < WINDOW / 2) {
+                const uint32_t u = unit0 + 2 * step + WINDOW / 2 + tid;
+                unit = find_unit(a, item.request, kv, u, end_unit);
+                unit.scales = find_scales(a, unit);
+                units[u % WINDOW] = unit;
+            }
             copy_values(step + 1 + AHEAD), copy_keys(step + 2 + AHEAD);
         };
         auto make = [&](uint32_t step) {
@@ -708,32 +808,65 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
         settle(acc);
     }
 
-    __syncthreads();  // nan_from is whole
+    __syncthreads();  // nan_from is whole, and what the tiles held has been read
+    // Through LDS, a half of the dims at a time, so that a wave stores two rows' 128 dims side by side.  A row's sum is behind its dims.
     l = across_rows<32, 64>(l, SumOp());
-    const uint32_t at = here(), hf = at >> 5, my_row = wave * 32 + (at & 31), token = my_row >> a.group_shift, head = kv * a.group + (my_row & (a.group - 1));
-    if (my_row >= rows) return;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const size_t slot = (size_t(item.parts > 1 ? item.slot : 0) * a.cache.kv_heads + kv) * CHUNK_ROWS + my_row;
+    const uint32_t at = here();
+    float *mine_out = reinterpret_cast<float *>(tiles) + wave * (32 * OUT_STRIDE);
+    mine_out[(at & 31) * OUT_STRIDE + 128] = l == 0.0f ? 0.0f : 1.0f / l;
+    if (wave * 32 >= rows) return;
+    const uint32_t wave_rows = min(rows - wave * 32, 32u), head0 = kv * a.group;
+    if (item.parts > 1 && at < wave_rows)
+        *reinterpret_cast<float2 *>(a.part_ml + ((size_t(item.slot) * a.cache.kv_heads + kv) * CHUNK_ROWS + wave * 32 + at) * 2) = float2{m, l};
 #pragma unroll
-    for (int i = 0; i < 8; i++)
+    for (int half = 0; half < 2; half++) {
+        wave_sync();  // the last half has been read
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const uint32_t dim = 32 * i + 4 * hf + 8 * k;
-            float o[4];
+        for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                o[j] = acc[i][4 * k + j];
-                if (nan_from[dim + j] != ~0u && int32_t(nan_from[dim + j]) < sees) o[j] = __builtin_nanf("");
+            for (int k = 0; k < 4; k++) {
+                const floatx16 &x = acc[4 * half + i];
+                *reinterpret_cast<floatx4 *>(mine_out + (at & 31) * OUT_STRIDE + 32 * i + 4 * (at >> 5) + 8 * k) = floatx4{x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]};
             }
-            if (item.parts > 1) {
-                *reinterpret_cast<floatx4 *>(a.part_o + slot * DIM + dim) = floatx4{o[0], o[1], o[2], o[3]};
-            } else {
+        const uint32_t in_half = 4 * (at & 31), dim = 128 * half + in_half;
+        auto row_at = [&](int i) { return 2 * i + (at >> 5); };
+        auto place_of = [&](int i, const saetta_strided_rows &rows_of) {  // (a row past the tile's end: its last, unused)
+            const uint32_t row = wave * 32 + min(row_at(i), wave_rows - 1);
+            return static_cast<V *>(rows_of.data) + (uint64_t(item.row0) + (row >> a.group_shift)) * rows_of.token_stride + (head0 + (row & (a.group - 1))) * rows_of.head_stride + dim;
+        };
+        const uint4 nan4 = *reinterpret_cast<const uint4 *>(nan_from + dim);
+        const uint32_t nans[4] = {nan4.x, nan4.y, nan4.z, nan4.w};
+        const bool any_nan = (nans[0] & nans[1] & nans[2] & nans[3]) != ~0u;
+        const bool gated = a.gate.data && item.parts == 1;
+        typedef V value4 __attribute__((ext_vector_type(4)));
+        value4 gate[16];
+        if (gated) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) o[j] *= inv;
-                put_row<TYPE>(a, uint64_t(item.row0) + token, head, dim, o);
+            for (int i = 0; i < 16; i++) gate[i] = *reinterpret_cast<const value4 *>(place_of(i, a.gate));
+        }
+        wave_sync();
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const float *from = mine_out + row_at(i) * OUT_STRIDE;
+            floatx4 o = *reinterpret_cast<const floatx4 *>(from + in_half);
+            const uint32_t row = wave * 32 + row_at(i);
+            if (any_nan) {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (nans[j] != ~0u && int32_t(nans[j]) < item.pos0 + int32_t(row >> a.group_shift) + 1) o[j] = __builtin_nanf("");
+            }
+            if (row_at(i) >= wave_rows) continue;
+            if (item.parts > 1) {
+                *reinterpret_cast<floatx4 *>(a.part_o + ((size_t(item.slot) * a.cache.kv_heads + kv) * CHUNK_ROWS + row) * DIM + dim) = o;
+            } else {
+                o *= from[128];
+                value4 w;
+#pragma unroll
+                for (int j = 0; j < 4; j++) w[j] = Row<TYPE>::store(gated ? o[j] * sigmoid(Row<TYPE>::load(gate[i][j])) : o[j]);
+                *reinterpret_cast<value4 *>(place_of(i, a.out)) = w;
             }
         }
-    if (item.parts > 1 && hf == 0) *reinterpret_cast<float2 *>(a.part_ml + slot * 2) = float2{m, l};
+    }
 }
 
 // Joins the parts of the tiles that were taken in parts: out = sum_p 2^(M_p - M) O_p / sum_p 2^(M_p - M) l_p.  A lane has four
@@ -741,10 +874,11 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
 // its four waves in turn.  Chunks: a wave a row.  (Joining in the attention kernel, by the workgroup that ends last, costs more than this launch:
 // all workgroups run at once, so their stores' way to the memory that the XCDs share, the count and the loads come on top of the longest walk;
 // 48 ragged contexts 67 -> 72 us, one of 517 tokens 9.3 -> 9.7.)
-template <int TYPE, bool FEW>
+template <int TYPE, int COLUMNS>
 __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, const Item *tiles) {
     typedef typename Row<TYPE>::value V;
-    constexpr uint32_t TILE = FEW ? FEW_ROWS : CHUNK_ROWS, BY = FEW ? 4 : 1;
+    constexpr bool FEW = COLUMNS > 0;
+    constexpr uint32_t TILE = FEW ? COLUMNS * FEW_ROWS : CHUNK_ROWS, BY = FEW ? 4 : 1;
     const uint32_t there = a.head->tiles, kv = blockIdx.z;
     const Item item = tiles[blockIdx.x];
     if (!(int(blockIdx.x < there) & int(item.parts > 1) & int(item_ok(a, item, item.parts)))) return;
@@ -835,14 +969,17 @@ uint32_t shift_of(uint32_t n) { return uint32_t(__builtin_ctz(n)); }
 template <int TYPE>
 void launch_attn(hipStream_t stream, const AttnArgs &a, const Shape &s, const saetta_paged_attn_params &p, const Item *tiles) {
     const dim3 grid(s.most_items * p.kv_heads);
-    const uint32_t joined = s.most_joined;
-    if (s.tile_rows == FEW_ROWS) {
-        launch(paged_few_kernel<TYPE>, grid, dim3(64 * FEW_WAVES), 0, stream, a);
-        if (joined) launch(paged_merge_kernel<TYPE, true>, dim3(joined, p.rows * s.group, p.kv_heads), dim3(256), 0, stream, a, tiles);
-    } else {
-        launch(paged_chunk_kernel<TYPE>, grid, dim3(64 * CHUNK_WAVES), CHUNK_LDS, stream, a);
-        if (joined) launch(paged_merge_kernel<TYPE, false>, dim3(joined, CHUNK_ROWS / 4, p.kv_heads), dim3(256), 0, stream, a, tiles);
+    auto few = [&](auto attention, auto merge) {
+        launch(attention, grid, dim3(few_threads(int(s.columns))), 0, stream, a);
+        launch(merge, dim3(s.most_joined, p.rows * s.group, p.kv_heads), dim3(256), 0, stream, a, tiles);
+    };
+    switch (s.columns) {
+        case 1: return few(paged_few_kernel<TYPE, 1>, paged_merge_kernel<TYPE, 1>);
+        case 2: return few(paged_few_kernel<TYPE, 2>, paged_merge_kernel<TYPE, 2>);
+        case 4: return few(paged_few_kernel<TYPE, 4>, paged_merge_kernel<TYPE, 4>);
     }
+    launch(paged_chunk_kernel<TYPE>, grid, dim3(64 * CHUNK_WAVES), CHUNK_LDS, stream, a);
+    launch(paged_merge_kernel<TYPE, 0>, dim3(s.most_joined, CHUNK_ROWS / 4, p.kv_heads), dim3(256), 0, stream, a, tiles);
 }
 
 }  // namespace
@@ -879,7 +1016,7 @@ extern "C" int saetta_paged_split(saetta_stream_t stream, saetta_paged_batch bat
     if (int rc = ensure_device()) return rc;
     const Shape s = shape_of(p, batch.requests);
     unsigned char *at = static_cast<unsigned char *>(split);
-    const bool few = s.tile_rows == FEW_ROWS;
+    const bool few = s.columns > 0;
     const SplitArgs a = {batch, reinterpret_cast<SplitHead *>(at), reinterpret_cast<Item *>(at + items_offset()), reinterpret_cast<Item *>(at + tiles_offset(s)),
                          s.tile_tokens, s.target, s.most_items, s.most_joined, s.slots, p.tokens, p.rows,
                          few, few ? STEP_KEYS * FEW_WAVES : STEP_KEYS, few ? STEP_KEYS * FEW_WAVES : 256u, few ? 0u : s.tile_tokens / 2};
