@@ -600,7 +600,8 @@ int saetta_paged_tables(saetta_stream_t stream, const uint32_t *context_lens, co
                         saetta_paged_state state, saetta_paged_step step, saetta_paged_tables_params p);
 
 /* Rows of `heads` rows of 256 values, of a type of the call's: token t's head h begins at data + t * token_stride +
- * h * head_stride, both in values.  data is 16-byte aligned and the strides are multiples of 16 bytes. */
+ * h * head_stride, both in values.  data is 16-byte aligned and the strides are multiples of 16 bytes (of the
+ * attention's rows less than 2^32 values). */
 typedef struct saetta_strided_rows {
     void *data;
     uint64_t token_stride;

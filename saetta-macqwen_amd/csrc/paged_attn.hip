@@ -251,8 +251,19 @@ __global__ __launch_bounds__(SPLIT_THREADS) void paged_split_kernel(SplitArgs a)
 
 // ---- the attention kernels ----------------------------------------------------------------------------------------
 
+// Rows whose strides fit 32 bits: a lane's address is two multiply-adds (with 64 bits to both factors it was a dozen instructions of a quarter of the
+// rate, half the time of a chunk tile's end).
+struct Rows {
+    void *data;
+    uint32_t token_stride, head_stride;
+};
+template <class V>
+__device__ __forceinline__ V *row_at(const Rows &r, uint32_t token, uint32_t head) {
+    return static_cast<V *>(r.data) + uint64_t(token) * r.token_stride + uint64_t(head) * r.head_stride;
+}
+
 struct AttnArgs {
-    saetta_strided_rows q, gate, out;
+    Rows q, gate, out;
     saetta_paged_cache cache;
     const int32_t *block_table;
     const SplitHead *head;
@@ -345,15 +356,15 @@ __device__ __forceinline__ uint32_t clean_values(uint32_t w, uint32_t key, uint3
 
 // out of a row's four dims
 template <int TYPE>
-__device__ __forceinline__ void put_row(const AttnArgs &a, uint64_t row, uint32_t head, uint32_t dim, float (&o)[4]) {
+__device__ __forceinline__ void put_row(const AttnArgs &a, uint32_t row, uint32_t head, uint32_t dim, float (&o)[4]) {
     typedef typename Row<TYPE>::value V;
     if (a.gate.data) {
         float g[4];
-        load_values<TYPE, 4>(static_cast<const V *>(a.gate.data) + row * a.gate.token_stride + head * a.gate.head_stride + dim, g);
+        load_values<TYPE, 4>(row_at<const V>(a.gate, row, head) + dim, g);
 #pragma unroll
         for (int i = 0; i < 4; i++) o[i] *= sigmoid(g[i]);
     }
-    store_values<TYPE, 4>(static_cast<V *>(a.out.data) + row * a.out.token_stride + head * a.out.head_stride + dim, o);
+    store_values<TYPE, 4>(row_at<V>(a.out, row, head) + dim, o);
 }
 
 // Few rows: a workgroup of 4 waves walks an item's keys, every wave 32 of 128 at a time, straight from memory into registers, the
@@ -427,7 +438,7 @@ __global__ __launch_bounds__(few_threads(TILE_COLUMNS), TILE_COLUMNS == 2 ? 1 : 
     auto row_of = [&](uint32_t g) { return min(g * FEW_ROWS + col, rows - 1); };
     auto q_of = [&](uint32_t g, int i) {
         const uint32_t row = row_of(g), token = row >> a.group_shift, head = kv * a.group + (row & (a.group - 1));
-        const V *qp = static_cast<const V *>(a.q.data) + (uint64_t(item.row0) + token) * a.q.token_stride + head * a.q.head_stride;
+        const V *qp = row_at<const V>(a.q, item.row0 + token, head);
         return *reinterpret_cast<const u32x4 *>(qp + (i >> 1) * 64 + quarter * 16 + (i & 1) * 8);
     };
 #pragma unroll
@@ -590,7 +601,7 @@ __global__ __launch_bounds__(few_threads(TILE_COLUMNS), TILE_COLUMNS == 2 ? 1 : 
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
                 for (int d = 0; d < 4; d++) o[d] *= inv;
-                put_row<TYPE>(a, uint64_t(item.row0) + token, kv * a.group + (r & (a.group - 1)), dim, o);
+                put_row<TYPE>(a, item.row0 + token, kv * a.group + (r & (a.group - 1)), dim, o);
             }
         }
     }
@@ -636,7 +647,7 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
     auto get_queries = [&] {
         const uint32_t row = min(wave * 32 + (lane & 31), rows - 1), token = row >> a.group_shift, head = kv * a.group + (row & (a.group - 1));
         sees = item.pos0 + int32_t(token) + 1;
-        const V *qp = static_cast<const V *>(a.q.data) + (uint64_t(item.row0) + token) * a.q.token_stride + head * a.q.head_stride + (lane >> 5) * 8;
+        const V *qp = row_at<const V>(a.q, item.row0 + token, head) + (lane >> 5) * 8;
 #pragma unroll
         for (int i = 0; i < 16; i++) q[i] = *reinterpret_cast<const half8 *>(qp + i * 16);
     };
@@ -829,10 +840,10 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
                 *reinterpret_cast<floatx4 *>(mine_out + (at & 31) * OUT_STRIDE + 32 * i + 4 * (at >> 5) + 8 * k) = floatx4{x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]};
             }
         const uint32_t in_half = 4 * (at & 31), dim = 128 * half + in_half;
-        auto row_at = [&](int i) { return 2 * i + (at >> 5); };
-        auto place_of = [&](int i, const saetta_strided_rows &rows_of) {  // (a row past the tile's end: its last, unused)
-            const uint32_t row = wave * 32 + min(row_at(i), wave_rows - 1);
-            return static_cast<V *>(rows_of.data) + (uint64_t(item.row0) + (row >> a.group_shift)) * rows_of.token_stride + (head0 + (row & (a.group - 1))) * rows_of.head_stride + dim;
+        auto in_wave = [&](int i) { return 2 * i + (at >> 5); };
+        auto place_of = [&](int i, const Rows &rows_of) {  // (a row past the tile's end: its last, unused)
+            const uint32_t row = wave * 32 + min(in_wave(i), wave_rows - 1);
+            return row_at<V>(rows_of, item.row0 + (row >> a.group_shift), head0 + (row & (a.group - 1))) + dim;
         };
         const uint4 nan4 = *reinterpret_cast<const uint4 *>(nan_from + dim);
         const uint32_t nans[4] = {nan4.x, nan4.y, nan4.z, nan4.w};
@@ -847,15 +858,15 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
         wave_sync();
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            const float *from = mine_out + row_at(i) * OUT_STRIDE;
+            const float *from = mine_out + in_wave(i) * OUT_STRIDE;
             floatx4 o = *reinterpret_cast<const floatx4 *>(from + in_half);
-            const uint32_t row = wave * 32 + row_at(i);
+            const uint32_t row = wave * 32 + in_wave(i);
             if (any_nan) {
 #pragma unroll
                 for (int j = 0; j < 4; j++)
                     if (nans[j] != ~0u && int32_t(nans[j]) < item.pos0 + int32_t(row >> a.group_shift) + 1) o[j] = __builtin_nanf("");
             }
-            if (row_at(i) >= wave_rows) continue;
+            if (in_wave(i) >= wave_rows) continue;
             if (item.parts > 1) {
                 *reinterpret_cast<floatx4 *>(a.part_o + ((size_t(item.slot) * a.cache.kv_heads + kv) * CHUNK_ROWS + row) * DIM + dim) = o;
             } else {
@@ -886,10 +897,10 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, const Item
     const uint32_t r = FEW ? blockIdx.y : blockIdx.y * 4 + wave;
     if (r >= item.tokens << a.group_shift) return;  // (FEW: the whole workgroup)
     const size_t stride = size_t(a.cache.kv_heads) * TILE, slot = (size_t(item.slot) * a.cache.kv_heads + kv) * TILE + r;
-    const uint64_t row = uint64_t(item.row0) + (r >> a.group_shift);
+    const uint32_t row = item.row0 + (r >> a.group_shift);
     const uint32_t head = kv * a.group + (r & (a.group - 1)), dim = lane * 4;
     float gate[4];
-    if (a.gate.data) load_values<TYPE, 4>(static_cast<const V *>(a.gate.data) + row * a.gate.token_stride + head * a.gate.head_stride + dim, gate);
+    if (a.gate.data) load_values<TYPE, 4>(row_at<const V>(a.gate, row, head) + dim, gate);
 
     float m = NO_MAXIMUM, l = 0.0f;
     floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -940,7 +951,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, const Item
     float x[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) x[i] = a.gate.data ? o[i] * inv * sigmoid(gate[i]) : o[i] * inv;
-    store_values<TYPE, 4>(static_cast<V *>(a.out.data) + row * a.out.token_stride + head * a.out.head_stride + dim, x);
+    store_values<TYPE, 4>(row_at<V>(a.out, row, head) + dim, x);
 }
 
 int check_attn(const saetta_paged_attn_params &p, uint32_t requests, const char *what) {
@@ -964,6 +975,7 @@ int check_batch(const saetta_paged_batch &b, const char *what) {
 size_t items_offset() { return sizeof(SplitHead); }
 size_t tiles_offset(const Shape &s) { return items_offset() + sizeof(Item) * s.most_items; }
 
+Rows narrow(const saetta_strided_rows &r) { return {r.data, uint32_t(r.token_stride), uint32_t(r.head_stride)}; }
 uint32_t shift_of(uint32_t n) { return uint32_t(__builtin_ctz(n)); }
 
 template <int TYPE>
@@ -1036,6 +1048,9 @@ extern "C" int saetta_paged_attn(saetta_stream_t stream, int type, saetta_stride
     SAETTA_REQUIRE(q.data && out.data && split && workspace, SAETTA_E_NULL, "paged_attn: null buffer");
     SAETTA_REQUIRE(rows_aligned(q, type) && rows_aligned(out, type) && rows_aligned(gate, type), SAETTA_E_ALIGN,
                    "paged_attn: q, gate and out must be 16-byte aligned, with strides of multiples of 16 bytes");
+    for (const saetta_strided_rows &r : {q, gate, out})
+        SAETTA_REQUIRE(r.token_stride < (1ull << 32) && r.head_stride < (1ull << 32), SAETTA_E_SHAPE, "paged_attn: strides of %llu and %llu values (less than 2^32)",
+                       static_cast<unsigned long long>(r.token_stride), static_cast<unsigned long long>(r.head_stride));
     SAETTA_REQUIRE(aligned(split, 16) && aligned(workspace, 16), SAETTA_E_ALIGN, "paged_attn: split and workspace must be 16-byte aligned");
     const size_t need = saetta_paged_workspace_bytes(p, batch.requests);
     SAETTA_REQUIRE(workspace_bytes >= need, SAETTA_E_SCRATCH, "paged_attn: workspace of %zu bytes (%zu needed)", workspace_bytes, need);
@@ -1044,7 +1059,7 @@ extern "C" int saetta_paged_attn(saetta_stream_t stream, int type, saetta_stride
     const Shape s = shape_of(p, batch.requests);
     const unsigned char *at = static_cast<const unsigned char *>(split);
     float *part_o = static_cast<float *>(workspace);
-    const AttnArgs a = {q, gate, out, cache, batch.block_table, reinterpret_cast<const SplitHead *>(at), reinterpret_cast<const Item *>(at + items_offset()),
+    const AttnArgs a = {narrow(q), narrow(gate), narrow(out), cache, batch.block_table, reinterpret_cast<const SplitHead *>(at), reinterpret_cast<const Item *>(at + items_offset()),
                         part_o, part_o + size_t(s.slots) * p.kv_heads * s.tile_rows * DIM, batch.requests, batch.max_blocks, p.tokens,
                         s.group, shift_of(s.group), shift_of(cache.block_tokens), s.slots, s.tile_tokens, p.scale};
     const Item *tiles = reinterpret_cast<const Item *>(at + tiles_offset(s));

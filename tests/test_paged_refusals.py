@@ -99,6 +99,8 @@ def test_attention_refuses_buffers():
     refused(attn(ws=A + 8), -4, "16-byte")
     refused(attn(q=rows(head=252)), -4, "16-byte")
     refused(attn(gate=rows(A + 2)), -4, "16-byte")
+    refused(attn(q=rows(token=1 << 32)), -2, "2^32")
+    refused(attn(out=rows(head=1 << 33)), -2, "2^32")
     refused(attn(size=need - 1), -6, "needed")
     refused(attn(c=cache(kv_heads=4)), -2, "kv heads")
     refused(attn(c=cache(block_tokens=32)), -2, "blocks of 32")
