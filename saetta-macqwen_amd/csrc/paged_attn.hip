@@ -607,6 +607,9 @@ __global__ __launch_bounds__(few_threads(TILE_COLUMNS), TILE_COLUMNS == 2 ? 1 : 
     }
 }
 
+// A workgroup barrier for what went through LDS: the copies of later steps stay on their way (__syncthreads waits for them).
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 // Chunks: a workgroup of 8 waves takes 256 rows (256 / group tokens of the q heads of a kv head), 32 a wave, over an item's keys, 32 a
 // step.  The codes travel global -> LDS, AHEAD steps before they are wanted; the wave that asked for a kilobyte of keys and one of values
 // makes halves of them, in the order of the operands, once for all eight waves.  A wave's step is a softmax and one stream of products, O^T +=
@@ -676,10 +679,13 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
     };
     // the wave's kilobyte of a step: 64 dims (part) of the unit `mine`
     const uint32_t mine = wave >> 2, part = wave & 3;
+    // What the lanes hold of the units of 32 steps, unit j of step i in lane 2 i + j: where the codes to be copied are, and the scales of the steps that are
+    // worked on.  (A lane's register is read at once; read from LDS each time, with nothing to do meanwhile, they were a third of a step.)
+    uint32_t places = 0, scales = 0;
+    auto hold = [&](uint32_t step) { return units[(unit0 + 2 * step + here()) % WINDOW]; };
     auto copy = [&](const uint8_t *codes, uint32_t step, uint32_t place) {
-        const uint32_t u = unit0 + 2 * step + mine;
-        const uint32_t row = __builtin_amdgcn_readfirstlane(units[u % WINDOW].block);
-        const uint64_t src = reinterpret_cast<uint64_t>(codes) + row * block_bytes + (u & unit_mask) * UNIT_BYTES + part * 1024;
+        const uint32_t row = __builtin_amdgcn_readlane(places, (2 * step + mine) % 64);
+        const uint64_t src = reinterpret_cast<uint64_t>(codes) + row * block_bytes + ((unit0 + 2 * step + mine) & unit_mask) * UNIT_BYTES + part * 1024;
         asm volatile(
             "s_mov_b32 m0, %[dst]\n"
             "s_nop 0\n"
@@ -688,20 +694,23 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
             : [off] "v"(here() * 16), [src] "s"(src), [dst] "s"(lds0 + place + (step % PLACES) * CODE_BYTES + wave * 1024)
             : "memory", "m0");
     };
-    auto copy_keys = [&](uint32_t step) { copy(a.cache.keys, step, K_CODES); };
     auto copy_values = [&](uint32_t step) { copy(a.cache.values, step, V_CODES); };
-    auto make_keys = [&](uint32_t step) {  // token t, dims 64 part + 16 quarter .. + 15: both halves of fragment 4 part + quarter
+    auto copy_keys = [&](uint32_t step) {  // (the keys are a step ahead of the values: the first to want the next 32)
+        if (step % 32 == 0) places = hold(step).block;
+        copy(a.cache.keys, step, K_CODES);
+    };
+    auto keys_of = [&](uint32_t step) { return *reinterpret_cast<const u32x4 *>(tiles + K_CODES + (step % PLACES) * CODE_BYTES + wave * 1024 + here() * 16); };
+    auto values_of = [&](uint32_t step) { return *reinterpret_cast<const u32x4 *>(tiles + V_CODES + (step % PLACES) * CODE_BYTES + wave * 1024 + here() * 16); };
+    auto make_keys = [&](const u32x4 &x, uint32_t step) {  // token t, dims 64 part + 16 quarter .. + 15: both halves of fragment 4 part + quarter
         const uint32_t at = here(), t = at & 15, quarter = at >> 4;
-        const u32x4 x = *reinterpret_cast<const u32x4 *>(tiles + K_CODES + (step % PLACES) * CODE_BYTES + wave * 1024 + at * 16);
         unsigned char *to = tiles + K_HALVES + (step & 1) * HALF_BYTES + (4 * part + quarter) * 1024 + (mine * 16 + t) * 16;
         *reinterpret_cast<u32x4 *>(to) = operands_of<TYPE>(x.x, x.y);
         *reinterpret_cast<u32x4 *>(to + 512) = operands_of<TYPE>(x.z, x.w);
     };
-    auto make_values = [&](uint32_t step) {  // tokens 4 quarter .. + 3 of dims 16 (4 part + i) + t
+    auto make_values = [&](u32x4 x, uint32_t step) {  // tokens 4 quarter .. + 3 of dims 16 (4 part + i) + t
         const uint32_t at = here(), t = at & 15, quarter = at >> 4;
-        u32x4 x = *reinterpret_cast<const u32x4 *>(tiles + V_CODES + (step % PLACES) * CODE_BYTES + wave * 1024 + at * 16);
-        const uint32_t u = unit0 + 2 * step + mine, key = u * UNIT_TOKENS;
-        const bool there = __builtin_amdgcn_readfirstlane(units[u % WINDOW].scales) & 0x10000;
+        const uint32_t key = (unit0 + 2 * step + mine) * UNIT_TOKENS;
+        const bool there = __builtin_amdgcn_readlane(scales, (2 * step + mine) % 64) & 0x10000;
         if (key + UNIT_TOKENS > min(all_see, item.key1) || !there) {
 #pragma unroll
             for (int i = 0; i < 4; i++) x[i] = clean_values(x[i], key + 4 * quarter, there ? item.key1 : 0, all_see, (4 * part + i) * 16 + t, nan_from);
@@ -715,18 +724,18 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
     };
     // Probabilities of a step from its scores, as operands.
     auto softmax = [&](floatx16 &s, uint32_t step, half8 (&p)[2]) {
-        const uint32_t u = unit0 + 2 * step, key = u * UNIT_TOKENS;
-        const uint32_t scales[2] = {uint32_t(__builtin_amdgcn_readfirstlane(units[u % WINDOW].scales)), uint32_t(__builtin_amdgcn_readfirstlane(units[(u + 1) % WINDOW].scales))};
+        const uint32_t key = (unit0 + 2 * step) * UNIT_TOKENS;
+        const uint32_t scale[2] = {uint32_t(__builtin_amdgcn_readlane(scales, 2 * step % 64)), uint32_t(__builtin_amdgcn_readlane(scales, (2 * step + 1) % 64))};
         float ck[2], sum[2] = {0.0f, 0.0f}, top = NO_SCORE;
         int ev[2];
 #pragma unroll
-        for (int i = 0; i < 2; i++) ck[i] = c * key_scale(scales[i]), ev[i] = value_exponent(scales[i]);
+        for (int i = 0; i < 2; i++) ck[i] = c * key_scale(scale[i]), ev[i] = value_exponent(scale[i]);
 #pragma unroll
         for (int r = 0; r < 16; r++) s[r] = fmaf(s[r], ck[r >> 3], float(ev[r >> 3]));
-        if (key + STEP_KEYS > wave_all || !(scales[0] & scales[1] & 0x10000)) {
+        if (key + STEP_KEYS > wave_all || !(scale[0] & scale[1] & 0x10000)) {
             // keys of the step that the row sees, less the lane half's four; none of a unit that is not there
             const int n = min(sees, int(item.key1)) - int(key) - 4 * int(here() >> 5);
-            const int seen[2] = {scales[0] & 0x10000 ? n : -1, scales[1] & 0x10000 ? n : -1};
+            const int seen[2] = {scale[0] & 0x10000 ? n : -1, scale[1] & 0x10000 ? n : -1};
 #pragma unroll
             for (int r = 0; r < 16; r++) s[r] = int((r & 3) + 8 * (r >> 2)) < (r < 8 ? seen[0] : seen[1]) ? s[r] : NO_SCORE;
         }
@@ -760,11 +769,12 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
         units[(unit0 + tid) % WINDOW].scales = find_scales(a, unit);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();  // the scales are there
-        make_keys(0), make_keys(1), make_values(0);
+        scales = hold(0).scales;
+        make_keys(keys_of(0), 0), make_keys(keys_of(1), 1), make_values(values_of(0), 0);
         static_assert(PLACES == AHEAD + 1, "a place is free again when the step after next asks for it");
 #pragma unroll
         for (uint32_t i = 0; i < AHEAD; i++) copy_values(1 + i), copy_keys(2 + i);
-        __syncthreads();
+        lds_barrier();
         static_assert(AHEAD == 3, "the copies of three steps are on their way: six of a wave");
         auto begin = [&](uint32_t step) {
             // half of the window ahead, before a step comes near it
@@ -776,22 +786,22 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
             }
             copy_values(step + 1 + AHEAD), copy_keys(step + 2 + AHEAD);
         };
-        auto make = [&](uint32_t step) {
-            asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
-            make_values(step + 1), make_keys(step + 2);
-        };
+        auto arrived = [&] { asm volatile("s_waitcnt vmcnt(6)" ::: "memory"); };  // V(step + 1), K(step + 2)
         if (wave < 4) {
             floatx16 s;
             if (key_at(0) < wave_end) scores_block<BRAIN>(s, q, k_halves(0));
-            __syncthreads();  // K(0) has been read
+            lds_barrier();  // K(0) has been read
             for (uint32_t step = 0; step < steps; step++) {
                 begin(step);
+                arrived();
+                const u32x4 v_codes = values_of(step + 1), k_codes = keys_of(step + 2);
                 half8 p[2];
                 const bool works = key_at(step) < wave_end;
                 if (works) softmax(s, step, p);
-                make(step);
+                if ((step + 1) % 32 == 0) scales = hold(step + 1).scales;
+                make_values(v_codes, step + 1), make_keys(k_codes, step + 2);
                 if (works) stream_block_alone<BRAIN>(s, acc, q, p, k_halves(step + 1), v_halves(step));
-                __syncthreads();
+                lds_barrier();
             }
         } else {
             half8 p[2] = {};
@@ -800,19 +810,23 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
                 scores_block<BRAIN>(s, q, k_halves(0));
                 softmax(s, 0, p);
             }
-            __syncthreads();
+            lds_barrier();
             for (uint32_t step = 0; step < steps; step++) {
                 begin(step);
-                if (key_at(step) < wave_end) {
+                floatx16 s;
+                const bool works = key_at(step) < wave_end;
+                if (works) {
                     // (its products go first: its softmax then finds the other wave's to run under)
-                    floatx16 s;
                     __builtin_amdgcn_s_setprio(2);
                     stream_block_alone<BRAIN>(s, acc, q, p, k_halves(step + 1), v_halves(step));
                     __builtin_amdgcn_s_setprio(0);
-                    if (key_at(step + 1) < wave_end) softmax(s, step + 1, p);
                 }
-                make(step);
-                __syncthreads();
+                arrived();
+                const u32x4 v_codes = values_of(step + 1), k_codes = keys_of(step + 2);
+                if ((step + 1) % 32 == 0) scales = hold(step + 1).scales;
+                if (works && key_at(step + 1) < wave_end) softmax(s, step + 1, p);
+                make_values(v_codes, step + 1), make_keys(k_codes, step + 2);
+                lds_barrier();
             }
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
