@@ -85,8 +85,12 @@ struct SplitArgs {
     SplitHead *head;
     Item *items, *tiles;
     uint32_t tile_tokens, target, most_items, most_joined, slots, tokens, rows;
-    uint32_t few, granule, least, half_tokens;
+    uint32_t few, granule, least, extra, half_tokens;
 };
+
+// What an item of a chunk costs besides its keys, in keys (15 us of a workgroup, and its sums' way through memory): seven prompts of 90 to 1900
+// tokens 118 us with 0, 115 with 256, 110 with 512, 123 with 1024; a chunk beside drafts 365, 353, 352, 352 a layer.
+constexpr uint32_t CHUNK_EXTRA = 512;
 
 constexpr int SPLIT_THREADS = 1024, SPLIT_WAVES = SPLIT_THREADS / 64;
 constexpr uint32_t SIZES = 64;  // classes of items by what they cost
@@ -156,11 +160,11 @@ __device__ __forceinline__ uint32_t last_at_most(const uint32_t *starts, uint32_
 // parts' sums follow from atomic counts, in any order: what is computed does not depend on them.)
 __global__ __launch_bounds__(SPLIT_THREADS) void paged_split_kernel(SplitArgs a) {
     __shared__ uint32_t waves[SPLIT_WAVES], starts[SPLIT_THREADS], ends[SPLIT_THREADS], classes[SIZES], slots_there, tiles_there;
-    __shared__ unsigned long long total;
+    __shared__ unsigned long long total, items_there;
     __shared__ Item cut[SPLIT_THREADS];
     const uint32_t tid = threadIdx.x, requests = a.batch.requests;
     if (tid < SIZES) classes[tid] = 0;
-    if (tid == 0) slots_there = tiles_there = 0, total = 0;
+    if (tid == 0) slots_there = tiles_there = 0, total = items_there = 0;
     __syncthreads();
 
     // Requests by rounds of as many as there are threads, their tiles by rounds too: f(a tile of this thread's, or one of no tokens), all threads
@@ -189,18 +193,29 @@ __global__ __launch_bounds__(SPLIT_THREADS) void paged_split_kernel(SplitArgs a)
     };
     auto price = [&](const Item &tile) { return tile.tokens <= a.half_tokens ? 5u : 8u; };
 
+    // a number of every thread, added up into `into`, which is 0
+    auto add_up = [&](unsigned long long x, unsigned long long *into) {
+#pragma unroll
+        for (int d = 32; d > 0; d /= 2) x += __shfl_xor(x, d);
+        if ((tid & 63) == 0 && x) atomicAdd(into, x);
+        __syncthreads();
+    };
     unsigned long long sum = 0;
     for_tiles([&](const Item &tile) { sum += tile.tokens ? static_cast<unsigned long long>(tile.key1) * price(tile) : 0; });
-#pragma unroll
-    for (int d = 32; d > 0; d /= 2) sum += __shfl_xor(sum, d);
-    if ((tid & 63) == 0 && sum) atomicAdd(&total, sum);
-    __syncthreads();
+    add_up(sum, &total);
     // what a part costs at most, and its keys
-    const unsigned long long fair = max(total / a.target + 1, static_cast<unsigned long long>(a.least) * 8);
+    unsigned long long fair = max(total / a.target + 1, static_cast<unsigned long long>(a.least) * 8);
     auto length_of = [&](const Item &tile) {
         const unsigned long long keys = fair / price(tile) + a.granule;
         return uint32_t(keys > 0x7fffffffu ? 0x7fffffffu : keys) / a.granule * a.granule;
     };
+    if (a.extra) {
+        // An item costs `extra` keys besides its own (its start and end, its sums through memory): a share of as many items as there now are
+        unsigned long long items = 0;
+        for_tiles([&](const Item &tile) { items += tile.tokens ? max((tile.key1 + length_of(tile) - 1) / length_of(tile), 1u) : 0; });
+        add_up(items, &items_there);
+        if (items_there > a.target) fair += (items_there - a.target) * 8 * a.extra / a.target;
+    }
     const float per_class = float(SIZES) / float(fair + 8ull * a.granule);
     auto class_of = [&](uint32_t keys, uint32_t price) { return SIZES - 1 - min(uint32_t(float(keys) * float(price) * per_class), SIZES - 1); };
     for_tiles([&](const Item &tile) {
@@ -903,7 +918,7 @@ template <int TYPE, int COLUMNS>
 __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, const Item *tiles) {
     typedef typename Row<TYPE>::value V;
     constexpr bool FEW = COLUMNS > 0;
-    constexpr uint32_t TILE = FEW ? COLUMNS * FEW_ROWS : CHUNK_ROWS, BY = FEW ? 4 : 1;
+    constexpr uint32_t TILE = FEW ? COLUMNS * FEW_ROWS : CHUNK_ROWS, BY = FEW ? 4 : 1, AT_ONCE = FEW ? 8 : 4;
     const uint32_t there = a.head->tiles, kv = blockIdx.z;
     const Item item = tiles[blockIdx.x];
     if (!(int(blockIdx.x < there) & int(item.parts > 1) & int(item_ok(a, item, item.parts)))) return;
@@ -918,23 +933,25 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, const Item
 
     float m = NO_MAXIMUM, l = 0.0f;
     floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t p0 = FEW ? wave : 0; p0 < item.parts; p0 += BY * 8) {
-        float2 ml[8];
-        floatx4 x[8];
+    for (uint32_t p0 = FEW ? wave : 0; p0 < item.parts; p0 += BY * AT_ONCE) {
+        float2 ml[AT_ONCE];
+        floatx4 x[AT_ONCE];
 #pragma unroll
-        for (uint32_t i = 0; i < 8; i++) {
-            const size_t at = slot + min(p0 + i * BY, item.parts - 1) * stride;
-            ml[i] = *reinterpret_cast<const float2 *>(a.part_ml + at * 2);
-            x[i] = *reinterpret_cast<const floatx4 *>(a.part_o + at * DIM + dim);
-            if (p0 + i * BY >= item.parts) ml[i] = float2{NO_MAXIMUM, 0.0f}, x[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t i = 0; i < AT_ONCE; i++) {
+            ml[i] = float2{NO_MAXIMUM, 0.0f}, x[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (p0 + i * BY < item.parts) {  // (for the wave alike)
+                const size_t at = slot + (p0 + i * BY) * stride;
+                ml[i] = *reinterpret_cast<const float2 *>(a.part_ml + at * 2);
+                x[i] = *reinterpret_cast<const floatx4 *>(a.part_o + at * DIM + dim);
+            }
         }
         float top = m;
 #pragma unroll
-        for (uint32_t i = 0; i < 8; i++) top = fmaxf(top, ml[i].x);
+        for (uint32_t i = 0; i < AT_ONCE; i++) top = fmaxf(top, ml[i].x);
         const float down = __builtin_amdgcn_exp2f(m - top);
         m = top, l *= down, o *= down;
 #pragma unroll
-        for (uint32_t i = 0; i < 8; i++) {
+        for (uint32_t i = 0; i < AT_ONCE; i++) {
             const float f = __builtin_amdgcn_exp2f(ml[i].x - top);
             l = fmaf(ml[i].y, f, l);
 #pragma unroll
@@ -1045,7 +1062,7 @@ extern "C" int saetta_paged_split(saetta_stream_t stream, saetta_paged_batch bat
     const bool few = s.columns > 0;
     const SplitArgs a = {batch, reinterpret_cast<SplitHead *>(at), reinterpret_cast<Item *>(at + items_offset()), reinterpret_cast<Item *>(at + tiles_offset(s)),
                          s.tile_tokens, s.target, s.most_items, s.most_joined, s.slots, p.tokens, p.rows,
-                         few, few ? STEP_KEYS * FEW_WAVES : STEP_KEYS, few ? STEP_KEYS * FEW_WAVES : 256u, few ? 0u : s.tile_tokens / 2};
+                         few, few ? STEP_KEYS * FEW_WAVES : STEP_KEYS, few ? STEP_KEYS * FEW_WAVES : 256u, few ? 0u : CHUNK_EXTRA, few ? 0u : s.tile_tokens / 2};
     launch(paged_split_kernel, dim3(1), dim3(SPLIT_THREADS), 0, as_stream(stream), a);
     return launch_status("paged_split");
 }
