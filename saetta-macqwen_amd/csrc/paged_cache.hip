@@ -8,7 +8,8 @@
 //
 // Store: memory-bound.  A workgroup takes one run of tokens inside one block (the first of the run's tokens finds that it is the
 // first from the slots alone), one kv head, keys or values: what shares an e is then one workgroup's, and its largest
-// magnitude is known before the first code is written, with the values held in registers.
+// magnitude is known before the first code is written, with the values held in registers.  A wave has four tokens of a unit, a lane four dims of
+// each: a load is a token's row, and what a wave stores of four tokens fills lines of 64 bytes.
 #include "common.hpp"
 #include "lanes.hpp"
 #include "paged_device.hpp"
@@ -17,108 +18,81 @@ namespace saetta {
 namespace {
 
 constexpr int STORE_THREADS = 256;
+// Up to this many tokens a workgroup looks at one, so that a step of single tokens is stored at once; more, where runs are long as a rule, by 16.
+constexpr uint32_t STORE_ALONE = 1024;
 
 struct StoreArgs {
     saetta_strided_rows x[2];  // keys, values
     const int32_t *slots;
     uint8_t *codes[2], *scales[2];
-    uint32_t blocks, block_tokens, kv_heads, tokens;
+    uint32_t blocks, block_tokens, kv_heads, tokens, span;
 };
 
-// Values of one unit of 16 tokens that a thread holds.  Keys: 16 dims of one token, a piece of 16 bytes.  Values: four dims
-// of four tokens, a dword of each of four pieces.
-struct KeyPlace {
-    static constexpr bool KEYS = true;
-    uint32_t token, dim;
-    __device__ __forceinline__ KeyPlace(uint32_t tid) : token(tid >> 4), dim((tid & 15) * 16) {}
-    __device__ __forceinline__ uint32_t byte() const { return dim / 64 * 1024 + (dim / 16 % 4 * 16 + token) * 16; }
-};
-struct ValuePlace {
-    static constexpr bool KEYS = false;
-    uint32_t token, dim;  // the first of four
-    // (lanes: dims of 64 side by side, 4 at a time, then the four 64s: what a token has is read whole)
-    __device__ __forceinline__ ValuePlace(uint32_t tid) : token((tid >> 6) * 4), dim((tid & 63) * 4) {}
-    __device__ __forceinline__ uint32_t byte() const { return dim / 64 * 1024 + (token / 4 * 16 + dim % 16) * 16 + dim / 16 % 4 * 4; }
-};
+// Where the four dims (from `dim` on) of token t, of keys, or dim `dim` of the four tokens from t on, of values, lie in a unit: a dword.
+__device__ __forceinline__ uint32_t key_dword(uint32_t t, uint32_t dim) { return dim / 64 * 1024 + (dim / 16 % 4 * 16 + t) * 16 + dim % 16; }
+__device__ __forceinline__ uint32_t value_dword(uint32_t t, uint32_t dim) { return dim / 64 * 1024 + (t / 4 * 16 + dim % 16) * 16 + dim / 16 % 4 * 4; }
 
-template <int TYPE, int UNITS, class Place>
-__device__ __forceinline__ void store_run(const StoreArgs &a, int which, uint32_t token, uint32_t head, uint32_t block, uint32_t offset, uint32_t count) {
+template <int TYPE, int UNITS, bool KEYS>
+__device__ __forceinline__ void store_run(const StoreArgs &a, uint32_t token, uint32_t head, uint32_t block, uint32_t offset, uint32_t count) {
     typedef typename Row<TYPE>::value V;
-    const uint32_t tid = threadIdx.x;
-    const Place place(tid);
+    constexpr int which = KEYS ? 0 : 1;
+    const uint32_t tid = threadIdx.x, token0 = (tid >> 6) * 4, dim = (tid & 63) * 4;
     const saetta_strided_rows &rows = a.x[which];
     // the run's token 0 sits at `offset`; token t of the block is row t - offset of the run
-    const V *x = static_cast<const V *>(rows.data) + uint64_t(token) * rows.token_stride + head * rows.head_stride + place.dim;
-    float held[UNITS][16];
+    const V *x = static_cast<const V *>(rows.data) + uint64_t(token) * rows.token_stride + head * rows.head_stride + dim;
+    const size_t at = size_t(block) * a.kv_heads + head;
+    uint8_t *scale = a.scales[which] + at;
+    const int before = int(*scale) - 127;
+    float held[UNITS][4][4];  // [unit][token][dim]
     float top = 0.0f;
 #pragma unroll
-    for (int u = 0; u < UNITS; u++) {
-        if constexpr (Place::KEYS) {
-            const uint32_t t = u * UNIT_TOKENS + place.token;
-            if (t >= offset && t < offset + count) load_values<TYPE, 16>(x + uint64_t(t - offset) * rows.token_stride, held[u]);
-            else {
+    for (int u = 0; u < UNITS; u++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) held[u][i] = 0.0f;
-            }
-        } else {
+        for (int i = 0; i < 4; i++) {
+            const uint32_t t = u * UNIT_TOKENS + token0 + i;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint32_t t = u * UNIT_TOKENS + place.token + i;
-                float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                if (t >= offset && t < offset + count) load_values<TYPE, 4>(x + uint64_t(t - offset) * rows.token_stride, v);
-#pragma unroll
-                for (int d = 0; d < 4; d++) held[u][4 * d + i] = v[d];
-            }
+            for (int d = 0; d < 4; d++) held[u][i][d] = 0.0f;
+            if (t >= offset && t < offset + count) load_values<TYPE, 4>(x + uint64_t(t - offset) * rows.token_stride, held[u][i]);
         }
+#pragma unroll
+    for (int u = 0; u < UNITS; u++)
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            const float m = fabsf(held[u][i]);
+            const float m = fabsf(held[u][i / 4][i % 4]);
             top = m < __builtin_inff() ? fmaxf(top, m) : top;
         }
-    }
     top = group_reduce<64>(top, MaxOp());
     __shared__ float tops[STORE_THREADS / 64];
+    __syncthreads();  // the last run's have been read
     if ((tid & 63) == 0) tops[tid >> 6] = top;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < STORE_THREADS / 64; w++) top = fmaxf(top, tops[w]);
 
-    const size_t at = size_t(block) * a.kv_heads + head;
-    uint8_t *scale = a.scales[which] + at;
-    const int before = int(*scale) - 127;
     int e = scale_exponent(top);
     if (offset > 0) e = max(e, min(max(before, LOWEST_EXPONENT), HIGHEST_EXPONENT));
     const bool raised = offset > 0 && e != before;
     const float down = power_of_two(-e), moved = power_of_two(max(before - e, -126));
     uint8_t *codes = a.codes[which] + at * (size_t(a.block_tokens) * SAETTA_HEAD_DIM);
+    auto rescaled = [&](uint32_t old) {
+        float v[4];
+        of_codes(old, v);
+        return to_codes(v[0] * moved, v[1] * moved, v[2] * moved, v[3] * moved);
+    };
 #pragma unroll
     for (int u = 0; u < UNITS; u++) {
-        const uint32_t first = u * UNIT_TOKENS;
-        // nothing of the unit is new, nor to be moved to another scale
-        if (first >= offset + count || (first + UNIT_TOKENS <= offset && !raised)) continue;
-        uint32_t w[4];
+        const uint32_t t = u * UNIT_TOKENS + token0;
+        // nothing of the four tokens is new, nor to be moved to another scale
+        if (t >= offset + count || (t + 4 <= offset && !raised)) continue;
+        uint8_t *unit = codes + u * UNIT_BYTES;
+        if constexpr (KEYS) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) w[i] = to_codes(held[u][4 * i] * down, held[u][4 * i + 1] * down, held[u][4 * i + 2] * down, held[u][4 * i + 3] * down);
-        uint8_t *to = codes + u * UNIT_BYTES + place.byte();
-        auto rescaled = [&](uint32_t old) {
-            float v[4];
-            of_codes(old, v);
-            return to_codes(v[0] * moved, v[1] * moved, v[2] * moved, v[3] * moved);
-        };
-        if constexpr (Place::KEYS) {
-            const uint32_t t = first + place.token;
-            if (t >= offset + count) continue;
-            uint4 *piece = reinterpret_cast<uint4 *>(to);
-            if (t >= offset) {
-                *piece = uint4{w[0], w[1], w[2], w[3]};
-            } else if (raised) {
-                const uint4 old = *piece;
-                *piece = uint4{rescaled(old.x), rescaled(old.y), rescaled(old.z), rescaled(old.w)};
+            for (int i = 0; i < 4; i++) {
+                uint32_t *p = reinterpret_cast<uint32_t *>(unit + key_dword(token0 + i, dim));
+                if (t + i >= offset + count || (t + i < offset && !raised)) continue;
+                *p = t + i >= offset ? to_codes(held[u][i][0] * down, held[u][i][1] * down, held[u][i][2] * down, held[u][i][3] * down) : rescaled(*p);
             }
         } else {
-            const uint32_t t = first + place.token;
-            if (t >= offset + count || (t + 4 <= offset && !raised)) continue;
-            const bool whole = t >= offset && t + 4 <= offset + count;
             uint32_t fresh = 0, earlier = 0;  // bytes of tokens that are new; of tokens before them
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -127,8 +101,9 @@ __device__ __forceinline__ void store_run(const StoreArgs &a, int which, uint32_
             }
 #pragma unroll
             for (int d = 0; d < 4; d++) {
-                uint32_t *p = reinterpret_cast<uint32_t *>(to + d * 16), value = w[d];
-                if (!whole) {
+                uint32_t *p = reinterpret_cast<uint32_t *>(unit + value_dword(token0, dim + d));
+                uint32_t value = to_codes(held[u][0][d] * down, held[u][1][d] * down, held[u][2][d] * down, held[u][3][d] * down);
+                if (fresh != ~0u) {
                     const uint32_t old = *p, kept = raised ? rescaled(old) : old;
                     value = (value & fresh) | (kept & earlier) | (old & ~(fresh | earlier));
                 }
@@ -136,36 +111,40 @@ __device__ __forceinline__ void store_run(const StoreArgs &a, int which, uint32_
             }
         }
     }
-    if (tid == 0) *scale = uint8_t(e + 127);
+    if (tid == 0) *scale = uint8_t(e + 127);  // (everyone has read it: there was a barrier since)
 }
 
+// A workgroup looks at a.span tokens and takes the runs that begin there, one after the other.
 template <int TYPE, int UNITS>
 __global__ __launch_bounds__(STORE_THREADS) void paged_store_kernel(StoreArgs a) {
-    const uint32_t token = blockIdx.x, head = blockIdx.y >> 1;
-    const int which = blockIdx.y & 1;
-    const uint32_t slot = uint32_t(a.slots[token]), bt = UNITS * UNIT_TOKENS;
-    const uint32_t block = slot / bt, offset = slot % bt;
-    if (block >= a.blocks) return;  // (-1 among them)
-    // the run's first token: what is before it in the call is in another block, or not the slot before
-    if (offset > 0 && token > 0 && uint32_t(a.slots[token - 1]) == slot - 1) return;
-    __shared__ uint32_t found;
-    // the tokens that follow it in the block, slot by slot: one wave looks at up to 64 at a time
-    if (threadIdx.x < 64) {
+    constexpr uint32_t BT = UNITS * UNIT_TOKENS;
+    const uint32_t head = blockIdx.y >> 1, lane = threadIdx.x & 63, first = blockIdx.x * a.span;
+    // Lane i: slot of token first + i; whether a run begins there: what is before it in the call is in another block, or not the slot before.
+    // (Every wave by itself: no barrier.)
+    uint32_t slot = ~0u;
+    bool begins = false;
+    if (lane < a.span && first + lane < a.tokens) {
+        const uint32_t t = first + lane;
+        slot = uint32_t(a.slots[t]);
+        const uint32_t prior = t > 0 ? uint32_t(a.slots[t - 1]) : ~0u;
+        begins = slot / BT < a.blocks && (slot % BT == 0 || t == 0 || prior != slot - 1);  // (-1 is in no block)
+    }
+    for (uint64_t runs = __ballot(begins); runs; runs &= runs - 1) {
+        const uint32_t i = uint32_t(__builtin_ctzll(runs)), token = first + i, from = __builtin_amdgcn_readlane(slot, i);
+        const uint32_t block = from / BT, offset = from % BT;
+        // the tokens that follow it in the block, slot by slot: up to 64 at a time
         uint32_t count = 1;
-        for (uint32_t i0 = 1; i0 < bt - offset; i0 += 64) {
-            const uint32_t i = i0 + threadIdx.x;
-            const bool follows = i < bt - offset && uint64_t(token) + i < a.tokens && uint32_t(a.slots[token + i]) == slot + i;
+        for (uint32_t j0 = 1; j0 < BT - offset; j0 += 64) {
+            const uint32_t j = j0 + lane;
+            const bool follows = j < BT - offset && uint64_t(token) + j < a.tokens && uint32_t(a.slots[token + j]) == from + j;
             const uint64_t all = __ballot(follows);
             const uint32_t n = all == ~0ull ? 64 : uint32_t(__builtin_ctzll(~all));
             count += n;
             if (n < 64) break;
         }
-        if (threadIdx.x == 0) found = count;
+        if (blockIdx.y & 1) store_run<TYPE, UNITS, false>(a, token, head, block, offset, count);
+        else store_run<TYPE, UNITS, true>(a, token, head, block, offset, count);
     }
-    __syncthreads();
-    const uint32_t count = found;
-    if (which == 0) store_run<TYPE, UNITS, KeyPlace>(a, 0, token, head, block, offset, count);
-    else store_run<TYPE, UNITS, ValuePlace>(a, 1, token, head, block, offset, count);
 }
 
 struct GatherArgs {
@@ -175,47 +154,54 @@ struct GatherArgs {
     uint32_t blocks, block_tokens, kv_heads, tokens;
 };
 
-// A workgroup takes 16 slots of one kv head, keys or values, a thread 16 dims of a slot.
+// A workgroup takes 16 slots of one kv head, keys or values: a wave a slot at a time, a lane four dims, so that a store is a whole row.
+// Where the slots lie in two units at most (16 that follow each other do), the units come through LDS by whole kilobytes, for values are stored
+// four tokens to a dword; else a lane reads its bytes where they are.
+constexpr uint32_t GATHER_SLOTS = 16;
 template <int TYPE>
 __global__ __launch_bounds__(256) void paged_gather_kernel(GatherArgs a) {
     typedef typename Row<TYPE>::value V;
-    const uint32_t tid = threadIdx.x, head = blockIdx.y >> 1, which = blockIdx.y & 1;
-    const uint64_t row = uint64_t(blockIdx.x) * 16 + (tid >> 4);
-    if (row >= a.tokens || a.out[which] == nullptr) return;
-    const uint32_t slot = uint32_t(a.slots[row]), block = slot / a.block_tokens;
-    if (block >= a.blocks) return;
-    const size_t at = size_t(block) * a.kv_heads + head;
-    const uint8_t *unit = a.codes[which] + at * (size_t(a.block_tokens) * SAETTA_HEAD_DIM) + slot % a.block_tokens / UNIT_TOKENS * UNIT_BYTES;
-    const float scale = power_of_two(int(a.scales[which][at]) - 127);
-    const uint32_t t = slot % UNIT_TOKENS, piece = tid & 15;  // dims 16 piece ..
-    float x[16];
-    if (which == 0) {
-        const uint4 w = *reinterpret_cast<const uint4 *>(unit + (piece >> 2) * 1024 + ((piece & 3) * 16 + t) * 16);
-        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            float v[4];
-            of_codes(ws[i], v);
-#pragma unroll
-            for (int j = 0; j < 4; j++) x[4 * i + j] = v[j] * scale;
-        }
-    } else {
-        const uint8_t *p = unit + (piece >> 2) * 1024 + (t >> 2) * 256 + (piece & 3) * 4 + (t & 3);
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const uint32_t w = uint32_t(p[i * 16]) | uint32_t(p[i * 16 + 16]) << 8 | uint32_t(p[i * 16 + 32]) << 16 | uint32_t(p[i * 16 + 48]) << 24;
-            float v[4];
-            of_codes(w, v);
-#pragma unroll
-            for (int j = 0; j < 4; j++) x[i + j] = v[j] * scale;
-        }
+    __shared__ __attribute__((aligned(16))) uint8_t units[2][UNIT_BYTES];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, head = blockIdx.y >> 1, which = blockIdx.y & 1;
+    if (a.out[which] == nullptr) return;
+    const uint64_t row0 = uint64_t(blockIdx.x) * GATHER_SLOTS;
+    // lane i (< 16): slot i; those that are not there take no part
+    uint32_t slot = ~0u;
+    if (lane < GATHER_SLOTS && row0 + lane < a.tokens) slot = uint32_t(a.slots[row0 + lane]);
+    const uint64_t there = __ballot(slot / a.block_tokens < a.blocks);
+    if (there == 0) return;
+    const uint32_t first = __builtin_amdgcn_readlane(slot, __builtin_ctzll(there)) / UNIT_TOKENS, last = __builtin_amdgcn_readlane(slot, 63 - __builtin_clzll(there)) / UNIT_TOKENS;
+    const bool near = (__ballot(slot / UNIT_TOKENS == first || slot / UNIT_TOKENS == last) & there) == there;
+    auto row_of = [&](uint32_t unit) { return size_t(unit / (a.block_tokens / UNIT_TOKENS)) * a.kv_heads + head; };
+    auto codes_of = [&](uint32_t unit) { return a.codes[which] + row_of(unit) * (size_t(a.block_tokens) * SAETTA_HEAD_DIM) + unit % (a.block_tokens / UNIT_TOKENS) * UNIT_BYTES; };
+    if (near) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(codes_of(first) + tid * 16), y = *reinterpret_cast<const uint4 *>(codes_of(last) + tid * 16);
+        *reinterpret_cast<uint4 *>(units[0] + tid * 16) = x, *reinterpret_cast<uint4 *>(units[1] + tid * 16) = y;
     }
-    store_values<TYPE, 16>(static_cast<V *>(a.out[which]) + (row * a.kv_heads + head) * SAETTA_HEAD_DIM + piece * 16, x);
+    __syncthreads();
+    const uint32_t dim = lane * 4;
+#pragma unroll
+    for (uint32_t k = 0; k < GATHER_SLOTS / 4; k++) {
+        const uint32_t i = wave * (GATHER_SLOTS / 4) + k;
+        if (!(there >> i & 1)) continue;
+        const uint32_t from = __builtin_amdgcn_readlane(slot, i), unit = from / UNIT_TOKENS, t = from % UNIT_TOKENS;
+        const float scale = power_of_two(int(a.scales[which][row_of(unit)]) - 127);
+        auto bytes = [&](const uint8_t *p) {
+            if (which == 0) return *reinterpret_cast<const uint32_t *>(p + key_dword(t, dim));
+            p += value_dword(t, dim) + t % 4;
+            return uint32_t(p[0]) | uint32_t(p[16]) << 8 | uint32_t(p[32]) << 16 | uint32_t(p[48]) << 24;
+        };
+        float x[4];
+        of_codes(near ? bytes(units[unit == first ? 0 : 1]) : bytes(codes_of(unit)), x);
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[j] *= scale;
+        store_values<TYPE, 4>(static_cast<V *>(a.out[which]) + ((row0 + i) * a.kv_heads + head) * SAETTA_HEAD_DIM + dim, x);
+    }
 }
 
 template <int TYPE>
 void launch_store(hipStream_t stream, const StoreArgs &a) {
-    const dim3 grid(a.tokens, a.kv_heads * 2);
+    const dim3 grid((a.tokens + a.span - 1) / a.span, a.kv_heads * 2);
     switch (a.block_tokens) {
         case 16: return launch(paged_store_kernel<TYPE, 1>, grid, dim3(STORE_THREADS), 0, stream, a);
         case 32: return launch(paged_store_kernel<TYPE, 2>, grid, dim3(STORE_THREADS), 0, stream, a);
@@ -242,7 +228,7 @@ extern "C" int saetta_paged_store(saetta_stream_t stream, int type, saetta_strid
     if (int rc = ensure_device()) return rc;
     if (tokens == 0) return SAETTA_OK;
     const StoreArgs a = {{keys, values}, slots, {cache.keys, cache.values}, {cache.key_scales, cache.value_scales},
-                         cache.blocks, cache.block_tokens, cache.kv_heads, tokens};
+                         cache.blocks, cache.block_tokens, cache.kv_heads, tokens, tokens <= STORE_ALONE ? 1u : UNIT_TOKENS};
     if (type == SAETTA_F32) launch_store<SAETTA_F32>(as_stream(stream), a);
     else if (type == SAETTA_F16) launch_store<SAETTA_F16>(as_stream(stream), a);
     else launch_store<SAETTA_BF16>(as_stream(stream), a);
@@ -259,7 +245,7 @@ extern "C" int saetta_paged_gather(saetta_stream_t stream, int type, saetta_page
     if (tokens == 0 || (!keys && !values)) return SAETTA_OK;
     const GatherArgs a = {{cache.keys, cache.values}, {cache.key_scales, cache.value_scales}, slots, {keys, values},
                           cache.blocks, cache.block_tokens, cache.kv_heads, tokens};
-    const dim3 grid((tokens + 15) / 16, cache.kv_heads * 2);
+    const dim3 grid((tokens + GATHER_SLOTS - 1) / GATHER_SLOTS, cache.kv_heads * 2);
     if (type == SAETTA_F32) launch(paged_gather_kernel<SAETTA_F32>, grid, dim3(256), 0, as_stream(stream), a);
     else if (type == SAETTA_F16) launch(paged_gather_kernel<SAETTA_F16>, grid, dim3(256), 0, as_stream(stream), a);
     else launch(paged_gather_kernel<SAETTA_BF16>, grid, dim3(256), 0, as_stream(stream), a);
