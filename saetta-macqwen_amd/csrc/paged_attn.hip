@@ -92,7 +92,6 @@ struct SplitArgs {
 // tokens 118 us with 0, 115 with 256, 110 with 512, 123 with 1024; a chunk beside drafts 365, 353, 352, 352 a layer.
 constexpr uint32_t CHUNK_EXTRA = 512;
 
-constexpr int SPLIT_THREADS = 1024, SPLIT_WAVES = SPLIT_THREADS / 64;
 constexpr uint32_t SIZES = 64;  // classes of items by what they cost
 
 // A request as the split sees it.
@@ -122,6 +121,7 @@ __device__ __forceinline__ Item tile_of(const SplitArgs &a, const Work &w, uint3
 }
 
 // x summed over the threads before this one; `all`: over all of them.  (All threads; `waves` is free again on return.)
+template <uint32_t SPLIT_THREADS>
 __device__ __forceinline__ uint32_t before_this(uint32_t x, uint32_t *waves, uint32_t &all) {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t through = x;
@@ -135,7 +135,7 @@ __device__ __forceinline__ uint32_t before_this(uint32_t x, uint32_t *waves, uin
     uint32_t before = 0;
     all = 0;
 #pragma unroll
-    for (uint32_t w = 0; w < SPLIT_WAVES; w++) {
+    for (uint32_t w = 0; w < SPLIT_THREADS / 64; w++) {
         if (w < wave) before += waves[w];
         all += waves[w];
     }
@@ -158,8 +158,9 @@ __device__ __forceinline__ uint32_t last_at_most(const uint32_t *starts, uint32_
 // and a rest; the items go out from the dearest class to the cheapest, so that who ends early takes what is small.  (One workgroup: a sum over the
 // tiles, a count of the classes, and the items themselves; the tiles by turns over its threads.  The places of the items in a class and of the
 // parts' sums follow from atomic counts, in any order: what is computed does not depend on them.)
+template <uint32_t SPLIT_THREADS>
 __global__ __launch_bounds__(SPLIT_THREADS) void paged_split_kernel(SplitArgs a) {
-    __shared__ uint32_t waves[SPLIT_WAVES], starts[SPLIT_THREADS], ends[SPLIT_THREADS], classes[SIZES], slots_there, tiles_there;
+    __shared__ uint32_t waves[SPLIT_THREADS / 64], starts[SPLIT_THREADS], ends[SPLIT_THREADS], classes[SIZES], slots_there, tiles_there;
     __shared__ unsigned long long total, items_there;
     __shared__ Item cut[SPLIT_THREADS];
     const uint32_t tid = threadIdx.x, requests = a.batch.requests;
@@ -175,7 +176,7 @@ __global__ __launch_bounds__(SPLIT_THREADS) void paged_split_kernel(SplitArgs a)
         if (found) return f(mine);
         for (uint32_t r0 = 0; r0 < requests; r0 += SPLIT_THREADS) {
             uint32_t all;
-            const uint32_t tiles = work_of(a, r0 + tid).tiles, before = before_this(tiles, waves, all), n = min(uint32_t(SPLIT_THREADS), requests - r0);
+            const uint32_t tiles = work_of(a, r0 + tid).tiles, before = before_this<SPLIT_THREADS>(tiles, waves, all), n = min(SPLIT_THREADS, requests - r0);
             starts[tid] = before;
             __syncthreads();
             for (uint32_t k0 = 0; k0 < all; k0 += SPLIT_THREADS) {
@@ -248,7 +249,7 @@ __global__ __launch_bounds__(SPLIT_THREADS) void paged_split_kernel(SplitArgs a)
             if (t < a.most_joined) a.tiles[t] = tile;
         }
         uint32_t all;
-        ends[tid] = before_this(tile.parts, waves, all);
+        ends[tid] = before_this<SPLIT_THREADS>(tile.parts, waves, all);
         cut[tid] = tile;
         __syncthreads();
         for (uint32_t k = tid; k < all; k += SPLIT_THREADS) {
@@ -1063,7 +1064,9 @@ extern "C" int saetta_paged_split(saetta_stream_t stream, saetta_paged_batch bat
     const SplitArgs a = {batch, reinterpret_cast<SplitHead *>(at), reinterpret_cast<Item *>(at + items_offset()), reinterpret_cast<Item *>(at + tiles_offset(s)),
                          s.tile_tokens, s.target, s.most_items, s.most_joined, s.slots, p.tokens, p.rows,
                          few, few ? STEP_KEYS * FEW_WAVES : STEP_KEYS, few ? STEP_KEYS * FEW_WAVES : 256u, few ? 0u : CHUNK_EXTRA, few ? 0u : s.tile_tokens / 2};
-    launch(paged_split_kernel, dim3(1), dim3(SPLIT_THREADS), 0, as_stream(stream), a);
+    // (few tiles: four waves, whose barriers are cheaper)
+    if (s.most_tiles <= 256) launch(paged_split_kernel<256>, dim3(1), dim3(256), 0, as_stream(stream), a);
+    else launch(paged_split_kernel<1024>, dim3(1), dim3(1024), 0, as_stream(stream), a);
     return launch_status("paged_split");
 }
 

@@ -5,8 +5,8 @@
 // more gives the rest back behind what is left of the list, in the same order (another prefix sum).  So what a step takes
 // and the next gives back whole leaves the list as it was.  The tokens' first rows are a third prefix sum.
 //
-// Bound by latency: a few bytes a request, two numbers a token.  The sums want every request, so one workgroup of 1024
-// makes them, requests 1024 at a time, and moves the blocks' numbers, entry by entry over all its threads (a request is
+// Bound by latency: a few bytes a request, two numbers a token.  The sums want every request, so one workgroup
+// makes them, a request a thread, and moves the blocks' numbers, entry by entry over all its threads (a request is
 // found by bisection in the prefix sums in LDS).  The tokens' slots are independent of each other: a second launch of as
 // many workgroups as they fill, or, where few workgroups' worth of tokens come (a decode step), the first does them itself.
 #include "common.hpp"
@@ -16,8 +16,8 @@
 namespace saetta {
 namespace {
 
-constexpr int TABLE_THREADS = 1024, TABLE_WAVES = TABLE_THREADS / 64;
-constexpr uint32_t SLOT_TOKENS = 1024;  // of a workgroup of the second launch
+constexpr uint32_t SLOT_TOKENS = 256;  // of a workgroup of the second launch, one a thread
+constexpr uint32_t AT_ONCE = 4;         // blocks' numbers that a thread has on their way
 
 struct TablesArgs {
     const uint32_t *context_lens, *new_lens;
@@ -30,6 +30,7 @@ struct TablesArgs {
 __device__ __forceinline__ uint32_t add_up(uint32_t a, uint32_t b) { return a + b < a ? 0xffffffffu : a + b; }
 
 // x summed over the threads before this one; `all`: over all of them.  (All threads; `waves` is free again on return.)
+template <uint32_t TABLE_THREADS>
 __device__ __forceinline__ uint32_t sum_before(uint32_t x, uint32_t *waves, uint32_t &all) {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t through = x;
@@ -43,7 +44,7 @@ __device__ __forceinline__ uint32_t sum_before(uint32_t x, uint32_t *waves, uint
     uint32_t before = 0;
     all = 0;
 #pragma unroll
-    for (uint32_t w = 0; w < TABLE_WAVES; w++) {
+    for (uint32_t w = 0; w < TABLE_THREADS / 64; w++) {
         if (w == wave) before = all;
         all = add_up(all, waves[w]);
     }
@@ -66,8 +67,7 @@ __device__ __forceinline__ Lengths lengths_of(const TablesArgs &a, uint32_t r) {
 }
 
 // The last of `starts` (rising, starts[0] <= x) that is no more than x.
-template <class T>
-__device__ __forceinline__ uint32_t last_at_most(const T *starts, uint32_t n, uint32_t x) {
+__device__ __forceinline__ uint32_t last_at_most(const uint32_t *starts, uint32_t n, uint32_t x) {
     uint32_t low = 0;
     while (n > 1) {
         const uint32_t half = n / 2;
@@ -76,29 +76,36 @@ __device__ __forceinline__ uint32_t last_at_most(const T *starts, uint32_t n, ui
     }
     return low;
 }
-
-// Token t's slot and position (-1 past the step's last token).  Whether it has a slot.
-__device__ __forceinline__ bool place_token(const TablesArgs &a, uint32_t t, uint32_t total) {
-    int32_t slot = -1, position = -1;
-    if (t < total) {
-        // (requests without new tokens share their start with the next: the last of them is the token's)
-        const uint32_t r = last_at_most(a.step.query_starts, a.p.requests, t), bt = a.p.block_tokens;
-        // (from the sum and not from context_lens, which kv_lens may be: those have grown by now)
-        const uint32_t context = a.step.kv_lens[r] - a.new_lens[r], at = add_up(context, t - a.step.query_starts[r]);
-        position = int32_t(min(at, 0x7fffffffu));
-        const uint32_t entry = at / bt;
-        if (entry < min(a.state.held[r], a.p.max_blocks)) {
-            const uint32_t block = uint32_t(a.state.block_table[size_t(r) * a.p.max_blocks + entry]);
-            if (block < a.p.blocks) slot = int32_t(block * bt + at % bt);
-        }
+// The same by a wave at once, 64 places a look, over memory.
+__device__ __forceinline__ uint32_t wave_last_at_most(const uint32_t *starts, uint32_t n, uint32_t x) {
+    uint32_t low = 0;
+    const uint32_t lane = threadIdx.x & 63;
+    while (n > 1) {
+        const uint32_t each = (n + 63) / 64, at = lane * each;  // (lane 0's is one that is no more than x)
+        const uint32_t found = 63 - uint32_t(__builtin_clzll(__ballot(at < n && (lane == 0 || starts[low + min(at, n - 1)] <= x)) | 1));
+        low += found * each, n = min(each, n - found * each);
     }
-    a.step.slots[t] = slot, a.step.positions[t] = position;
-    return slot >= 0;
+    return low;
 }
 
-template <bool SLOTS>
+// Slot and position of token t of request r, `at` tokens behind the request's first, of a request that holds `held` blocks.
+__device__ __forceinline__ void place_token(const TablesArgs &a, uint32_t t, uint32_t r, uint32_t at, uint32_t held) {
+    const uint32_t bt = a.p.block_tokens, entry = at / bt;
+    int32_t slot = -1;
+    if (entry < held) {
+        const uint32_t block = uint32_t(a.state.block_table[size_t(r) * a.p.max_blocks + entry]);
+        if (block < a.p.blocks) slot = int32_t(block * bt + at % bt);
+    }
+    a.step.slots[t] = slot, a.step.positions[t] = int32_t(min(at, 0x7fffffffu));
+}
+__device__ __forceinline__ void place_nothing(const TablesArgs &a, uint32_t t) { a.step.slots[t] = a.step.positions[t] = -1; }
+
+template <bool SLOTS, uint32_t TABLE_THREADS>
 __global__ __launch_bounds__(TABLE_THREADS) void paged_tables_kernel(TablesArgs a) {
-    __shared__ uint32_t waves[TABLE_WAVES], starts[TABLE_THREADS], firsts[TABLE_THREADS];
+    auto sum_before = [](uint32_t x, uint32_t *waves, uint32_t &all) { return saetta::sum_before<TABLE_THREADS>(x, waves, all); };
+    __shared__ uint32_t waves[TABLE_THREADS / 64], starts[TABLE_THREADS], firsts[TABLE_THREADS];
+    // of a step of one round of requests: their first tokens, contexts and blocks, for the tokens' slots
+    __shared__ uint32_t tokens_from[SLOTS ? TABLE_THREADS : 1], contexts[SLOTS ? TABLE_THREADS : 1], holds[SLOTS ? TABLE_THREADS : 1];
     const uint32_t tid = threadIdx.x, requests = a.p.requests, room = a.p.tokens;
     const uint32_t free_count = min(*a.state.free_count, a.p.blocks);
 
@@ -116,7 +123,7 @@ __global__ __launch_bounds__(TABLE_THREADS) void paged_tables_kernel(TablesArgs 
     total = min(all_tokens, room);
 
     // blocks that are taken; the requests' first tokens and lengths
-    uint32_t takes_before = 0, tokens_before = 0;
+    uint32_t takes_before = 0, tokens_before = 0, placed = 0;
     for (uint32_t r0 = 0; r0 < requests; r0 += TABLE_THREADS) {
         const uint32_t r = r0 + tid;
         const Lengths l = lengths_of(a, r);
@@ -129,19 +136,35 @@ __global__ __launch_bounds__(TABLE_THREADS) void paged_tables_kernel(TablesArgs 
         if (r < requests) {
             a.step.query_starts[r] = min(token, room);
             a.step.kv_lens[r] = add_up(l.context, l.fresh);
-            if (take > 0) a.state.held[r] = l.held + min(take, taken - min(before, taken));
+            const uint32_t held = l.held + min(take, taken - min(before, taken));
+            if (take > 0) a.state.held[r] = held;
+            // tokens that its blocks have places for, and the step room
+            const uint32_t places = min(held, l.want) * a.p.block_tokens;
+            if (token < room && l.context < places) placed += min(min(l.fresh, room - token), places - l.context);
+            if constexpr (SLOTS) tokens_from[tid] = min(token, room), contexts[tid] = l.context, holds[tid] = min(held, l.want);
         }
         if (here == 0) continue;  // (for all threads alike)
         starts[tid] = before, firsts[tid] = l.held;
         __syncthreads();
-        const uint32_t first = starts[0], end = min(takes_before, taken), n = min(TABLE_THREADS, int(requests - r0));
-        for (uint32_t k = first + tid; k < end; k += TABLE_THREADS) {
-            const uint32_t i = last_at_most(starts, n, k);
-            a.state.block_table[size_t(r0 + i) * a.p.max_blocks + firsts[i] + (k - starts[i])] = a.state.free_list[left + k];
+        const uint32_t first = starts[0], end = min(takes_before, taken), n = min(TABLE_THREADS, requests - r0);
+        for (uint32_t k0 = first + tid; k0 < end; k0 += AT_ONCE * TABLE_THREADS) {
+            int32_t block[AT_ONCE];
+#pragma unroll
+            for (uint32_t j = 0; j < AT_ONCE; j++) block[j] = a.state.free_list[left + min(k0 + j * TABLE_THREADS, end - 1)];
+#pragma unroll
+            for (uint32_t j = 0; j < AT_ONCE; j++) {
+                const uint32_t k = k0 + j * TABLE_THREADS;
+                if (k >= end) break;
+                const uint32_t i = last_at_most(starts, n, k);
+                a.state.block_table[size_t(r0 + i) * a.p.max_blocks + firsts[i] + (k - starts[i])] = block[j];
+            }
         }
         __syncthreads();
     }
+    uint32_t all_placed;
+    sum_before(placed, waves, all_placed);
     if (tid == 0) {
+        *a.step.unplaced = all_tokens - all_placed;
         a.step.query_starts[requests] = total;
         *a.state.free_count = min(add_up(left, all_gives), a.p.blocks);
     }
@@ -165,13 +188,23 @@ __global__ __launch_bounds__(TABLE_THREADS) void paged_tables_kernel(TablesArgs 
             if (here == 0) continue;
             starts[tid] = before, firsts[tid] = l.want;
             __syncthreads();
-            const uint32_t first = starts[0], n = min(TABLE_THREADS, int(requests - r0));
-            for (uint32_t k = first + tid; k < gives_before; k += TABLE_THREADS) {
-                const uint32_t i = last_at_most(starts, n, k);
-                int32_t *entry = a.state.block_table + size_t(r0 + i) * a.p.max_blocks + firsts[i] + (k - starts[i]);
-                // (more than the list has room for: a table that names blocks twice; they are lost, not written past its end)
-                if (left + k < a.p.blocks) a.state.free_list[left + k] = *entry;
-                *entry = -1;
+            const uint32_t first = starts[0], n = min(TABLE_THREADS, requests - r0);
+            for (uint32_t k0 = first + tid; k0 < gives_before; k0 += AT_ONCE * TABLE_THREADS) {
+                int32_t *entry[AT_ONCE], block[AT_ONCE];
+#pragma unroll
+                for (uint32_t j = 0; j < AT_ONCE; j++) {
+                    const uint32_t k = min(k0 + j * TABLE_THREADS, gives_before - 1), i = last_at_most(starts, n, k);
+                    entry[j] = a.state.block_table + size_t(r0 + i) * a.p.max_blocks + firsts[i] + (k - starts[i]);
+                    block[j] = *entry[j];
+                }
+#pragma unroll
+                for (uint32_t j = 0; j < AT_ONCE; j++) {
+                    const uint32_t k = k0 + j * TABLE_THREADS;
+                    if (k >= gives_before) break;
+                    // (more than the list has room for: a table that names blocks twice; they are lost, not written past its end)
+                    if (left + k < a.p.blocks) a.state.free_list[left + k] = block[j];
+                    *entry[j] = -1;
+                }
             }
             __syncthreads();
             if (give > 0) a.state.held[r] = l.want;
@@ -180,27 +213,39 @@ __global__ __launch_bounds__(TABLE_THREADS) void paged_tables_kernel(TablesArgs 
 
     if constexpr (SLOTS) {
         __syncthreads();
-        uint32_t placed = 0;
-        for (uint32_t t = tid; t < room; t += TABLE_THREADS) placed += place_token(a, t, total);
-        uint32_t all;
-        sum_before(placed, waves, all);
-        if (tid == 0) *a.step.unplaced = all_tokens - all;
-    } else {
-        if (tid == 0) *a.step.unplaced = all_tokens;  // the second launch takes off what it places
+        for (uint32_t t = tid; t < room; t += TABLE_THREADS) {
+            if (t < total) {
+                // (requests without new tokens share their start with the next: the last of them is the token's)
+                const uint32_t r = last_at_most(tokens_from, requests, t);
+                place_token(a, t, r, add_up(contexts[r], t - tokens_from[r]), holds[r]);
+            } else {
+                place_nothing(a, t);
+            }
+        }
     }
 }
 
-// The second launch: SLOT_TOKENS tokens a workgroup.
-__global__ __launch_bounds__(256) void paged_slots_kernel(TablesArgs a) {
-    const uint32_t total = a.step.query_starts[a.p.requests];
-    uint32_t placed = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < SLOT_TOKENS; i += 256) {
-        const uint64_t t = uint64_t(blockIdx.x) * SLOT_TOKENS + i + threadIdx.x;
-        const bool has = t < a.p.tokens && place_token(a, uint32_t(t), total);
-        placed += __popcll(__ballot(has));
+// The second launch: SLOT_TOKENS tokens a workgroup.  The requests that they belong to are those between the first token's and the last's.
+__global__ __launch_bounds__(SLOT_TOKENS) void paged_slots_kernel(TablesArgs a) {
+    constexpr uint32_t HELD = 1024;
+    __shared__ uint32_t starts[HELD];
+    const uint32_t *query_starts = a.step.query_starts, total = query_starts[a.p.requests], t0 = blockIdx.x * SLOT_TOKENS;
+    uint32_t first = 0, n = 1;
+    if (t0 < total) {
+        first = wave_last_at_most(query_starts, a.p.requests, t0);
+        n = first + wave_last_at_most(query_starts + first, a.p.requests - first, min(t0 + SLOT_TOKENS, total) - 1) + 1 - first;
+        for (uint32_t i = threadIdx.x; i < min(n, HELD); i += SLOT_TOKENS) starts[i] = query_starts[first + i];
     }
-    if ((threadIdx.x & 63) == 0 && placed > 0) atomicSub(a.step.unplaced, placed);  // (whole numbers: any order gives the same)
+    __syncthreads();
+    const uint32_t t = t0 + threadIdx.x;
+    if (t < total) {
+        const uint32_t r = first + (n <= HELD ? last_at_most(starts, n, t) : last_at_most(query_starts + first, n, t));
+        // (the context from the sum and not from context_lens, which kv_lens may be: those have grown by now)
+        const uint32_t context = a.step.kv_lens[r] - a.new_lens[r];
+        place_token(a, t, r, add_up(context, t - query_starts[r]), min(a.state.held[r], a.p.max_blocks));
+    } else if (t < a.p.tokens) {
+        place_nothing(a, t);
+    }
 }
 
 }  // namespace
@@ -228,12 +273,14 @@ extern "C" int saetta_paged_tables(saetta_stream_t stream, const uint32_t *conte
     SAETTA_REQUIRE(p.requests < (1u << 24) && p.tokens < (1u << 31), SAETTA_E_SHAPE, "paged_tables: %u requests, room for %u tokens", p.requests, p.tokens);
     if (int rc = ensure_device()) return rc;
     const TablesArgs a = {context_lens, new_lens, state, step, p};
-    // (one workgroup's slots: 1024 at a time)
-    if (p.tokens <= 2 * TABLE_THREADS) {
-        launch(paged_tables_kernel<true>, dim3(1), dim3(TABLE_THREADS), 0, as_stream(stream), a);
+    // One workgroup's slots, of requests that it has in LDS, or two launches.  A small step's workgroup is four waves, whose barriers are cheaper.
+    if (p.tokens <= 512 && p.requests <= 256) {
+        launch(paged_tables_kernel<true, 256>, dim3(1), dim3(256), 0, as_stream(stream), a);
+    } else if (p.tokens <= 2048 && p.requests <= 1024) {
+        launch(paged_tables_kernel<true, 1024>, dim3(1), dim3(1024), 0, as_stream(stream), a);
     } else {
-        launch(paged_tables_kernel<false>, dim3(1), dim3(TABLE_THREADS), 0, as_stream(stream), a);
-        launch(paged_slots_kernel, dim3((p.tokens + SLOT_TOKENS - 1) / SLOT_TOKENS), dim3(256), 0, as_stream(stream), a);
+        launch(paged_tables_kernel<false, 1024>, dim3(1), dim3(1024), 0, as_stream(stream), a);
+        launch(paged_slots_kernel, dim3((p.tokens + SLOT_TOKENS - 1) / SLOT_TOKENS), dim3(SLOT_TOKENS), 0, as_stream(stream), a);
     }
     return launch_status("paged_tables");
 }
