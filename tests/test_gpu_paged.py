@@ -142,6 +142,25 @@ def test_store_and_gather(dtype, block, kv_heads):
             assert torch.equal(o, torch.tensor(x, dtype=out_type, device="cuda"))
 
 
+def test_store_of_many_short_runs():
+    """More tokens than workgroups of their own: runs of one to a few tokens, blocks begun anew and continued, in one call."""
+    gen = np.random.default_rng(41)
+    cache, want = saetta.PagedCache(2, DIM, 900, 16), Cache(2, 900, 16)
+    for call in range(2):
+        pieces = []
+        for _ in range(700):
+            at = 0 if call == 0 else int(gen.integers(0, 16))
+            pieces.append((at, int(gen.integers(1, 17 - at))))
+        slots = runs_of(gen, 900, 16, pieces)
+        assert len(slots) > 1500
+        k, v = values_of(gen, len(slots), 2, F16), values_of(gen, len(slots), 2, F16)
+        cache.encode(k, v, ints(slots))
+        want.store(numbers(k), numbers(v), slots)
+    got = Cache.of(cache)
+    for w in ("keys", "values"):
+        assert np.array_equal(got.e[w], want.e[w]) and np.array_equal(got.rows[w], want.rows[w])
+
+
 def test_store_of_no_numbers_and_the_range():
     """Not finite: NaN, and the others' scale is theirs.  Zero, the smallest, the largest, past the range."""
     cache = saetta.PagedCache(1, DIM, 2, 16)
@@ -291,6 +310,19 @@ def test_scales_that_differ_widely():
         loud[32:48] = 0.0
         k, v = gen.standard_normal((2, len(b.slots), 2, DIM)) * loud
         b.cache.encode(torch.tensor(np.clip(k, -4, 4), dtype=F32, device="cuda"), torch.tensor(v, dtype=F32, device="cuda"), ints(b.slots))
+        b.run()
+        b.compare()
+
+
+def test_many_small_weights_beside_a_large_one():
+    """20000 keys whose weights are subnormal in f16 beside one of weight 1: together they are half of the output."""
+    for new in (1, 9):
+        b = Batch(31, [20000], [new], 64, 16, 2, F16, gate=False)
+        b.q.zero_(), b.q[..., 0].fill_(16.0)
+        n = len(b.slots)
+        k, v = torch.zeros(n, 2, DIM, device="cuda"), torch.ones(n, 2, DIM, device="cuda")
+        k[777, :, 0], v[777] = 10.0, -1.0  # a score of 10 above the others': 4.5e-5 of weight each, 0.9 of the largest together
+        b.cache.encode(k, v, ints(b.slots))
         b.run()
         b.compare()
 
