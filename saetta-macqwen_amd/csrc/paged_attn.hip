@@ -34,8 +34,8 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int DIM = SAETTA_HEAD_DIM;
 #include "prefill_stream.hpp"  // scores_block, stream_block_alone, settle
-constexpr float NO_SCORE = -1e30f;               // of a key that a row does not see
-constexpr float NO_MAXIMUM = 0.25f * NO_SCORE;   // where nothing was seen: 2^(NO_SCORE - NO_MAXIMUM) is 0
+constexpr float NO_SCORE = -__builtin_inff();    // of a key that a row does not see
+constexpr float NO_MAXIMUM = -1e30f;             // where nothing was seen: 2^(NO_SCORE - NO_MAXIMUM) is 0
 constexpr float TAU = 8.0f;                      // the reference maximum is raised only past this many powers of two
 constexpr uint32_t STEP_KEYS = 32;               // keys of a step: two units
 constexpr uint32_t FEW_ROWS = 16, CHUNK_ROWS = 256;  // FEW_ROWS: of a group of columns; a tile of few rows has 1, 2 or 4 groups
@@ -525,11 +525,6 @@ __global__ __launch_bounds__(few_threads(TILE_COLUMNS), TILE_COLUMNS == 2 ? 1 : 
             u32x4 w[COLUMNS];
 #pragma unroll
             for (int g = 0; g < COLUMNS; g++) {
-                float p[2][4], top = NO_SCORE;
-#pragma unroll
-                for (int i = 0; i < 2; i++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) p[i][r] = fmaf(s[g][i][r], ck[i], float(ev[i]));
                 if (masked) {
                     // keys of the step that the row sees, less the quarter's four; none of a unit that is not there
                     const int n = min(sees[g], int(item.key1)) - int(key + (at >> 4) * 4);
@@ -537,13 +532,13 @@ __global__ __launch_bounds__(few_threads(TILE_COLUMNS), TILE_COLUMNS == 2 ? 1 : 
                     for (int i = 0; i < 2; i++) {
                         const int seen = scale[i] & 0x10000 ? n - i * int(UNIT_TOKENS) : -1;
 #pragma unroll
-                        for (int r = 0; r < 4; r++) p[i][r] = r < seen ? p[i][r] : NO_SCORE;
+                        for (int r = 0; r < 4; r++) s[g][i][r] = r < seen ? s[g][i][r] : NO_SCORE;
                     }
                 }
+                // (the scale is a power of two times a positive number: a unit's largest score is that of its largest product)
+                float top = NO_SCORE;
 #pragma unroll
-                for (int i = 0; i < 2; i++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) top = fmaxf(top, p[i][r]);
+                for (int i = 0; i < 2; i++) top = fmaxf(top, fmaf(fmaxf(fmaxf(s[g][i][0], s[g][i][1]), fmaxf(s[g][i][2], s[g][i][3])), ck[i], float(ev[i])));
                 top = across_rows<16, 64>(top, MaxOp());
                 if (__any(top > m[g] + TAU)) {
                     const float next = top > m[g] + TAU ? top : m[g], down = __builtin_amdgcn_exp2f(m[g] - next);
@@ -551,11 +546,11 @@ __global__ __launch_bounds__(few_threads(TILE_COLUMNS), TILE_COLUMNS == 2 ? 1 : 
 #pragma unroll
                     for (int i = 0; i < 16; i++) acc[g][i] *= down;
                 }
-                float part[2] = {0.0f, 0.0f};
+                float p[2][4], part[2] = {0.0f, 0.0f};
 #pragma unroll
                 for (int i = 0; i < 2; i++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) p[i][r] = __builtin_amdgcn_exp2f(p[i][r] - m[g]), part[i] += p[i][r];
+                    for (int r = 0; r < 4; r++) p[i][r] = __builtin_amdgcn_exp2f(fmaf(s[g][i][r], ck[i], float(ev[i]) - m[g])), part[i] += p[i][r];
                 l[g] = fmaf(part[0], power_of_two(-ev[0]), fmaf(part[1], power_of_two(-ev[1]), l[g]));
                 w[g] = u32x4{pack_half2(p[0][0], p[0][1]), pack_half2(p[0][2], p[0][3]), pack_half2(p[1][0], p[1][1]), pack_half2(p[1][2], p[1][3])};
             }
@@ -742,12 +737,10 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
     auto softmax = [&](floatx16 &s, uint32_t step, half8 (&p)[2]) {
         const uint32_t key = (unit0 + 2 * step) * UNIT_TOKENS;
         const uint32_t scale[2] = {uint32_t(__builtin_amdgcn_readlane(scales, 2 * step % 64)), uint32_t(__builtin_amdgcn_readlane(scales, (2 * step + 1) % 64))};
-        float ck[2], sum[2] = {0.0f, 0.0f}, top = NO_SCORE;
+        float ck[2], sum[2] = {0.0f, 0.0f}, tops[2] = {NO_SCORE, NO_SCORE};
         int ev[2];
 #pragma unroll
         for (int i = 0; i < 2; i++) ck[i] = c * key_scale(scale[i]), ev[i] = value_exponent(scale[i]);
-#pragma unroll
-        for (int r = 0; r < 16; r++) s[r] = fmaf(s[r], ck[r >> 3], float(ev[r >> 3]));
         if (key + STEP_KEYS > wave_all || !(scale[0] & scale[1] & 0x10000)) {
             // keys of the step that the row sees, less the lane half's four; none of a unit that is not there
             const int n = min(sees, int(item.key1)) - int(key) - 4 * int(here() >> 5);
@@ -755,9 +748,10 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
 #pragma unroll
             for (int r = 0; r < 16; r++) s[r] = int((r & 3) + 8 * (r >> 2)) < (r < 8 ? seen[0] : seen[1]) ? s[r] : NO_SCORE;
         }
+        // (the scale is a power of two times a positive number: a unit's largest score is that of its largest product)
 #pragma unroll
-        for (int r = 0; r < 16; r++) top = fmaxf(top, s[r]);
-        top = across_rows<32, 64>(top, MaxOp());
+        for (int r = 0; r < 16; r++) tops[r >> 3] = fmaxf(tops[r >> 3], s[r]);
+        const float top = across_rows<32, 64>(fmaxf(fmaf(tops[0], ck[0], float(ev[0])), fmaf(tops[1], ck[1], float(ev[1]))), MaxOp());
         if (__any(top > m + TAU)) {
             const float next = top > m + TAU ? top : m, down = __builtin_amdgcn_exp2f(m - next);
             m = next, l *= down;
@@ -765,7 +759,7 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
             for (int i = 0; i < 8; i++) acc[i] *= down;
         }
 #pragma unroll
-        for (int r = 0; r < 16; r++) s[r] = __builtin_amdgcn_exp2f(s[r] - m), sum[r >> 3] += s[r];
+        for (int r = 0; r < 16; r++) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], ck[r >> 3], float(ev[r >> 3]) - m)), sum[r >> 3] += s[r];
         l = fmaf(sum[0], power_of_two(-ev[0]), fmaf(sum[1], power_of_two(-ev[1]), l));
 #pragma unroll
         for (int sp = 0; sp < 2; sp++) {
