@@ -614,7 +614,7 @@ typedef struct saetta_strided_rows {
  * become what they stand for times 2^(their e - e), rounded to nearest even like the new ones; e falls only when the
  * block begins anew.  A value that is not finite, or larger than 448 * 2^60, is stored as NaN.  The tokens of one block follow each other
  * in the call, at rising slots without a gap, as saetta_paged_tables gives them; what a block holds that a call
- * names by two such runs is undefined. */
+ * names by two such runs is undefined.  tokens < 2^28, as for saetta_paged_gather. */
 int saetta_paged_store(saetta_stream_t stream, int type, saetta_strided_rows keys, saetta_strided_rows values,
                        const int32_t *slots, saetta_paged_cache cache, uint32_t tokens);
 
@@ -638,9 +638,9 @@ typedef struct saetta_paged_attn_params {
     uint32_t heads;
     uint32_t kv_heads;
     uint32_t tokens; /* rows of q and out: the room for a step's new tokens */
-    uint32_t rows;   /* the most new tokens that a request has; with up to 16 (tokens * q heads per kv head) a
+    uint32_t rows;   /* the most new tokens that a request has; with up to 64 (tokens * q heads per kv head) a
                         kernel for few rows runs, with more one for chunks, which takes any mixture */
-    float scale;
+    float scale;     /* 2^-60 to 2^60 */
 } saetta_paged_attn_params;
 
 /* Bytes of `split` and of `workspace` for calls with these parameters and up to `requests` requests, for the current

@@ -986,8 +986,10 @@ int check_attn(const saetta_paged_attn_params &p, uint32_t requests, const char 
     SAETTA_REQUIRE(group == 1 || group == 2 || group == 4 || group == 8 || group == 16, SAETTA_E_SHAPE, "%s: %u q heads per kv head (1, 2, 4, 8 or 16)", what, group);
     SAETTA_REQUIRE(p.tokens < (1u << 31) && requests < (1u << 24), SAETTA_E_SHAPE, "%s: %u tokens of %u requests", what, p.tokens, requests);
     SAETTA_REQUIRE(p.rows > 0, SAETTA_E_SHAPE, "%s: rows 0", what);
-    // (one workgroup to an item and kv head)
-    SAETTA_REQUIRE(uint64_t(shape_of(p, requests).most_items) * p.kv_heads < (1u << 31), SAETTA_E_SHAPE, "%s: %u tokens of %u requests over %u kv heads", what,
+    // (the largest score is taken from the largest product)
+    SAETTA_REQUIRE(p.scale >= 0x1p-60f && p.scale <= 0x1p60f, SAETTA_E_SHAPE, "%s: scale %g (2^-60 to 2^60)", what, double(p.scale));
+    // (one workgroup of up to 512 threads to an item and kv head: fewer than 2^32 threads)
+    SAETTA_REQUIRE(uint64_t(shape_of(p, requests).most_items) * p.kv_heads < (1u << 23), SAETTA_E_SHAPE, "%s: %u tokens of %u requests over %u kv heads", what,
                    p.tokens, requests, p.kv_heads);
     return SAETTA_OK;
 }

@@ -225,6 +225,7 @@ extern "C" int saetta_paged_store(saetta_stream_t stream, int type, saetta_strid
     if (int rc = check_cache(cache, "paged_store")) return rc;
     SAETTA_REQUIRE(aligned(slots, 4) && rows_aligned(keys, type) && rows_aligned(values, type), SAETTA_E_ALIGN,
                    "paged_store: keys and values must be 16-byte aligned, with strides of multiples of 16 bytes");
+    SAETTA_REQUIRE(tokens < (1u << 28), SAETTA_E_SHAPE, "paged_store: %u tokens (fewer than 2^28)", tokens);
     if (int rc = ensure_device()) return rc;
     if (tokens == 0) return SAETTA_OK;
     const StoreArgs a = {{keys, values}, slots, {cache.keys, cache.values}, {cache.key_scales, cache.value_scales},
@@ -241,6 +242,7 @@ extern "C" int saetta_paged_gather(saetta_stream_t stream, int type, saetta_page
     SAETTA_REQUIRE(slots, SAETTA_E_NULL, "paged_gather: null slots");
     if (int rc = check_cache(cache, "paged_gather")) return rc;
     SAETTA_REQUIRE(aligned(slots, 4) && aligned(keys, 16) && aligned(values, 16), SAETTA_E_ALIGN, "paged_gather: keys and values must be 16-byte aligned");
+    SAETTA_REQUIRE(tokens < (1u << 28), SAETTA_E_SHAPE, "paged_gather: %u tokens (fewer than 2^28)", tokens);
     if (int rc = ensure_device()) return rc;
     if (tokens == 0 || (!keys && !values)) return SAETTA_OK;
     const GatherArgs a = {{cache.keys, cache.values}, {cache.key_scales, cache.value_scales}, slots, {keys, values},

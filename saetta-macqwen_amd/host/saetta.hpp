@@ -13,6 +13,7 @@
 //   attention_prefill::FlashParams, KERNELS, DEFAULT, KEY_BLOCK, encode
 //                                      src/attention_prefill.rs:4-72
 //   attention_gemm::KEYS, AttGemm      src/attention_gemm.rs:28, 95-364
+//   paged::PagedCache, PagedTables, PagedAttention   (no counterpart: the reference serves one sequence)
 //
 // Where the reference asserts or panics, these throw std::runtime_error.  Buffers are
 // reference-counted and zero-filled like Metal's (src/gpu.rs:287-290); a Plan keeps every
@@ -900,5 +901,137 @@ class RowBackup {
 };
 
 }  // namespace gpu_layers
+
+// A cache in blocks that several requests share, the tables over it and the attention that reads it (include/saetta_hip.h; the
+// reference's caches are one sequence's).
+namespace paged {
+
+constexpr size_t HEAD_DIM = SAETTA_HEAD_DIM;
+enum class Type { F32 = SAETTA_F32, F16 = SAETTA_F16, BF16 = SAETTA_BF16 };
+inline size_t type_bytes(Type t) { return t == Type::F32 ? 4 : 2; }
+
+// Rows of `heads` rows of 256 values; strides in values (0: contiguous).
+struct Rows {
+    View view;
+    uint64_t token_stride, head_stride;
+    Rows() : token_stride(0), head_stride(0) {}
+    Rows(View v, size_t heads) : view(std::move(v)), token_stride(heads * HEAD_DIM), head_stride(HEAD_DIM) {}
+    Rows(View v, uint64_t token, uint64_t head) : view(std::move(v)), token_stride(token), head_stride(head) {}
+    saetta_strided_rows c() const { return saetta_strided_rows{view.buffer.get() ? view.ptr<void>() : nullptr, token_stride, head_stride}; }
+};
+
+// The keys and values of one layer.
+struct PagedCache {
+    gpu::Buffer keys, values, key_scales, value_scales;
+    size_t kv_heads, blocks, block_tokens;
+
+    PagedCache(const gpu::Gpu &gpu, size_t kv_heads_, size_t head_dim, size_t blocks_, size_t block_tokens_ = 64)
+        : kv_heads(kv_heads_), blocks(blocks_), block_tokens(block_tokens_) {
+        if (head_dim != HEAD_DIM) throw std::runtime_error("a paged cache is written for head dim 256");
+        if (kv_heads == 0 || blocks == 0 || (block_tokens != 16 && block_tokens != 32 && block_tokens != 64 && block_tokens != 128) ||
+            blocks >= (size_t(1) << 31) / block_tokens)
+            throw std::runtime_error("PagedCache::new: blocks of 16, 32, 64 or 128 tokens, fewer than 2^31 in all");
+        const size_t rows = blocks * kv_heads;
+        keys = gpu.buffer(rows * block_tokens * HEAD_DIM), values = gpu.buffer(rows * block_tokens * HEAD_DIM);
+        key_scales = gpu.buffer(rows), value_scales = gpu.buffer(rows);
+    }
+    saetta_paged_cache c() const {
+        return saetta_paged_cache{static_cast<uint8_t *>(keys.get()), static_cast<uint8_t *>(values.get()), static_cast<uint8_t *>(key_scales.get()),
+                                  static_cast<uint8_t *>(value_scales.get()), uint32_t(blocks), uint32_t(block_tokens), uint32_t(kv_heads)};
+    }
+    // The keys and values of `tokens` tokens into their slots (i32; -1: nowhere).
+    void record(plan::Plan &plan, Type type, const Rows &k, const Rows &v, const View &slots, size_t tokens) const {
+        const PagedCache self = *this;
+        plan.op("paged_store", [=](hipStream_t s) { self.store(s, type, k, v, slots, tokens); });
+    }
+    void encode(const gpu::Gpu &gpu, Type type, const Rows &k, const Rows &v, const View &slots, size_t tokens) const {
+        store(gpu.stream(), type, k, v, slots, tokens);
+    }
+    // What the slots hold, as [tokens][kv_heads][256] of the type.
+    void encode_dequantize(const gpu::Gpu &gpu, Type type, const View &slots, const View &keys_out, const View &values_out, size_t tokens) const {
+        check(saetta_paged_gather(gpu.stream(), int(type), c(), slots.ptr<int32_t>(), keys_out.ptr<void>(), values_out.ptr<void>(), uint32_t(tokens)), "paged_gather");
+    }
+
+  private:
+    void store(hipStream_t s, Type type, const Rows &k, const Rows &v, const View &slots, size_t tokens) const {
+        check(saetta_paged_store(s, int(type), k.c(), v.c(), slots.ptr<int32_t>(), c(), uint32_t(tokens)), "paged_store");
+    }
+};
+
+// Which blocks the requests hold, and what a step's tokens are given.
+struct PagedTables {
+    size_t requests, tokens, max_blocks, blocks, block_tokens;
+    gpu::Buffer block_table, held, free_list, free_count, query_starts, kv_lens, slots, positions, unplaced;
+
+    PagedTables(const gpu::Gpu &gpu, size_t requests_, size_t tokens_, size_t max_blocks_, size_t blocks_, size_t block_tokens_ = 64)
+        : requests(requests_), tokens(tokens_), max_blocks(max_blocks_), blocks(blocks_), block_tokens(block_tokens_) {
+        if (requests == 0 || tokens == 0 || max_blocks == 0 || blocks == 0) throw std::runtime_error("PagedTables::new: sizes of one at least");
+        block_table = gpu.buffer_from(std::vector<int32_t>(requests * max_blocks, -1));
+        held = gpu.buffer(requests * 4);
+        std::vector<int32_t> all(blocks);
+        for (size_t i = 0; i < blocks; i++) all[i] = int32_t(i);
+        free_list = gpu.buffer_from(all);
+        free_count = gpu.buffer_from(std::vector<uint32_t>{uint32_t(blocks)});
+        query_starts = gpu.buffer((requests + 1) * 4), kv_lens = gpu.buffer(requests * 4);
+        slots = gpu.buffer(tokens * 4), positions = gpu.buffer(tokens * 4), unplaced = gpu.buffer(4);
+    }
+    saetta_paged_batch batch() const {
+        return saetta_paged_batch{static_cast<const uint32_t *>(query_starts.get()), static_cast<const uint32_t *>(kv_lens.get()),
+                                  static_cast<const int32_t *>(block_table.get()), uint32_t(requests), uint32_t(max_blocks), uint32_t(block_tokens)};
+    }
+    // A step of new_lens[r] tokens behind context_lens[r] (u32 both; context_lens may be kv_lens).
+    void record(plan::Plan &plan, const View &context_lens, const View &new_lens) const {
+        const PagedTables self = *this;
+        plan.op("paged_tables", [=](hipStream_t s) { self.step(s, context_lens, new_lens); });
+    }
+    void encode(const gpu::Gpu &gpu, const View &context_lens, const View &new_lens) const { step(gpu.stream(), context_lens, new_lens); }
+
+  private:
+    void step(hipStream_t s, const View &context_lens, const View &new_lens) const {
+        const saetta_paged_state state{static_cast<int32_t *>(block_table.get()), static_cast<uint32_t *>(held.get()), static_cast<int32_t *>(free_list.get()),
+                                       static_cast<uint32_t *>(free_count.get())};
+        const saetta_paged_step out{static_cast<uint32_t *>(query_starts.get()), static_cast<uint32_t *>(kv_lens.get()), static_cast<int32_t *>(slots.get()),
+                                    static_cast<int32_t *>(positions.get()), static_cast<uint32_t *>(unplaced.get())};
+        const saetta_paged_tables_params p{uint32_t(requests), uint32_t(max_blocks), uint32_t(block_tokens), uint32_t(blocks), uint32_t(tokens)};
+        check(saetta_paged_tables(s, context_lens.ptr<uint32_t>(), new_lens.ptr<uint32_t>(), state, out, p), "paged_tables");
+    }
+};
+
+// Attention of a step's new tokens, up to `rows` a request, over caches of one shape.  One call's scratch at a time.
+class PagedAttention {
+  public:
+    PagedAttention(const gpu::Gpu &gpu, size_t heads, size_t kv_heads, size_t head_dim, const PagedTables &tables, size_t rows)
+        : tables_(tables), p_{uint32_t(heads), uint32_t(kv_heads), uint32_t(tables.tokens), uint32_t(rows), 1.0f / 16.0f} {
+        if (head_dim != HEAD_DIM) throw std::runtime_error("paged attention is written for head dim 256");
+        const size_t split = saetta_paged_split_bytes(p_, uint32_t(tables.requests)), workspace = saetta_paged_workspace_bytes(p_, uint32_t(tables.requests));
+        if (split == 0 || workspace == 0) throw std::runtime_error(std::string("PagedAttention::new: ") + saetta_last_error());
+        split_ = gpu.buffer(split), workspace_ = gpu.buffer(workspace);
+    }
+    // Once a step, for all layers.
+    void record_split(plan::Plan &plan) const {
+        const PagedAttention self = *this;
+        plan.op("paged_split", [=](hipStream_t s) { self.deal(s); });
+    }
+    void encode_split(const gpu::Gpu &gpu) const { deal(gpu.stream()); }
+    // q, gate (or Rows()) and out [tokens][heads][256] of f16 or bf16.
+    void record(plan::Plan &plan, Type type, const Rows &q, const PagedCache &cache, const Rows &out, const Rows &gate = Rows()) const {
+        const PagedAttention self = *this;
+        plan.op("paged_attention", [=](hipStream_t s) { self.attend(s, type, q, cache, out, gate); });
+    }
+    void encode(const gpu::Gpu &gpu, Type type, const Rows &q, const PagedCache &cache, const Rows &out, const Rows &gate = Rows()) const {
+        attend(gpu.stream(), type, q, cache, out, gate);
+    }
+
+  private:
+    void deal(hipStream_t s) const { check(saetta_paged_split(s, tables_.batch(), p_, split_.get()), "paged_split"); }
+    void attend(hipStream_t s, Type type, const Rows &q, const PagedCache &cache, const Rows &out, const Rows &gate) const {
+        check(saetta_paged_attn(s, int(type), q.c(), cache.c(), tables_.batch(), split_.get(), gate.c(), out.c(), p_, workspace_.get(), workspace_.length()), "paged_attn");
+    }
+    PagedTables tables_;
+    saetta_paged_attn_params p_;
+    gpu::Buffer split_, workspace_;
+};
+
+}  // namespace paged
 
 }  // namespace saetta

@@ -477,3 +477,66 @@ def test_steps_of_a_program(graph):
                 assert np.array_equal(a, b)
         lengths += np.array(fresh)
     assert math.isclose(float(t.unplaced[0]), 0.0)
+
+
+def test_a_cache_of_more_than_four_gigabytes():
+    """Blocks whose codes lie past 2^32 bytes: stored, read back and attended over."""
+    blocks, block = 70000, 128  # 4.6 GB of keys, as many of values
+    cache = saetta.PagedCache(2, DIM, blocks, block)
+    gen = np.random.default_rng(51)
+    order = [blocks - 1, 3, blocks - 2, 65536, 65535, 0]
+    for new in (1, 20):
+        t = saetta.PagedTables(1, new, 8, blocks, block)
+        length = 5 * block + 40 + new
+        t.block_table[0, :6] = ints(order)
+        t.kv_lens.fill_(length), t.query_starts.copy_(ints([0, new]))
+        slots = [order[p // block] * block + p % block for p in range(length)]
+        k, v = values_of(gen, length, 2, F16), values_of(gen, length, 2, F16)
+        cache.encode(k, v, ints(slots))
+        small = saetta.PagedCache(2, DIM, 6, block)  # the same in a cache of six blocks
+        near = [(p // block) * block + p % block for p in range(length)]
+        small.encode(k, v, ints(near))
+        outs = [torch.empty(2, length, 2, DIM, device="cuda") for _ in range(2)]
+        cache.encode_dequantize(ints(slots), *outs[0]), small.encode_dequantize(ints(near), *outs[1])
+        assert torch.equal(outs[0], outs[1])
+        q = torch.randn(new, 16, DIM, dtype=F16, device="cuda")
+        got, want = torch.zeros_like(q), torch.zeros_like(q)
+        attention = saetta.PagedAttention(16, 2, DIM, t, rows=new)
+        attention.encode_split(t)
+        attention.encode(q, cache, t, got)
+        t.block_table[0, :6] = ints(range(6))
+        attention.encode(q, small, t, want)
+        assert torch.equal(got, want) and float(want.abs().max()) > 0
+
+
+def test_calls_captured_by_torch():
+    """The calls as they are, under torch's own capture, replayed over other lengths with eager work between."""
+    b = Batch(61, [150, 40, 3], [2, 1, 2], 16, 16, 2, F16)
+    b.run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        b.run()
+    for lengths in ([152, 41, 5], [100, 41, 4], [17, 2, 2], [152, 41, 5]):
+        b.tables.kv_lens.copy_(ints(lengths))
+        b.out.fill_(7.25)
+        graph.replay()
+        b.compare()
+        first = b.out.clone()
+        b.run()
+        assert torch.equal(b.out, first)
+
+
+def test_a_split_of_another_call_leads_nowhere_outside():
+    """Attention by a split that was made for other rows: what it says is followed only as far as the buffers go."""
+    b = Batch(62, [70, 40], [1, 1], 16, 16, 2, F16)
+    other = saetta.PagedAttention(16, 2, DIM, b.tables, rows=30)
+    other.encode_split(b.tables)
+    n = min(other.split.numel(), b.attention.split.numel())
+    b.attention.split[:n].copy_(other.split[:n])
+    b.attention.encode(b.q, b.cache, b.tables, b.out, gate=b.gate)
+    b.attention.split.fill_(0x5a)
+    b.attention.encode(b.q, b.cache, b.tables, b.out, gate=b.gate)
+    torch.cuda.synchronize()
+    b.run()
+    b.compare()

@@ -57,6 +57,8 @@ def test_store_and_gather_refuse():
     refused(l.saetta_paged_store(None, 1, rows(A + 2), rows(), A, cache(), 1), -4, "16-byte")
     refused(l.saetta_paged_store(None, 1, rows(), rows(head=260), A, cache(), 1), -4, "16-byte")
     refused(l.saetta_paged_store(None, 0, rows(), rows(token=513), A, cache(), 1), -4, "16-byte")
+    refused(l.saetta_paged_store(None, 0, rows(), rows(), A, cache(), 1 << 28), -2, "2^28")
+    refused(l.saetta_paged_gather(None, 0, cache(), A, A, A, 1 << 28), -2, "2^28")
     refused(l.saetta_paged_gather(None, -1, cache(), A, A, A, 1), -1, "type")
     refused(l.saetta_paged_gather(None, 0, cache(), None, A, A, 1), -3, "null")
     refused(l.saetta_paged_gather(None, 0, cache(), A, A + 4, A, 1), -4, "16-byte")
@@ -77,7 +79,9 @@ def test_tables_refuse(over, code):
 
 @pytest.mark.parametrize("over, text", [(dict(heads=15), "15 q heads"), (dict(heads=6), "3 q heads per kv head"), (dict(heads=64), "32 q heads"),
                                         (dict(kv_heads=0), "0 kv heads"), (dict(heads=0), "0 q heads"), (dict(rows=0), "rows 0"),
-                                        (dict(tokens=1 << 31), "tokens")])
+                                        (dict(tokens=1 << 31), "tokens"), (dict(scale=0.0), "scale"), (dict(scale=-0.0625), "scale"),
+                                        (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
+                                        (dict(tokens=(1 << 30), rows=100), "tokens")])
 def test_attention_refuses_shapes(over, text):
     l = ffi.lib()
     refused(l.saetta_paged_split(None, batch(), params(**over), A), -2, text)
