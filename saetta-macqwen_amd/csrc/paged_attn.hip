@@ -865,9 +865,10 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
             }
         const uint32_t in_half = 4 * (at & 31), dim = 128 * half + in_half;
         auto in_wave = [&](int i) { return 2 * i + (at >> 5); };
-        auto place_of = [&](int i, const Rows &rows_of) {  // (a row past the tile's end: its last, unused)
-            const uint32_t row = wave * 32 + min(in_wave(i), wave_rows - 1);
-            return row_at<V>(rows_of, item.row0 + (row >> a.group_shift), head0 + (row & (a.group - 1))) + dim;
+        // Rows 2 i and 2 i + 1 are a head apart, or, of one head, a token: a lane's part of the address is the same for all i
+        auto place_of = [&](int i, const Rows &rows_of) {
+            const uint32_t row = wave * 32 + 2 * i;
+            return row_at<V>(rows_of, item.row0 + (row >> a.group_shift), head0 + (row & (a.group - 1))) + (uint64_t((at >> 5) * (a.group > 1 ? rows_of.head_stride : rows_of.token_stride)) + dim);
         };
         const uint4 nan4 = *reinterpret_cast<const uint4 *>(nan_from + dim);
         const uint32_t nans[4] = {nan4.x, nan4.y, nan4.z, nan4.w};
@@ -877,29 +878,51 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
         value4 gate[16];
         if (gated) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) gate[i] = *reinterpret_cast<const value4 *>(place_of(i, a.gate));
+            for (int i = 0; i < 16; i++)
+                if (uint32_t(in_wave(i)) < wave_rows) gate[i] = *reinterpret_cast<const value4 *>(place_of(i, a.gate));
         }
         wave_sync();
+        // (what is read is asked for eight rows at a time, with no branch but the stores' between: row by row the reads' latencies were 6 us of
+        // a tile's end)
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const float *from = mine_out + in_wave(i) * OUT_STRIDE;
-            floatx4 o = *reinterpret_cast<const floatx4 *>(from + in_half);
-            const uint32_t row = wave * 32 + in_wave(i);
+        for (int i0 = 0; i0 < 16; i0 += 8) {
+            floatx4 o[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) o[i] = *reinterpret_cast<const floatx4 *>(mine_out + in_wave(i0 + i) * OUT_STRIDE + in_half);
             if (any_nan) {
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (nans[j] != ~0u && int32_t(nans[j]) < item.pos0 + int32_t(row >> a.group_shift) + 1) o[j] = __builtin_nanf("");
-            }
-            if (in_wave(i) >= wave_rows) continue;
-            if (item.parts > 1) {
-                *reinterpret_cast<floatx4 *>(a.part_o + ((size_t(item.slot) * a.cache.kv_heads + kv) * CHUNK_ROWS + row) * DIM + dim) = o;
-            } else {
-                o *= from[128];
-                value4 w;
+                for (int i = 0; i < 8; i++) {
+                    const int32_t row_sees = item.pos0 + int32_t((wave * 32 + in_wave(i0 + i)) >> a.group_shift) + 1;
 #pragma unroll
-                for (int j = 0; j < 4; j++) w[j] = Row<TYPE>::store(gated ? o[j] * sigmoid(Row<TYPE>::load(gate[i][j])) : o[j]);
-                *reinterpret_cast<value4 *>(place_of(i, a.out)) = w;
+                    for (int j = 0; j < 4; j++)
+                        if (nans[j] != ~0u && int32_t(nans[j]) < row_sees) o[i][j] = __builtin_nanf("");
+                }
             }
+            if (item.parts > 1) {
+                float *part = a.part_o + ((size_t(item.slot) * a.cache.kv_heads + kv) * CHUNK_ROWS + wave * 32) * DIM + dim;
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (uint32_t(in_wave(i0 + i)) < wave_rows) *reinterpret_cast<floatx4 *>(part + in_wave(i0 + i) * DIM) = o[i];
+                continue;
+            }
+            float inv[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) inv[i] = mine_out[in_wave(i0 + i) * OUT_STRIDE + 128];
+            value4 w[8];
+            if (gated) {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) w[i][j] = Row<TYPE>::store(o[i][j] * inv[i] * sigmoid(Row<TYPE>::load(gate[i0 + i][j])));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) w[i][j] = Row<TYPE>::store(o[i][j] * inv[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (uint32_t(in_wave(i0 + i)) < wave_rows) *reinterpret_cast<value4 *>(place_of(i0 + i, a.out)) = w[i];
         }
     }
 }
