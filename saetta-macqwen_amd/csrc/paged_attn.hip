@@ -390,7 +390,7 @@ __device__ __forceinline__ void put_row(const AttnArgs &a, uint32_t row, uint32_
 // unit a lane: no barrier in the walk, and the scales, which only the scores want, come behind the first codes.
 // One group is two workgroups to a CU; two have the registers of a SIMD to themselves; of four, two teams of four waves take two each over the
 // same keys, whose codes the second team finds in the caches.  (The kernel for chunks, where most of a tile is empty, takes 102 to 108 us for 64 drafts of 3
-// to 8 rows at 4000 tokens, this one 46 to @@; four groups to a wave are more registers than there are: 353.)
+// to 8 rows at 4000 tokens, this one 46 to 69; four groups to a wave are more registers than there are: 353.)
 constexpr int few_threads(int columns) { return 64 * FEW_WAVES * (columns == 4 ? 2 : 1); }
 constexpr uint32_t FEW_STEPS = 32;     // steps that a wave looks up at a time
 constexpr int FEW_STRIDE = DIM + 4;    // floats of a row in LDS: neighbouring rows on other banks
@@ -651,20 +651,21 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
     for (uint32_t i = tid; i < DIM; i += 64 * CHUNK_WAVES) nan_from[i] = ~0u;
     const uint32_t unit0 = item.key0 / UNIT_TOKENS, end_unit = (item.key1 + UNIT_TOKENS - 1) / UNIT_TOKENS;
     const uint32_t steps = end_unit > unit0 ? (end_unit - unit0 + 1) / 2 : 0;
-    static_assert(WINDOW == 64 * CHUNK_WAVES, "a thread a unit");
-    Unit unit = find_unit(a, item.request, kv, unit0 + tid, end_unit);
-    units[(unit0 + tid) % WINDOW] = unit;
-    __syncthreads();  // where the codes are is known; how they are scaled comes with them
+    // What a wave holds of the units of 32 steps, unit j of step i in lane 2 i + j: where the codes to be copied are, and the scales of the steps that are
+    // worked on.  (A lane's register is read at once; read from LDS each time, with nothing to do meanwhile, they were a third of a step.)  Those of
+    // the first steps every wave looks up by itself: the queries' loads go out behind that one, and the codes' copies as soon as it is back.
+    Unit unit = find_unit(a, item.request, kv, unit0 + lane, end_unit);
+    uint32_t places = 0, scales = 0;
 
     half8 q[16];
     int32_t sees;
-    auto get_queries = [&] {
+    {
         const uint32_t row = min(wave * 32 + (lane & 31), rows - 1), token = row >> a.group_shift, head = kv * a.group + (row & (a.group - 1));
         sees = item.pos0 + int32_t(token) + 1;
         const V *qp = row_at<const V>(a.q, item.row0 + token, head) + (lane >> 5) * 8;
 #pragma unroll
         for (int i = 0; i < 16; i++) q[i] = *reinterpret_cast<const half8 *>(qp + i * 16);
-    };
+    }
     const float c = a.scale * 1.4426950408889634f;
     const uint32_t all_see = uint32_t(max(item.pos0 + 1, 0));
     // what the wave's first and last rows see
@@ -690,9 +691,6 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
     };
     // the wave's kilobyte of a step: 64 dims (part) of the unit `mine`
     const uint32_t mine = wave >> 2, part = wave & 3;
-    // What the lanes hold of the units of 32 steps, unit j of step i in lane 2 i + j: where the codes to be copied are, and the scales of the steps that are
-    // worked on.  (A lane's register is read at once; read from LDS each time, with nothing to do meanwhile, they were a third of a step.)
-    uint32_t places = 0, scales = 0;
     auto hold = [&](uint32_t step) { return units[(unit0 + 2 * step + here()) % WINDOW]; };
     auto copy = [&](const uint8_t *codes, uint32_t step, uint32_t place) {
         const uint32_t row = __builtin_amdgcn_readlane(places, (2 * step + mine) % 64);
@@ -707,7 +705,7 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
     };
     auto copy_values = [&](uint32_t step) { copy(a.cache.values, step, V_CODES); };
     auto copy_keys = [&](uint32_t step) {  // (the keys are a step ahead of the values: the first to want the next 32)
-        if (step % 32 == 0) places = hold(step).block;
+        if (step % 32 == 0) places = step < steps ? hold(step).block : kv;  // (from the last step on: block 0, whose codes nobody looks at)
         copy(a.cache.keys, step, K_CODES);
     };
     auto keys_of = [&](uint32_t step) { return *reinterpret_cast<const u32x4 *>(tiles + K_CODES + (step % PLACES) * CODE_BYTES + wave * 1024 + here() * 16); };
@@ -774,13 +772,18 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
 
     if (steps) {
         // K(0), K(1), V(0), then what the steps before the first would have asked for
-        copy_keys(0), copy_keys(1), copy_values(0);
-        get_queries();
-        units[(unit0 + tid) % WINDOW].scales = find_scales(a, unit);
+        places = unit.block;
+        copy(a.cache.keys, 0, K_CODES), copy(a.cache.keys, 1, K_CODES), copy_values(0);
+        scales = find_scales(a, unit);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();  // the scales are there
-        scales = hold(0).scales;
+        lds_barrier();  // nan_from is clear
         make_keys(keys_of(0), 0), make_keys(keys_of(1), 1), make_values(values_of(0), 0);
+        if (steps > 32 - (AHEAD + 2)) {  // the units of later steps: a window, from which a wave takes those of its next 32
+            static_assert(WINDOW == 64 * CHUNK_WAVES, "a thread a unit");
+            unit = find_unit(a, item.request, kv, unit0 + tid, end_unit);
+            unit.scales = find_scales(a, unit);
+            units[(unit0 + tid) % WINDOW] = unit;
+        }
         static_assert(PLACES == AHEAD + 1, "a place is free again when the step after next asks for it");
 #pragma unroll
         for (uint32_t i = 0; i < AHEAD; i++) copy_values(1 + i), copy_keys(2 + i);
@@ -808,7 +811,7 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
                 half8 p[2];
                 const bool works = key_at(step) < wave_end;
                 if (works) softmax(s, step, p);
-                if ((step + 1) % 32 == 0) scales = hold(step + 1).scales;
+                if ((step + 1) % 32 == 0) scales = step + 1 < steps ? hold(step + 1).scales : 0;
                 make_values(v_codes, step + 1), make_keys(k_codes, step + 2);
                 if (works) stream_block_alone<BRAIN>(s, acc, q, p, k_halves(step + 1), v_halves(step));
                 lds_barrier();
@@ -833,7 +836,7 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
                 }
                 arrived();
                 const u32x4 v_codes = values_of(step + 1), k_codes = keys_of(step + 2);
-                if ((step + 1) % 32 == 0) scales = hold(step + 1).scales;
+                if ((step + 1) % 32 == 0) scales = step + 1 < steps ? hold(step + 1).scales : 0;
                 if (works && key_at(step + 1) < wave_end) softmax(s, step + 1, p);
                 make_values(v_codes, step + 1), make_keys(k_codes, step + 2);
                 lds_barrier();
@@ -843,14 +846,31 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
         settle(acc);
     }
 
-    __syncthreads();  // nan_from is whole, and what the tiles held has been read
+    const uint32_t at = here();
+    const uint32_t wave_rows = wave * 32 < rows ? min(rows - wave * 32, 32u) : 0, head0 = kv * a.group, in_half = 4 * (at & 31);
+    auto in_wave = [&](int i) { return 2 * i + (at >> 5); };
+    // Rows 2 i and 2 i + 1 are a head apart, or, of one head, a token: a lane's part of the address is the same for all i
+    auto place_of = [&](int i, const Rows &rows_of) {
+        const uint32_t row = wave * 32 + 2 * i;
+        return row_at<V>(rows_of, item.row0 + (row >> a.group_shift), head0 + (row & (a.group - 1))) + (uint64_t((at >> 5) * (a.group > 1 ? rows_of.head_stride : rows_of.token_stride)) + in_half);
+    };
+    // (the gates of a half of the dims travel while what comes before them is done)
+    const bool gated = a.gate.data && item.parts == 1;
+    typedef V value4 __attribute__((ext_vector_type(4)));
+    value4 gates[2][16];
+    auto get_gates = [&](int half) {
+        if (!gated) return;
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            if (in_wave(i) < wave_rows) gates[half][i] = *reinterpret_cast<const value4 *>(place_of(i, a.gate) + 128 * half);
+    };
+    get_gates(0);
+    lds_barrier();  // nan_from is whole, and what the tiles held has been read
     // Through LDS, a half of the dims at a time, so that a wave stores two rows' 128 dims side by side.  A row's sum is behind its dims.
     l = across_rows<32, 64>(l, SumOp());
-    const uint32_t at = here();
     float *mine_out = reinterpret_cast<float *>(tiles) + wave * (32 * OUT_STRIDE);
     mine_out[(at & 31) * OUT_STRIDE + 128] = l == 0.0f ? 0.0f : 1.0f / l;
-    if (wave * 32 >= rows) return;
-    const uint32_t wave_rows = min(rows - wave * 32, 32u), head0 = kv * a.group;
+    if (wave_rows == 0) return;
     if (item.parts > 1 && at < wave_rows)
         *reinterpret_cast<float2 *>(a.part_ml + ((size_t(item.slot) * a.cache.kv_heads + kv) * CHUNK_ROWS + wave * 32 + at) * 2) = float2{m, l};
 #pragma unroll
@@ -863,24 +883,11 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
                 const floatx16 &x = acc[4 * half + i];
                 *reinterpret_cast<floatx4 *>(mine_out + (at & 31) * OUT_STRIDE + 32 * i + 4 * (at >> 5) + 8 * k) = floatx4{x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]};
             }
-        const uint32_t in_half = 4 * (at & 31), dim = 128 * half + in_half;
-        auto in_wave = [&](int i) { return 2 * i + (at >> 5); };
-        // Rows 2 i and 2 i + 1 are a head apart, or, of one head, a token: a lane's part of the address is the same for all i
-        auto place_of = [&](int i, const Rows &rows_of) {
-            const uint32_t row = wave * 32 + 2 * i;
-            return row_at<V>(rows_of, item.row0 + (row >> a.group_shift), head0 + (row & (a.group - 1))) + (uint64_t((at >> 5) * (a.group > 1 ? rows_of.head_stride : rows_of.token_stride)) + dim);
-        };
+        if (half == 0) get_gates(1);
+        const uint32_t dim = 128 * half + in_half;
         const uint4 nan4 = *reinterpret_cast<const uint4 *>(nan_from + dim);
         const uint32_t nans[4] = {nan4.x, nan4.y, nan4.z, nan4.w};
         const bool any_nan = (nans[0] & nans[1] & nans[2] & nans[3]) != ~0u;
-        const bool gated = a.gate.data && item.parts == 1;
-        typedef V value4 __attribute__((ext_vector_type(4)));
-        value4 gate[16];
-        if (gated) {
-#pragma unroll
-            for (int i = 0; i < 16; i++)
-                if (uint32_t(in_wave(i)) < wave_rows) gate[i] = *reinterpret_cast<const value4 *>(place_of(i, a.gate));
-        }
         wave_sync();
         // (what is read is asked for eight rows at a time, with no branch but the stores' between: row by row the reads' latencies were 6 us of
         // a tile's end)
@@ -913,7 +920,7 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
 #pragma unroll
                 for (int i = 0; i < 8; i++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) w[i][j] = Row<TYPE>::store(o[i][j] * inv[i] * sigmoid(Row<TYPE>::load(gate[i0 + i][j])));
+                    for (int j = 0; j < 4; j++) w[i][j] = Row<TYPE>::store(o[i][j] * inv[i] * sigmoid(Row<TYPE>::load(gates[half][i0 + i][j])));
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; i++)
@@ -922,7 +929,7 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
             }
 #pragma unroll
             for (int i = 0; i < 8; i++)
-                if (uint32_t(in_wave(i0 + i)) < wave_rows) *reinterpret_cast<value4 *>(place_of(i0 + i, a.out)) = w[i];
+                if (uint32_t(in_wave(i0 + i)) < wave_rows) *reinterpret_cast<value4 *>(place_of(i0 + i, a.out) + 128 * half) = w[i];
         }
     }
 }
