@@ -594,8 +594,9 @@ typedef struct saetta_paged_tables_params {
  * rejected draft is a shorter context) gives the rest back behind those that are left, its entries set to -1.  Token
  * i of request r is token query_starts[r] + i of the step, at position context_lens[r] + i, in slot
  * block * block_tokens + position % block_tokens, or -1 where it has no block.  Past the last token slots and positions
- * are -1.  query_starts are at most p.tokens, and tokens past the room have no place.  *unplaced: the tokens without
- * a slot.  kv_lens may be context_lens itself: then the call, replayed, goes on by new_lens each time. */
+ * are -1.  New tokens past the room are no part of the step: lengths, blocks and query_starts count those before it.  *unplaced: the
+ * new tokens without a slot, those among them.  kv_lens may be context_lens itself: then the call, replayed, goes on by the step's
+ * tokens each time.  requests * max_blocks is less than 2^31. */
 int saetta_paged_tables(saetta_stream_t stream, const uint32_t *context_lens, const uint32_t *new_lens,
                         saetta_paged_state state, saetta_paged_step step, saetta_paged_tables_params p);
 
@@ -614,7 +615,7 @@ typedef struct saetta_strided_rows {
  * become what they stand for times 2^(their e - e), rounded to nearest even like the new ones; e falls only when the
  * block begins anew.  A value that is not finite, or larger than 448 * 2^60, is stored as NaN.  The tokens of one block follow each other
  * in the call, at rising slots without a gap, as saetta_paged_tables gives them; what a block holds that a call
- * names by two such runs is undefined.  tokens < 2^28, as for saetta_paged_gather. */
+ * names by two such runs is undefined.  What a block holds behind the last token that was stored in it counts no more.  tokens < 2^28, as for saetta_paged_gather. */
 int saetta_paged_store(saetta_stream_t stream, int type, saetta_strided_rows keys, saetta_strided_rows values,
                        const int32_t *slots, saetta_paged_cache cache, uint32_t tokens);
 
@@ -656,7 +657,7 @@ int saetta_paged_split(saetta_stream_t stream, saetta_paged_batch batch, saetta_
  * the cache already: token i of the n that request r has now sits at position kv_lens[r] - n + i and sees the positions up to its
  * own.  q, gate and out are f16 or bf16 (type) rows of p.heads heads; gate.data NULL: no gate.  out may be q.  Rows past the step's last token,
  * and tokens of a request past p.rows where p.rows is for few rows, are left as they were; a row that sees nothing (its position is
- * below 0, or its blocks are not there) becomes zeros.  split: made by saetta_paged_split with the same batch and p.
+ * below 0, or its blocks are not there) becomes zeros.  A score (times log2 e) below -1e30 counts as not seen.  split: made by saetta_paged_split with the same batch and p.
  * workspace: 16-byte aligned, of saetta_paged_workspace_bytes, the call's own until its kernels have run; calls that may
  * overlap bring different ones. */
 int saetta_paged_attn(saetta_stream_t stream, int type, saetta_strided_rows q, saetta_paged_cache cache,

@@ -174,9 +174,11 @@ __global__ __launch_bounds__(SPLIT_THREADS) void paged_split_kernel(SplitArgs a)
     Item mine;
     auto for_tiles = [&](auto f) {
         if (found) return f(mine);
+        uint32_t most = a.most_items - a.target;  // as many tiles as there can be, whatever the starts say
         for (uint32_t r0 = 0; r0 < requests; r0 += SPLIT_THREADS) {
             uint32_t all;
             const uint32_t tiles = work_of(a, r0 + tid).tiles, before = before_this<SPLIT_THREADS>(tiles, waves, all), n = min(SPLIT_THREADS, requests - r0);
+            all = min(all, most), most -= all;
             starts[tid] = before;
             __syncthreads();
             for (uint32_t k0 = 0; k0 < all; k0 += SPLIT_THREADS) {

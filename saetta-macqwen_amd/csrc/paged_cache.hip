@@ -221,7 +221,7 @@ using namespace saetta;
 extern "C" int saetta_paged_store(saetta_stream_t stream, int type, saetta_strided_rows keys, saetta_strided_rows values,
                                   const int32_t *slots, saetta_paged_cache cache, uint32_t tokens) {
     SAETTA_REQUIRE(type == SAETTA_F32 || type == SAETTA_F16 || type == SAETTA_BF16, SAETTA_E_BITS, "paged_store: type %d (f32, f16 or bf16)", type);
-    SAETTA_REQUIRE(keys.data && values.data && slots, SAETTA_E_NULL, "paged_store: null buffer");
+    SAETTA_REQUIRE(tokens == 0 || (keys.data && values.data && slots), SAETTA_E_NULL, "paged_store: null buffer");
     if (int rc = check_cache(cache, "paged_store")) return rc;
     SAETTA_REQUIRE(aligned(slots, 4) && rows_aligned(keys, type) && rows_aligned(values, type), SAETTA_E_ALIGN,
                    "paged_store: keys and values must be 16-byte aligned, with strides of multiples of 16 bytes");
@@ -239,7 +239,7 @@ extern "C" int saetta_paged_store(saetta_stream_t stream, int type, saetta_strid
 extern "C" int saetta_paged_gather(saetta_stream_t stream, int type, saetta_paged_cache cache, const int32_t *slots, void *keys,
                                    void *values, uint32_t tokens) {
     SAETTA_REQUIRE(type == SAETTA_F32 || type == SAETTA_F16 || type == SAETTA_BF16, SAETTA_E_BITS, "paged_gather: type %d (f32, f16 or bf16)", type);
-    SAETTA_REQUIRE(slots, SAETTA_E_NULL, "paged_gather: null slots");
+    SAETTA_REQUIRE(tokens == 0 || slots, SAETTA_E_NULL, "paged_gather: null slots");
     if (int rc = check_cache(cache, "paged_gather")) return rc;
     SAETTA_REQUIRE(aligned(slots, 4) && aligned(keys, 16) && aligned(values, 16), SAETTA_E_ALIGN, "paged_gather: keys and values must be 16-byte aligned");
     SAETTA_REQUIRE(tokens < (1u << 28), SAETTA_E_SHAPE, "paged_gather: %u tokens (fewer than 2^28)", tokens);

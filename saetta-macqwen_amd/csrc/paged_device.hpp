@@ -21,6 +21,7 @@ inline int check_cache(const saetta_paged_cache &c, const char *what) {
     SAETTA_REQUIRE(c.kv_heads > 0 && c.kv_heads <= 65535 / 2, SAETTA_E_SHAPE, "%s: %u kv heads", what, c.kv_heads);
     SAETTA_REQUIRE(c.blocks > 0 && uint64_t(c.blocks) * c.block_tokens < (1ull << 31), SAETTA_E_SHAPE,
                    "%s: %u blocks of %u tokens (fewer than 2^31 tokens)", what, c.blocks, c.block_tokens);
+    SAETTA_REQUIRE(uint64_t(c.blocks) * c.kv_heads < (1ull << 32), SAETTA_E_SHAPE, "%s: %u blocks of %u kv heads (fewer than 2^32 in all)", what, c.blocks, c.kv_heads);
     return SAETTA_OK;
 }
 

@@ -1,6 +1,7 @@
 // Block tables, slots and positions of a step, from the lengths of the requests.
 //
-// want[r] = min(ceil((context[r] + new[r]) / block), max_blocks).  A request that holds fewer takes what is missing out of
+// new'[r]: what of new[r] has room in the step, behind the requests before it.
+// want[r] = min(ceil((context[r] + new'[r]) / block), max_blocks).  A request that holds fewer takes what is missing out of
 // one segment at the end of the free list, request by request (an exclusive prefix sum of what they take); one that holds
 // more gives the rest back behind what is left of the list, in the same order (another prefix sum).  So what a step takes
 // and the next gives back whole leaves the list as it was.  The tokens' first rows are a third prefix sum.
@@ -56,14 +57,22 @@ __device__ __forceinline__ uint32_t sum_before(uint32_t x, uint32_t *waves, uint
 struct Lengths {
     uint32_t context, fresh, held, want;
 };
+__device__ __forceinline__ uint32_t blocks_of(const TablesArgs &a, uint32_t length) {
+    const uint32_t bt = a.p.block_tokens;
+    return min(length / bt + (length % bt != 0), a.p.max_blocks);
+}
 __device__ __forceinline__ Lengths lengths_of(const TablesArgs &a, uint32_t r) {
     Lengths l = {0, 0, 0, 0};
     if (r < a.p.requests) {
         l.context = a.context_lens[r], l.fresh = a.new_lens[r], l.held = min(a.state.held[r], a.p.max_blocks);
-        const uint32_t length = add_up(l.context, l.fresh), bt = a.p.block_tokens;
-        l.want = min(length / bt + (length % bt != 0), a.p.max_blocks);
+        l.want = blocks_of(a, add_up(l.context, l.fresh));
     }
     return l;
+}
+// ... of a request whose first new token is token `token` of the step: those past the room are no part of it.
+__device__ __forceinline__ void cut_to_room(const TablesArgs &a, uint32_t token, Lengths &l) {
+    l.fresh = min(l.fresh, a.p.tokens - min(token, a.p.tokens));
+    l.want = blocks_of(a, add_up(l.context, l.fresh));
 }
 
 // The last of `starts` (rising, starts[0] <= x) that is no more than x.
@@ -118,7 +127,20 @@ __global__ __launch_bounds__(TABLE_THREADS) void paged_tables_kernel(TablesArgs 
         total = add_up(total, l.fresh);
     }
     uint32_t all_takes, all_gives, all_tokens;
-    sum_before(takes, waves, all_takes), sum_before(gives, waves, all_gives), sum_before(total, waves, all_tokens);
+    sum_before(total, waves, all_tokens);
+    if (all_tokens > room) {  // (where each begins is then wanted first)
+        takes = gives = 0;
+        uint32_t tokens_before = 0, here;
+        for (uint32_t r0 = 0; r0 < requests; r0 += TABLE_THREADS) {
+            Lengths l = lengths_of(a, r0 + tid);
+            const uint32_t token = add_up(tokens_before, sum_before(l.fresh, waves, here));
+            tokens_before = add_up(tokens_before, here);
+            if (r0 + tid < requests) cut_to_room(a, token, l);
+            takes = add_up(takes, l.want > l.held ? l.want - l.held : 0);
+            gives = add_up(gives, l.held > l.want ? l.held - l.want : 0);
+        }
+    }
+    sum_before(takes, waves, all_takes), sum_before(gives, waves, all_gives);
     const uint32_t taken = min(all_takes, free_count), left = free_count - taken;
     total = min(all_tokens, room);
 
@@ -126,11 +148,12 @@ __global__ __launch_bounds__(TABLE_THREADS) void paged_tables_kernel(TablesArgs 
     uint32_t takes_before = 0, tokens_before = 0, placed = 0;
     for (uint32_t r0 = 0; r0 < requests; r0 += TABLE_THREADS) {
         const uint32_t r = r0 + tid;
-        const Lengths l = lengths_of(a, r);
-        const uint32_t take = l.want > l.held ? l.want - l.held : 0;
+        Lengths l = lengths_of(a, r);
         uint32_t here;
         const uint32_t token = add_up(tokens_before, sum_before(l.fresh, waves, here));
         tokens_before = add_up(tokens_before, here);
+        if (r < requests) cut_to_room(a, token, l);
+        const uint32_t take = l.want > l.held ? l.want - l.held : 0;
         const uint32_t before = add_up(takes_before, sum_before(take, waves, here));
         takes_before = add_up(takes_before, here);
         if (r < requests) {
@@ -138,9 +161,9 @@ __global__ __launch_bounds__(TABLE_THREADS) void paged_tables_kernel(TablesArgs 
             a.step.kv_lens[r] = add_up(l.context, l.fresh);
             const uint32_t held = l.held + min(take, taken - min(before, taken));
             if (take > 0) a.state.held[r] = held;
-            // tokens that its blocks have places for, and the step room
+            // tokens that its blocks have places for
             const uint32_t places = min(held, l.want) * a.p.block_tokens;
-            if (token < room && l.context < places) placed += min(min(l.fresh, room - token), places - l.context);
+            if (l.context < places) placed += min(l.fresh, places - l.context);
             if constexpr (SLOTS) tokens_from[tid] = min(token, room), contexts[tid] = l.context, holds[tid] = min(held, l.want);
         }
         if (here == 0) continue;  // (for all threads alike)
@@ -178,8 +201,7 @@ __global__ __launch_bounds__(TABLE_THREADS) void paged_tables_kernel(TablesArgs 
             Lengths l = {0, 0, 0, 0};
             if (r < requests) {
                 l.held = min(a.state.held[r], a.p.max_blocks);
-                const uint32_t length = a.step.kv_lens[r], bt = a.p.block_tokens;
-                l.want = min(length / bt + (length % bt != 0), a.p.max_blocks);
+                l.want = blocks_of(a, a.step.kv_lens[r]);
             }
             const uint32_t give = l.held > l.want ? l.held - l.want : 0;
             uint32_t here;
@@ -241,7 +263,7 @@ __global__ __launch_bounds__(SLOT_TOKENS) void paged_slots_kernel(TablesArgs a) 
     if (t < total) {
         const uint32_t r = first + (n <= HELD ? last_at_most(starts, n, t) : last_at_most(query_starts + first, n, t));
         // (the context from the sum and not from context_lens, which kv_lens may be: those have grown by now)
-        const uint32_t context = a.step.kv_lens[r] - a.new_lens[r];
+        const uint32_t context = a.step.kv_lens[r] - (query_starts[r + 1] - query_starts[r]);
         place_token(a, t, r, add_up(context, t - query_starts[r]), min(a.state.held[r], a.p.max_blocks));
     } else if (t < a.p.tokens) {
         place_nothing(a, t);
@@ -270,6 +292,7 @@ extern "C" int saetta_paged_tables(saetta_stream_t stream, const uint32_t *conte
     SAETTA_REQUIRE(p.blocks > 0 && uint64_t(p.blocks) * p.block_tokens < (1ull << 31), SAETTA_E_SHAPE,
                    "paged_tables: %u blocks of %u tokens (fewer than 2^31 tokens)", p.blocks, p.block_tokens);
     SAETTA_REQUIRE(p.max_blocks > 0 && uint64_t(p.max_blocks) * p.block_tokens < (1ull << 31), SAETTA_E_SHAPE, "paged_tables: rows of %u blocks", p.max_blocks);
+    SAETTA_REQUIRE(uint64_t(p.requests) * p.max_blocks < (1ull << 31), SAETTA_E_SHAPE, "paged_tables: a table of %u rows of %u blocks (fewer than 2^31 entries)", p.requests, p.max_blocks);
     SAETTA_REQUIRE(p.requests < (1u << 24) && p.tokens < (1u << 31), SAETTA_E_SHAPE, "paged_tables: %u requests, room for %u tokens", p.requests, p.tokens);
     if (int rc = ensure_device()) return rc;
     const TablesArgs a = {context_lens, new_lens, state, step, p};
@@ -280,7 +303,7 @@ extern "C" int saetta_paged_tables(saetta_stream_t stream, const uint32_t *conte
         launch(paged_tables_kernel<true, 1024>, dim3(1), dim3(1024), 0, as_stream(stream), a);
     } else {
         launch(paged_tables_kernel<false, 1024>, dim3(1), dim3(1024), 0, as_stream(stream), a);
-        launch(paged_slots_kernel, dim3((p.tokens + SLOT_TOKENS - 1) / SLOT_TOKENS), dim3(SLOT_TOKENS), 0, as_stream(stream), a);
+        if (p.tokens > 0) launch(paged_slots_kernel, dim3((p.tokens + SLOT_TOKENS - 1) / SLOT_TOKENS), dim3(SLOT_TOKENS), 0, as_stream(stream), a);
     }
     return launch_status("paged_tables");
 }

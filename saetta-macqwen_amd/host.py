@@ -626,6 +626,11 @@ _TYPES = {torch.float32: ffi.F32, torch.float16: ffi.F16, torch.bfloat16: ffi.BF
 _HALVES = (torch.float16, torch.bfloat16)
 
 
+def _one_device(what, *tensors):
+    if len({t.device for t in tensors if t is not None}) > 1:
+        raise ValueError(f"{what}: tensors of one device, got " + ", ".join(sorted({str(t.device) for t in tensors if t is not None})))
+
+
 def _rows_of(t, heads, dtypes, what):
     """[tokens, heads, 256] with any strides that the library takes, as StridedRowsC."""
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes):
@@ -667,6 +672,7 @@ class PagedCache:
         _need(slots, torch.int32, "PagedCache slots")
         if k.dtype is not v.dtype or k.shape[0] != v.shape[0] or slots.numel() != k.shape[0]:
             raise ValueError("PagedCache: k, v and slots must be of as many tokens, k and v of one type")
+        _one_device("PagedCache", k, v, slots, *self.tensors())
         plan.op("paged_store", _Call("saetta_paged_store", "paged_store", (
             _TYPES[k.dtype], *rows, _ptr(slots), self.c(), slots.numel()), (k, v, slots, *self.tensors())))
 
@@ -683,6 +689,7 @@ class PagedCache:
             _need(t, outs[0].dtype, "PagedCache keys and values")
             if t.numel() < slots.numel() * self.kv_heads * DIM:
                 raise ValueError("PagedCache: keys and values do not hold the slots' rows")
+        _one_device("PagedCache", slots, keys, values, *self.tensors())
         plan.op("paged_gather", _Call("saetta_paged_gather", "paged_gather", (
             _TYPES[outs[0].dtype], self.c(), _ptr(slots), *[None if t is None else _ptr(t) for t in (keys, values)], slots.numel()),
             (slots, keys, values, *self.tensors())))
@@ -694,7 +701,7 @@ class PagedCache:
 class PagedTables:
     """Which blocks the requests hold, and what a step's tokens are given: all on the GPU, from the requests' lengths.
     `requests` rows, room for `tokens` new tokens a step, up to `max_blocks` blocks a request of a cache of `blocks`.
-    (The tensors are a program's own to fill, too, where it keeps tables on the host.)"""
+    (The tensors are a program's own to fill in place, too, where it keeps tables on the host.)"""
 
     def __init__(self, requests, tokens, max_blocks, blocks, block_tokens=64, device="cuda"):
         if requests < 1 or tokens < 1 or max_blocks < 1 or blocks < 1:
@@ -729,6 +736,7 @@ class PagedTables:
             _need(t, torch.int32, f"PagedTables {what}")
             if t.numel() != self.requests:
                 raise ValueError(f"PagedTables: {what} must be of {self.requests} requests")
+        _one_device("PagedTables", context_lens, new_lens, *self.tensors())
         at = [_ptr(t) for t in self.tensors()]
         plan.op("paged_tables", _Call("saetta_paged_tables", "paged_tables", (
             _ptr(context_lens), _ptr(new_lens), ffi.PagedStateC(*at[:4]), ffi.PagedStepC(*at[4:]), ffi.PagedTablesParamsC(*self._sizes)),
@@ -771,6 +779,7 @@ class PagedAttention:
     def record_split(self, plan, tables):
         """Deals a step's rows and keys out, once for all layers: behind the tables, before the first layer's attention."""
         self._check(tables)
+        _one_device("paged attention", self.split, *tables.tensors())
         plan.op("paged_split", _Call("saetta_paged_split", "paged_split", (
             tables.batch(), ffi.PagedAttnParamsC(*self._params), _ptr(self.split)),
             (self.split, tables.query_starts, tables.kv_lens, tables.block_table)))
@@ -790,6 +799,7 @@ class PagedAttention:
                 raise ValueError(f"paged attention: q, gate and out must be of one type and of {tables.tokens} tokens")
         if (out.shape[0] > 1 and out.stride(0) == 0) or (self.heads > 1 and out.stride(1) == 0):
             raise ValueError("paged attention: out's rows must lie apart")
+        _one_device("paged attention", q, gate, out, self.workspace, *cache.tensors(), *tables.tensors())
         plan.op("paged_attention", _Call("saetta_paged_attn", "paged_attn", (
             _TYPES[q.dtype], rows[0], cache.c(), tables.batch(), _ptr(self.split), gate_rows, rows[1], ffi.PagedAttnParamsC(*self._params),
             _ptr(self.workspace), self.workspace.numel()),

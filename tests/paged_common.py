@@ -123,7 +123,14 @@ def attend(q, cache, table, query_starts, kv_lens, gate, out, scale=1.0 / 16.0):
 
 
 def tables(state, context, new, block_tokens, tokens):
-    """A step: state is a dict of block_table, held, free (the list's used part).  What the step is given."""
+    """A step: state is a dict of block_table, held, free (the list's used part).  What the step is given.  New tokens past the room
+    (`tokens`) are no part of it."""
+    asked, before = sum(int(n) for n in new), 0
+    cut = []
+    for n in new:
+        cut.append(min(int(n), max(tokens - before, 0)))
+        before += int(n)
+    new = cut
     width = state["block_table"].shape[1]
     free, slots, positions, starts, kv_lens = state["free"], [], [], [0], []
     want = [min(-(-(int(c) + int(n)) // block_tokens), width) for c, n in zip(context, new)]
@@ -142,16 +149,13 @@ def tables(state, context, new, block_tokens, tokens):
             state["block_table"][r, w:state["held"][r]] = -1
             state["held"][r] = w
     state["free"] = free
-    unplaced = 0
+    unplaced = asked - sum(new)
     for r, (c, n) in enumerate(zip(context, new)):
         for p in range(int(c), int(c) + int(n)):
             has = p // block_tokens < state["held"][r]
             slot = int(state["block_table"][r, p // block_tokens]) * block_tokens + p % block_tokens if has else -1
-            if len(slots) >= tokens:
-                slot = -1
-            else:
-                slots.append(slot), positions.append(p)
+            slots.append(slot), positions.append(p)
             unplaced += slot < 0
-        starts.append(min(starts[-1] + int(n), tokens)), kv_lens.append(int(c) + int(n))
+        starts.append(starts[-1] + int(n)), kv_lens.append(int(c) + int(n))
     behind = [-1] * (tokens - len(slots))
     return {"slots": slots + behind, "positions": positions + behind, "query_starts": starts, "kv_lens": kv_lens, "unplaced": [unplaced]}

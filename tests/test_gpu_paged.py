@@ -83,6 +83,24 @@ def test_tables_of_wrong_numbers():
     assert (host(t.slots) == -1).all() and 0 <= int(t.free_count) <= 6
 
 
+def test_tables_without_new_tokens():
+    """Requests that only finish: a step with no room for tokens gives their blocks back."""
+    import ctypes
+    ffi = saetta.ffi
+    requests, blocks = 1100, 2500
+    t = saetta.PagedTables(requests, 2200, 3, blocks, 16)
+    t.encode(ints([0] * requests), ints([20] * requests))
+    state = plain_state(t)
+    zeros = ints([0] * requests)
+    at = [x.data_ptr() for x in t.tensors()]
+    p = ffi.PagedTablesParamsC(requests, 3, 16, blocks, 0)
+    ffi.check(ffi.lib().saetta_paged_tables(ctypes.c_void_p(torch.cuda.current_stream().cuda_stream), zeros.data_ptr(), zeros.data_ptr(),
+                                            ffi.PagedStateC(*at[:4]), ffi.PagedStepC(*at[4:]), p), "paged_tables")
+    want = tables(state, [0] * requests, [0] * requests, 16, 0)
+    assert host(t.free_list).tolist() == state["free"] and host(t.held).tolist() == [0] * requests and (host(t.block_table) == -1).all()
+    assert host(t.query_starts).tolist() == want["query_starts"] and int(t.unplaced) == 0
+
+
 # ---- store and gather --------------------------------------------------------------------------------------------------
 
 def values_of(gen, tokens, kv_heads, dtype):
@@ -213,6 +231,12 @@ def test_slots_that_do_not_exist():
     assert all(bool((o == 7.5).all()) for o in outs)
     cache.encode_dequantize(ints([0] * 5), outs[0], None)  # keys alone, one slot again and again
     assert bool((outs[0] == 0).all()) and bool((outs[1] == 7.5).all())
+
+
+def test_a_call_without_tokens():
+    cache, none = saetta.PagedCache(2, DIM, 3, 32), torch.zeros(0, 2, DIM, device="cuda")
+    cache.encode(none, none, ints([]))
+    cache.encode_dequantize(ints([]), none, none)
 
 
 # ---- attention -----------------------------------------------------------------------------------------------------------
@@ -477,6 +501,48 @@ def test_steps_of_a_program(graph):
                 assert np.array_equal(a, b)
         lengths += np.array(fresh)
     assert math.isclose(float(t.unplaced[0]), 0.0)
+
+
+@pytest.mark.parametrize("room, fresh", [(20, (12, 12, 3)), (4, (1, 2, 9)), (3, (1, 1, 1, 1, 1))])
+def test_a_step_past_its_room(room, fresh):
+    """More new tokens than the step has room for: those that have room are at their own positions, and the next step goes on behind them."""
+    heads, kv_heads, block, requests = 16, 2, 16, len(fresh)
+    gen = np.random.default_rng(33)
+    t = saetta.PagedTables(requests, room, 4, 20, block)
+    cache, plain = saetta.PagedCache(kv_heads, DIM, 20, block), Cache(kv_heads, 20, block)
+    poison(cache, gen)
+    attention = saetta.PagedAttention(heads, kv_heads, DIM, t, rows=max(fresh))
+    left = list(fresh)
+    for _ in range(2):
+        state, context = plain_state(t), host(t.kv_lens).tolist()
+        step = tables(state, context, left, block, room)
+        t.encode(t.kv_lens, ints(left))
+        compare_tables(t, state, step, room)
+        x = torch.tensor(gen.standard_normal((room, heads + 2 * kv_heads, DIM)), dtype=F16, device="cuda")
+        out = torch.full((room, heads, DIM), 7.25, dtype=F16, device="cuda")
+        cache.encode(x[:, heads:heads + kv_heads], x[:, heads + kv_heads:], t.slots)
+        attention.encode_split(t)
+        attention.encode(x[:, :heads], cache, t, out)
+        plain.store(numbers(x[:, heads:heads + kv_heads]), numbers(x[:, heads + kv_heads:]), step["slots"])
+        want, bound = attend(numbers(x[:, :heads]), plain, state["block_table"], step["query_starts"], step["kv_lens"], None,
+                             np.full((room, heads, DIM), 7.25))
+        assert (np.abs(numbers(out) - want) <= bound * 1.001 + 2.0 ** -11 * np.abs(want) + 2.0 ** -25).all()
+        left = [n - (after - before) for n, after, before in zip(left, step["kv_lens"], context)]
+    assert sum(fresh) - sum(left) == min(sum(fresh), 2 * room)
+
+
+def test_starts_that_go_back():
+    """First tokens that do not rise name more tiles than a step can have: as many as it can are dealt out, no row is outside."""
+    requests, room = 2000, 600
+    t = saetta.PagedTables(requests, room, 2, 4, 16)
+    cache, attention = saetta.PagedCache(2, DIM, 4, 16), saetta.PagedAttention(16, 2, DIM, t, rows=40)
+    t.query_starts.copy_(ints([0, 0xfffff] * (requests // 2) + [0])), t.kv_lens.fill_(700)
+    q = torch.zeros(room, 16, DIM, dtype=F16, device="cuda")
+    whole = torch.full((room + 8, 16, DIM), 7.25, dtype=F16, device="cuda")
+    attention.encode_split(t)
+    attention.encode(q, cache, t, whole[:room])
+    torch.cuda.synchronize()
+    assert int(attention.split[:4].view(torch.int32)) <= attention.split.numel() // 32 and bool((whole[room:] == 7.25).all())
 
 
 def test_a_cache_of_more_than_four_gigabytes():

@@ -89,6 +89,12 @@ def test_attention_refuses_shapes(over, text):
     assert l.saetta_paged_split_bytes(params(**over), 3) == 0 and l.saetta_paged_workspace_bytes(params(**over), 3) == 0
 
 
+def test_sizes_that_no_memory_holds():
+    p = ffi.PagedTablesParamsC(1 << 23, 1 << 9, 16, 8, 10)
+    refused(ffi.lib().saetta_paged_tables(None, A, A, ffi.PagedStateC(A, A, A, A), ffi.PagedStepC(A, A, A, A, A), p), -2, "2^31 entries")
+    refused(ffi.lib().saetta_paged_store(None, 0, rows(), rows(), A, cache(blocks=1 << 22, block_tokens=16, kv_heads=4096), 1), -2, "2^32")
+
+
 def test_attention_refuses_buffers():
     l, p = ffi.lib(), params()
     need = l.saetta_paged_workspace_bytes(p, 3)
@@ -127,6 +133,15 @@ def test_python_objects_refuse():
     t = saetta.PagedTables(2, 4, 4, 8, device="cpu")
     with pytest.raises(TypeError):
         t.encode(torch.zeros(2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32))
+
+
+def test_recorded_calls_refuse_tensors_of_two_devices():
+    import sys
+    one_device = sys.modules[saetta.PagedCache.__module__]._one_device
+    a, b = torch.zeros(2), torch.zeros(2, device="meta")
+    one_device("x", a, None, a), one_device("x", b, b)
+    with pytest.raises(ValueError, match="one device"):
+        one_device("x", a, None, b)
 
 
 def test_parameter_blocks_have_the_header_sizes():
