@@ -142,16 +142,6 @@ __device__ __forceinline__ uint32_t before_this(uint32_t x, uint32_t *waves, uin
     __syncthreads();
     return before + through - x;
 }
-// The last of `starts` (rising, starts[0] <= x) that is no more than x.
-__device__ __forceinline__ uint32_t last_at_most(const uint32_t *starts, uint32_t n, uint32_t x) {
-    uint32_t low = 0;
-    while (n > 1) {
-        const uint32_t half = n / 2;
-        if (starts[low + half] <= x) low += half, n -= half;
-        else n = half;
-    }
-    return low;
-}
 
 // Deals the work out so that the workgroups that run at once end together.  What a key of a tile costs is one of two numbers: a chunk's tile of
 // at most half the rows keeps half the waves and takes 5 / 8 of the time.  A tile that costs more than total / target is cut into parts of that

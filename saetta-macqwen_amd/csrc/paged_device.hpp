@@ -25,6 +25,25 @@ inline int check_cache(const saetta_paged_cache &c, const char *what) {
     return SAETTA_OK;
 }
 
+// The last of `starts` (rising, starts[0] <= x) that is no more than x, for N numbers at once: as many looks for each, none waiting for another's.
+template <int N>
+__device__ __forceinline__ void last_at_most(const uint32_t *starts, uint32_t n, const uint32_t (&x)[N], uint32_t (&low)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) low[i] = 0;
+    while (n > 1) {
+        const uint32_t half = n / 2;
+        n -= half;  // (of an odd n the lower part keeps a place that has been looked at)
+#pragma unroll
+        for (int i = 0; i < N; i++) low[i] += starts[low[i] + half] <= x[i] ? half : 0;
+    }
+}
+__device__ __forceinline__ uint32_t last_at_most(const uint32_t *starts, uint32_t n, uint32_t x) {
+    const uint32_t one[1] = {x};
+    uint32_t low[1];
+    last_at_most(starts, n, one, low);
+    return low[0];
+}
+
 typedef float floatx2 __attribute__((ext_vector_type(2)));
 
 // 2^e as it is, for e in -126..127

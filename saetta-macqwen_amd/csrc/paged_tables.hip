@@ -75,16 +75,6 @@ __device__ __forceinline__ void cut_to_room(const TablesArgs &a, uint32_t token,
     l.want = blocks_of(a, add_up(l.context, l.fresh));
 }
 
-// The last of `starts` (rising, starts[0] <= x) that is no more than x.
-__device__ __forceinline__ uint32_t last_at_most(const uint32_t *starts, uint32_t n, uint32_t x) {
-    uint32_t low = 0;
-    while (n > 1) {
-        const uint32_t half = n / 2;
-        if (starts[low + half] <= x) low += half, n -= half;
-        else n = half;
-    }
-    return low;
-}
 // The same by a wave at once, 64 places a look, over memory.
 __device__ __forceinline__ uint32_t wave_last_at_most(const uint32_t *starts, uint32_t n, uint32_t x) {
     uint32_t low = 0;
@@ -171,16 +161,14 @@ __global__ __launch_bounds__(TABLE_THREADS) void paged_tables_kernel(TablesArgs 
         __syncthreads();
         const uint32_t first = starts[0], end = min(takes_before, taken), n = min(TABLE_THREADS, requests - r0);
         for (uint32_t k0 = first + tid; k0 < end; k0 += AT_ONCE * TABLE_THREADS) {
+            uint32_t k[AT_ONCE], of[AT_ONCE];
             int32_t block[AT_ONCE];
 #pragma unroll
-            for (uint32_t j = 0; j < AT_ONCE; j++) block[j] = a.state.free_list[left + min(k0 + j * TABLE_THREADS, end - 1)];
+            for (uint32_t j = 0; j < AT_ONCE; j++) k[j] = min(k0 + j * TABLE_THREADS, end - 1), block[j] = a.state.free_list[left + k[j]];
+            last_at_most(starts, n, k, of);
 #pragma unroll
-            for (uint32_t j = 0; j < AT_ONCE; j++) {
-                const uint32_t k = k0 + j * TABLE_THREADS;
-                if (k >= end) break;
-                const uint32_t i = last_at_most(starts, n, k);
-                a.state.block_table[size_t(r0 + i) * a.p.max_blocks + firsts[i] + (k - starts[i])] = block[j];
-            }
+            for (uint32_t j = 0; j < AT_ONCE; j++)
+                if (k0 + j * TABLE_THREADS < end) a.state.block_table[size_t(r0 + of[j]) * a.p.max_blocks + firsts[of[j]] + (k[j] - starts[of[j]])] = block[j];
         }
         __syncthreads();
     }
@@ -212,19 +200,21 @@ __global__ __launch_bounds__(TABLE_THREADS) void paged_tables_kernel(TablesArgs 
             __syncthreads();
             const uint32_t first = starts[0], n = min(TABLE_THREADS, requests - r0);
             for (uint32_t k0 = first + tid; k0 < gives_before; k0 += AT_ONCE * TABLE_THREADS) {
+                uint32_t k[AT_ONCE], of[AT_ONCE];
                 int32_t *entry[AT_ONCE], block[AT_ONCE];
 #pragma unroll
+                for (uint32_t j = 0; j < AT_ONCE; j++) k[j] = min(k0 + j * TABLE_THREADS, gives_before - 1);
+                last_at_most(starts, n, k, of);
+#pragma unroll
                 for (uint32_t j = 0; j < AT_ONCE; j++) {
-                    const uint32_t k = min(k0 + j * TABLE_THREADS, gives_before - 1), i = last_at_most(starts, n, k);
-                    entry[j] = a.state.block_table + size_t(r0 + i) * a.p.max_blocks + firsts[i] + (k - starts[i]);
+                    entry[j] = a.state.block_table + size_t(r0 + of[j]) * a.p.max_blocks + firsts[of[j]] + (k[j] - starts[of[j]]);
                     block[j] = *entry[j];
                 }
 #pragma unroll
                 for (uint32_t j = 0; j < AT_ONCE; j++) {
-                    const uint32_t k = k0 + j * TABLE_THREADS;
-                    if (k >= gives_before) break;
+                    if (k0 + j * TABLE_THREADS >= gives_before) break;
                     // (more than the list has room for: a table that names blocks twice; they are lost, not written past its end)
-                    if (left + k < a.p.blocks) a.state.free_list[left + k] = block[j];
+                    if (left + k[j] < a.p.blocks) a.state.free_list[left + k[j]] = block[j];
                     *entry[j] = -1;
                 }
             }
