@@ -9,7 +9,9 @@
 // Store: memory-bound.  A workgroup takes one run of tokens inside one block (the first of the run's tokens finds that it is the
 // first from the slots alone), one kv head, keys or values: what shares an e is then one workgroup's, and its largest
 // magnitude is known before the first code is written, with the values held in registers.  A wave has four tokens of a unit, a lane four dims of
-// each: a load is a token's row, and what a wave stores of four tokens fills lines of 64 bytes.
+// each: a load is a token's row, and what a wave stores of four tokens fills lines of 64 bytes.  9700 tokens of five prompts, f32, 2 kv heads: 12.5 us,
+// 4.0 TB/s of what is read and written (a large copy: 4.8); a lane a token's 16 bytes, whose stores fill no lines, 22.9 us.  64 single tokens: 4.9 us, the
+// chain slot - rows - maximum - codes.
 #include "common.hpp"
 #include "lanes.hpp"
 #include "paged_device.hpp"
@@ -156,7 +158,8 @@ struct GatherArgs {
 
 // A workgroup takes 16 slots of one kv head, keys or values: a wave a slot at a time, a lane four dims, so that a store is a whole row.
 // Where the slots lie in two units at most (16 that follow each other do), the units come through LDS by whole kilobytes, for values are stored
-// four tokens to a dword; else a lane reads its bytes where they are.
+// four tokens to a dword; else a lane reads its bytes where they are.  32768 tokens, f16, 2 kv heads: 21.5 us, 4.7 TB/s of what is read and written (a
+// lane's bytes straight from memory: 42 us).
 constexpr uint32_t GATHER_SLOTS = 16;
 template <int TYPE>
 __global__ __launch_bounds__(256) void paged_gather_kernel(GatherArgs a) {
