@@ -85,7 +85,7 @@ struct SplitArgs {
     SplitHead *head;
     Item *items, *tiles;
     uint32_t tile_tokens, target, most_items, most_joined, slots, tokens, rows;
-    uint32_t few, granule, least, extra, half_tokens;
+    uint32_t few, granule, least, extra, half_tokens;  // (granule: a power of two)
 };
 
 // What an item of a chunk costs besides its keys, in keys (15 us of a workgroup, and its sums' way through memory): seven prompts of 90 to 1900
@@ -184,7 +184,8 @@ __global__ __launch_bounds__(SPLIT_THREADS) void paged_split_kernel(SplitArgs a)
             __syncthreads();  // `starts` may be written again
         }
     };
-    auto price = [&](const Item &tile) { return tile.tokens <= a.half_tokens ? 5u : 8u; };
+    constexpr uint32_t HALF = 5, WHOLE = 8;  // prices of a key
+    auto price = [&](const Item &tile) { return tile.tokens <= a.half_tokens ? HALF : WHOLE; };
 
     // a number of every thread, added up into `into`, which is 0
     auto add_up = [&](unsigned long long x, unsigned long long *into) {
@@ -198,16 +199,19 @@ __global__ __launch_bounds__(SPLIT_THREADS) void paged_split_kernel(SplitArgs a)
     add_up(sum, &total);
     // what a part costs at most, and its keys
     unsigned long long fair = max(total / a.target + 1, static_cast<unsigned long long>(a.least) * 8);
-    auto length_of = [&](const Item &tile) {
-        const unsigned long long keys = fair / price(tile) + a.granule;
-        return uint32_t(keys > 0x7fffffffu ? 0x7fffffffu : keys) / a.granule * a.granule;
+    auto length_at = [&](unsigned long long keys) {
+        keys += a.granule;
+        return uint32_t(keys > 0x7fffffffu ? 0x7fffffffu : keys) & ~(a.granule - 1);
     };
+    uint32_t half_length = length_at(fair / HALF), whole_length = length_at(fair / WHOLE);
+    auto length_of = [&](const Item &tile) { return tile.tokens <= a.half_tokens ? half_length : whole_length; };
     if (a.extra) {
         // An item costs `extra` keys besides its own (its start and end, its sums through memory): a share of as many items as there now are
         unsigned long long items = 0;
         for_tiles([&](const Item &tile) { items += tile.tokens ? max((tile.key1 + length_of(tile) - 1) / length_of(tile), 1u) : 0; });
         add_up(items, &items_there);
         if (items_there > a.target) fair += (items_there - a.target) * 8 * a.extra / a.target;
+        half_length = length_at(fair / HALF), whole_length = length_at(fair / WHOLE);
     }
     const float per_class = float(SIZES) / float(fair + 8ull * a.granule);
     auto class_of = [&](uint32_t keys, uint32_t price) { return SIZES - 1 - min(uint32_t(float(keys) * float(price) * per_class), SIZES - 1); };
