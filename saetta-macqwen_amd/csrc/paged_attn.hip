@@ -147,7 +147,8 @@ __device__ __forceinline__ uint32_t before_this(uint32_t x, uint32_t *waves, uin
 // at most half the rows keeps half the waves and takes 5 / 8 of the time.  A tile that costs more than total / target is cut into parts of that
 // and a rest; the items go out from the dearest class to the cheapest, so that who ends early takes what is small.  (One workgroup: a sum over the
 // tiles, a count of the classes, and the items themselves; the tiles by turns over its threads.  The places of the items in a class and of the
-// parts' sums follow from atomic counts, in any order: what is computed does not depend on them.)
+// parts' sums follow from atomic counts, in any order: what is computed does not depend on them.)  Latency: 5 us for one request, 7 for 48, 8.4 for a
+// chunk beside 30 drafts, once a step.
 template <uint32_t SPLIT_THREADS>
 __global__ __launch_bounds__(SPLIT_THREADS) void paged_split_kernel(SplitArgs a) {
     __shared__ uint32_t waves[SPLIT_THREADS / 64], starts[SPLIT_THREADS], ends[SPLIT_THREADS], classes[SIZES], slots_there, tiles_there;
@@ -387,8 +388,8 @@ __device__ __forceinline__ void put_row(const AttnArgs &a, uint32_t row, uint32_
 // One group is two workgroups to a CU; two have the registers of a SIMD to themselves; of four, two teams of four waves take two each over the
 // same keys, whose codes the second team finds in the caches.  (The kernel for chunks, where most of a tile is empty, takes 102 to 108 us for 64 drafts of 3
 // to 8 rows at 4000 tokens, this one 46 to 69; four groups to a wave are more registers than there are: 353.)
-// Measured, 2 kv heads, 8 q heads each, f16: a token of 8 requests at 131072 tokens 184 us, 5.9 TB/s of codes (a large copy: 4.8 TB/s read and
-// written); bf16, 48 ragged requests of some thousand tokens 62 us, 5.2 TB/s; one of 517 tokens 6.2 us, the launch and three loads that wait for each other.
+// Measured, 8 q heads over each of 2 kv heads: a token of 8 requests at 131072 tokens, f16, 184 us, 5.9 TB/s of codes (a large copy reaches 4.8, read and
+// written); of 48 requests at 330 to 30 thousand tokens, bf16, 62 us, 5.2 TB/s; of one at 517 tokens 6.3 us, the launch and three loads that wait for each other.
 constexpr int few_threads(int columns) { return 64 * FEW_WAVES * (columns == 4 ? 2 : 1); }
 constexpr uint32_t FEW_STEPS = 32;     // steps that a wave looks up at a time
 constexpr int FEW_STRIDE = DIM + 4;    // floats of a row in LDS: neighbouring rows on other banks
@@ -627,9 +628,9 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 //   waves 0..3:  softmax(s)                | O(s) + S(s+1)
 //   waves 4..7:  O(s) + S(s+1)             | softmax(s+1)
 // Step s reads V(s) and K(s+1) as halves and makes V(s+1) and K(s+2), in the places of V(s-1) and K(s): one barrier a step.
-// Bound by the matrix cores and the clock that they leave: 4096 tokens at 28672, bf16, 16 q heads over 2 kv heads, 1.85 ms, 1.11 PFLOP/s (a large
-// product of the library: 1.23); the streams of products alone 1.45 ms.  Without the two waves' opposite order 2.28.  A short item is bound by its start
-// and end, 13 to 16 us: seven prompts of 90 to 1900 tokens 75 us, a tile of 32 tokens 20.
+// Bound by the matrix cores and the clock that they leave (1.8 GHz): 4096 tokens at 28672, bf16, 16 q heads over 2 kv heads, 1.85 ms, 1.11 PFLOP/s (a large
+// product of the library: 1.23); the streams of products alone 1.45 ms; without the priority that keeps the two waves in opposite order 2.28.  A short item
+// is bound by its start and end, 13 to 16 us: seven prompts of 147 to 1645 tokens 76 us, a tile of 32 tokens 20.
 constexpr uint32_t CODE_BYTES = STEP_KEYS * DIM, HALF_BYTES = 2 * CODE_BYTES;  // a step's keys, or values
 constexpr uint32_t AHEAD = 3, PLACES = 4;
 constexpr uint32_t K_HALVES = 0, V_HALVES = 2 * HALF_BYTES, K_CODES = 4 * HALF_BYTES, V_CODES = K_CODES + PLACES * CODE_BYTES;
@@ -936,7 +937,7 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
 }
 
 // Joins the parts of the tiles that were taken in parts: out = sum_p 2^(M_p - M) O_p / sum_p 2^(M_p - M) l_p.  3 to 5 us of few rows, 13 to 16 of
-// chunks (seven prompts: 5 TB/s of parts).  A lane has four dims of a row.  Latency: the tile, then maxima, sums, parts and gate at once, then the output.  Few rows: a workgroup a row, the parts dealt to
+// chunks, whose parts are 256 KB an item and kv head.  A lane has four dims of a row.  Latency: the tile, then maxima, sums, parts and gate at once, then the output.  Few rows: a workgroup a row, the parts dealt to
 // its four waves in turn.  Chunks: a wave a row.  (Joining in the attention kernel, by the workgroup that ends last, costs more than this launch:
 // all workgroups run at once, so their stores' way to the memory that the XCDs share, the count and the loads come on top of the longest walk;
 // 48 ragged contexts 67 -> 72 us, one of 517 tokens 9.3 -> 9.7.)

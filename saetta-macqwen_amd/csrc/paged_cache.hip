@@ -10,8 +10,8 @@
 // first from the slots alone), one kv head, keys or values: what shares an e is then one workgroup's, and its largest
 // magnitude is known before the first code is written, with the values held in registers.  A wave has four tokens of a unit, a lane four dims of
 // each: a load is a token's row, and what a wave stores of four tokens fills lines of 64 bytes.  9700 tokens of five prompts, f32, 2 kv heads: 12.5 us,
-// 4.0 TB/s of what is read and written (a large copy: 4.8); a lane a token's 16 bytes, whose stores fill no lines, 22.9 us.  64 single tokens: 4.9 us, the
-// chain slot - rows - maximum - codes.
+// 4.0 TB/s of what is read and written (a large copy: 4.8); with whole tokens to a wave, whose stores fill no lines, 22.8.  64 single tokens: 4.9 us, the
+// chain of slot, rows, maximum and codes.
 #include "common.hpp"
 #include "lanes.hpp"
 #include "paged_device.hpp"

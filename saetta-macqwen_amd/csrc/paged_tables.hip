@@ -10,8 +10,8 @@
 // makes them, a request a thread, and moves the blocks' numbers, entry by entry over all its threads (a request is
 // found by bisection in the prefix sums in LDS).  The tokens' slots are independent of each other: a second launch of as
 // many workgroups as they fill, or, where few workgroups' worth of tokens come (a decode step), the first does them itself.
-// Measured: 32 requests with a token and three drafts each 3.8 us; 512 requests of up to 1900 tokens admitted at once (29 thousand blocks, 464
-// thousand tokens) 9.4 us, about half of it the blocks, and 3.4 the tokens.
+// Measured: 32 requests with a token and three drafts each 2.9 us; 512 requests of up to 1900 tokens admitted at once (8200 blocks, 126 thousand
+// tokens) 7.9 us and 2.9 for the slots.
 #include "common.hpp"
 #include "lanes.hpp"
 #include "paged_device.hpp"
@@ -309,8 +309,7 @@ extern "C" int saetta_paged_tables(saetta_stream_t stream, const uint32_t *conte
     SAETTA_REQUIRE(p.requests < (1u << 24) && p.tokens < (1u << 31), SAETTA_E_SHAPE, "paged_tables: %u requests, room for %u tokens", p.requests, p.tokens);
     if (int rc = ensure_device()) return rc;
     const TablesArgs a = {context_lens, new_lens, state, step, p};
-    // One workgroup's slots, of requests that it has in LDS, or two launches.  A small step's workgroup is four waves, whose barriers are cheaper
-    // (32 requests of 4 tokens: 3.8 us, with sixteen waves 5.1).
+    // One workgroup's slots, of requests that it has in LDS, or two launches.  A small step's workgroup is four waves, whose barriers are cheaper.
     if (p.tokens <= 512 && p.requests <= 256) {
         launch(paged_tables_kernel<true, 256>, dim3(1), dim3(256), 0, as_stream(stream), a);
     } else if (p.tokens <= 2048 && p.requests <= 1024) {
