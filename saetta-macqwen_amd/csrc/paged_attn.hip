@@ -85,11 +85,11 @@ struct SplitArgs {
     SplitHead *head;
     Item *items, *tiles;
     uint32_t tile_tokens, target, most_items, most_joined, slots, tokens, rows;
-    uint32_t few, granule, least, extra, half_tokens;  // (granule: a power of two)
+    uint32_t few, granule, least, extra, few_tokens, half_tokens;  // (granule: a power of two)
 };
 
-// What an item of a chunk costs besides its keys, in keys (15 us of a workgroup, and its sums' way through memory): seven prompts of 90 to 1900
-// tokens 118 us with 0, 115 with 256, 110 with 512, 123 with 1024; a chunk beside drafts 365, 353, 352, 352 a layer.
+// What an item of a chunk costs besides its keys, in keys (15 us of a workgroup, and its sums' way through memory): seven prompts of 147 to
+// 1645 tokens, attention and merge, 96 us with 0, 94 with 256, 92 with 512, 104 with 768; a chunk beside drafts the same with all.
 constexpr uint32_t CHUNK_EXTRA = 512;
 
 constexpr uint32_t SIZES = 64;  // classes of items by what they cost
@@ -143,8 +143,8 @@ __device__ __forceinline__ uint32_t before_this(uint32_t x, uint32_t *waves, uin
     return before + through - x;
 }
 
-// Deals the work out so that the workgroups that run at once end together.  What a key of a tile costs is one of two numbers: a chunk's tile of
-// at most half the rows keeps half the waves and takes 5 / 8 of the time.  A tile that costs more than total / target is cut into parts of that
+// Deals the work out so that the workgroups that run at once end together.  What a key of a tile costs is one of three numbers: a chunk's tile of
+// at most half the rows keeps half the waves and takes 6 / 8 of the time, one of up to 64 rows is taken as few rows are, by the memory's rate.  A tile that costs more than total / target is cut into parts of that
 // and a rest; the items go out from the dearest class to the cheapest, so that who ends early takes what is small.  (One workgroup: a sum over the
 // tiles, a count of the classes, and the items themselves; the tiles by turns over its threads.  The places of the items in a class and of the
 // parts' sums follow from atomic counts, in any order: what is computed does not depend on them.)  Latency: 5 us for one request, 7 for 48, 8.4 for a
@@ -185,8 +185,9 @@ __global__ __launch_bounds__(SPLIT_THREADS) void paged_split_kernel(SplitArgs a)
             __syncthreads();  // `starts` may be written again
         }
     };
-    constexpr uint32_t HALF = 5, WHOLE = 8;  // prices of a key
-    auto price = [&](const Item &tile) { return tile.tokens <= a.half_tokens ? HALF : WHOLE; };
+    // FEW: a chunk of 1500 tokens beside 30 drafts 283 us with 3, 267 with 4, 272 with 5.  HALF: seven prompts 92 us with 4, 79 with 5, 74 with 6 and 7.
+    constexpr uint32_t FEW = 4, HALF = 6, WHOLE = 8;
+    auto price = [&](const Item &tile) { return tile.tokens <= a.few_tokens ? FEW : tile.tokens <= a.half_tokens ? HALF : WHOLE; };
 
     // a number of every thread, added up into `into`, which is 0
     auto add_up = [&](unsigned long long x, unsigned long long *into) {
@@ -204,15 +205,18 @@ __global__ __launch_bounds__(SPLIT_THREADS) void paged_split_kernel(SplitArgs a)
         keys += a.granule;
         return uint32_t(keys > 0x7fffffffu ? 0x7fffffffu : keys) & ~(a.granule - 1);
     };
-    uint32_t half_length = length_at(fair / HALF), whole_length = length_at(fair / WHOLE);
-    auto length_of = [&](const Item &tile) { return tile.tokens <= a.half_tokens ? half_length : whole_length; };
+    uint32_t few_length = length_at(fair / FEW), half_length = length_at(fair / HALF), whole_length = length_at(fair / WHOLE);
+    // (sums: as three choices of a variable the compiler puts the tile in memory, and the kernel takes half as long again)
+    auto length_of = [&](const Item &tile) {
+        return whole_length + (tile.tokens <= a.half_tokens ? half_length - whole_length : 0) + (tile.tokens <= a.few_tokens ? few_length - half_length : 0);
+    };
     if (a.extra) {
         // An item costs `extra` keys besides its own (its start and end, its sums through memory): a share of as many items as there now are
         unsigned long long items = 0;
         for_tiles([&](const Item &tile) { items += tile.tokens ? max((tile.key1 + length_of(tile) - 1) / length_of(tile), 1u) : 0; });
         add_up(items, &items_there);
         if (items_there > a.target) fair += (items_there - a.target) * 8 * a.extra / a.target;
-        half_length = length_at(fair / HALF), whole_length = length_at(fair / WHOLE);
+        few_length = length_at(fair / FEW), half_length = length_at(fair / HALF), whole_length = length_at(fair / WHOLE);
     }
     const float per_class = float(SIZES) / float(fair + 8ull * a.granule);
     auto class_of = [&](uint32_t keys, uint32_t price) { return SIZES - 1 - min(uint32_t(float(keys) * float(price) * per_class), SIZES - 1); };
@@ -380,7 +384,7 @@ __device__ __forceinline__ void put_row(const AttnArgs &a, uint32_t row, uint32_
     store_values<TYPE, 4>(row_at<V>(a.out, row, head) + dim, o);
 }
 
-// Few rows: a workgroup of 4 waves walks an item's keys, every wave 32 of 128 at a time, straight from memory into registers, the
+// Few rows (a call's, or a tile's of a chunk call): a workgroup of 4 waves walks an item's keys, every wave 32 of 128 at a time, straight from memory into registers, the
 // keys of its next step on their way while this one's values are worked on, and the other way round.  Bound by memory: 16 KB a step of a
 // wave, against 64 + 64 conversions of two codes and, a group of 16 rows (COLUMNS of them), 16 + 16 products.  Row l % 16 of a group is lane
 // l's; the waves' sums are joined in LDS, a group after the other.  A wave looks up the places of the units of its next 32 steps by itself, a
@@ -393,33 +397,35 @@ __device__ __forceinline__ void put_row(const AttnArgs &a, uint32_t row, uint32_
 constexpr int few_threads(int columns) { return 64 * FEW_WAVES * (columns == 4 ? 2 : 1); }
 constexpr uint32_t FEW_STEPS = 32;     // steps that a wave looks up at a time
 constexpr int FEW_STRIDE = DIM + 4;    // floats of a row in LDS: neighbouring rows on other banks
-template <int TYPE, int TILE_COLUMNS>
-__global__ __launch_bounds__(few_threads(TILE_COLUMNS), TILE_COLUMNS == 2 ? 1 : 2) void paged_few_kernel(AttnArgs a) {
+// What the waves of a workgroup share.
+template <int COLUMNS, int TEAMS, int TURNS>
+struct FewShared {
+    float sums[TURNS][FEW_ROWS][FEW_STRIDE];
+    float ml[TURNS][FEW_ROWS][2];
+    u32x4 queries[TEAMS > 1 ? COLUMNS * TEAMS : 1][TEAMS > 1 ? 8 : 1][TEAMS > 1 ? 64 : 1];
+};
+// An item of up to COLUMNS * TEAMS groups by TEAMS teams of TURNS waves, COLUMNS groups to a wave; the parts' sums lie TILE rows apart.
+template <int TYPE, int COLUMNS, int TEAMS, int TURNS, uint32_t TILE>
+__device__ __forceinline__ void take_few(const AttnArgs &a, const Item &item, uint32_t kv, FewShared<COLUMNS, TEAMS, TURNS> &shared, uint32_t *nan_from) {
     typedef typename Row<TYPE>::value V;
-    constexpr uint32_t TILE = TILE_COLUMNS * FEW_ROWS;
-    constexpr int TEAMS = TILE_COLUMNS == 4 ? 2 : 1, COLUMNS = TILE_COLUMNS / TEAMS;  // groups of a wave
-    constexpr uint32_t WAVES = TEAMS * FEW_WAVES;
-    __shared__ __attribute__((aligned(16))) float sums[FEW_WAVES][FEW_ROWS][FEW_STRIDE];
-    __shared__ float ml[FEW_WAVES][FEW_ROWS][2];
-    __shared__ uint32_t nan_from[DIM];
-    const uint32_t index = blockIdx.x / a.cache.kv_heads, kv = blockIdx.x % a.cache.kv_heads;
-    const uint32_t items = a.head->items;
-    const Item item = a.items[index];
-    if (!(int(index < items) & int(item_ok(a, item, 1)))) return;
+    constexpr int TILE_COLUMNS = COLUMNS * TEAMS;
+    constexpr uint32_t WAVES = TEAMS * TURNS;
+    auto &sums = shared.sums;
+    auto &ml = shared.ml;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t col = lane & 15, quarter = lane >> 4;
-    const uint32_t team = wave / FEW_WAVES, turn = wave % FEW_WAVES;  // the wave's groups; its keys
+    const uint32_t team = wave / TURNS, turn = wave % TURNS;  // the wave's groups; its keys
     const uint32_t rows = item.tokens << a.group_shift;  // of the tile that are there
     for (uint32_t i = tid; i < DIM; i += 64 * WAVES) nan_from[i] = ~0u;
 
     const size_t block_bytes = size_t(DIM) << a.block_shift;
     const uint32_t unit_shift = a.block_shift - 4, unit_mask = (1u << unit_shift) - 1;
     const uint32_t end_unit = (item.key1 + UNIT_TOKENS - 1) / UNIT_TOKENS;
-    uint32_t first = item.key0 / UNIT_TOKENS + 2 * turn;  // the wave's first unit; its steps are 2 * FEW_WAVES units apart
+    uint32_t first = item.key0 / UNIT_TOKENS + 2 * turn;  // the wave's first unit; its steps are 2 * TURNS units apart
     // Lane 2 i + j: unit j of step i, its row of [blocks][kv heads] (of block 0 where there is none) and whether there is one.
     uint32_t place = 0, scales = 0;
     auto look_up = [&] {
-        const uint32_t unit = first + (lane >> 1) * (2 * FEW_WAVES) + (lane & 1), entry = unit >> unit_shift;
+        const uint32_t unit = first + (lane >> 1) * (2 * TURNS) + (lane & 1), entry = unit >> unit_shift;
         uint32_t block = ~0u;
         if (unit < end_unit && entry < a.max_blocks) block = uint32_t(a.block_table[size_t(item.request) * a.max_blocks + entry]);
         const bool there = block < a.cache.blocks;
@@ -431,14 +437,14 @@ __global__ __launch_bounds__(few_threads(TILE_COLUMNS), TILE_COLUMNS == 2 ? 1 : 
     auto fetch = [&](const uint8_t *codes, uint32_t step, u32x4 (&x)[2][4]) {
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            const uint32_t row = __builtin_amdgcn_readlane(place, 2 * step + i), unit = (first + step * (2 * FEW_WAVES) + i) & unit_mask;
+            const uint32_t row = __builtin_amdgcn_readlane(place, 2 * step + i), unit = (first + step * (2 * TURNS) + i) & unit_mask;
             const uint8_t *at = codes + row * block_bytes + unit * UNIT_BYTES;
 #pragma unroll
             for (int j = 0; j < 4; j++) x[i][j] = *reinterpret_cast<const u32x4 *>(at + j * 1024 + lane * 16);
         }
         __builtin_amdgcn_sched_barrier(0);  // (on their way from here on, not where they are wanted)
     };
-    uint32_t steps = first < end_unit ? (end_unit - first + 2 * FEW_WAVES - 1) / (2 * FEW_WAVES) : 0;  // that are left
+    uint32_t steps = first < end_unit ? (end_unit - first + 2 * TURNS - 1) / (2 * TURNS) : 0;  // that are left
     if (steps) {
         look_up();
         fetch(a.cache.keys, 0, k);
@@ -448,7 +454,7 @@ __global__ __launch_bounds__(few_threads(TILE_COLUMNS), TILE_COLUMNS == 2 ? 1 : 
     // The queries: [group][64 dims][8 of 16].  Of two teams they stay in LDS: two waves share the registers of a SIMD.
     constexpr bool IN_LDS = TEAMS > 1;
     u32x4 q[IN_LDS ? 1 : COLUMNS][8];
-    __shared__ u32x4 q_lds[IN_LDS ? TILE_COLUMNS : 1][IN_LDS ? 8 : 1][IN_LDS ? 64 : 1];
+    auto &q_lds = shared.queries;
     int32_t sees[COLUMNS];  // keys of this lane's rows
     auto row_of = [&](uint32_t g) { return min(g * FEW_ROWS + col, rows - 1); };
     auto q_of = [&](uint32_t g, int i) {
@@ -460,7 +466,7 @@ __global__ __launch_bounds__(few_threads(TILE_COLUMNS), TILE_COLUMNS == 2 ? 1 : 
     for (int g = 0; g < COLUMNS; g++) sees[g] = item.pos0 + int32_t(row_of(team * COLUMNS + g) >> a.group_shift) + 1;
     if constexpr (IN_LDS) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) q_lds[wave >> 1][(wave & 1) * 4 + i][lane] = q_of(wave >> 1, (wave & 1) * 4 + i);
+        for (uint32_t i = wave; i < TILE_COLUMNS * 8; i += WAVES) q_lds[i / 8][i % 8][lane] = q_of(i / 8, i % 8);
     } else {
 #pragma unroll
         for (int g = 0; g < COLUMNS; g++)
@@ -488,7 +494,7 @@ __global__ __launch_bounds__(few_threads(TILE_COLUMNS), TILE_COLUMNS == 2 ? 1 : 
     while (steps) {
         const uint32_t here = min(steps, FEW_STEPS);
         for (uint32_t step = 0; step < here; step++) {
-            const uint32_t key = (first + step * (2 * FEW_WAVES)) * UNIT_TOKENS;
+            const uint32_t key = (first + step * (2 * TURNS)) * UNIT_TOKENS;
             floatx4 s[COLUMNS][2];
 #pragma unroll
             for (int g = 0; g < COLUMNS; g++) s[g][0] = s[g][1] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -565,7 +571,7 @@ __global__ __launch_bounds__(few_threads(TILE_COLUMNS), TILE_COLUMNS == 2 ? 1 : 
         }
         steps -= here;
         if (steps) {
-            first += FEW_STEPS * 2 * FEW_WAVES;
+            first += FEW_STEPS * 2 * TURNS;
             look_up();
             fetch(a.cache.keys, 0, k);
             look_up_scales();
@@ -590,9 +596,9 @@ __global__ __launch_bounds__(few_threads(TILE_COLUMNS), TILE_COLUMNS == 2 ? 1 : 
             const uint32_t r = g * FEW_ROWS + i, dim = lane * 4;
             float top = NO_MAXIMUM, sum = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int w = 0; w < FEW_WAVES; w++) top = fmaxf(top, ml[w][i][0]);
+            for (int w = 0; w < TURNS; w++) top = fmaxf(top, ml[w][i][0]);
 #pragma unroll
-            for (int w = 0; w < FEW_WAVES; w++) {
+            for (int w = 0; w < TURNS; w++) {
                 const float f = __builtin_amdgcn_exp2f(ml[w][i][0] - top);
                 sum = fmaf(ml[w][i][1], f, sum);
                 const floatx4 x = *reinterpret_cast<const floatx4 *>(&sums[w][i][dim]);
@@ -617,6 +623,18 @@ __global__ __launch_bounds__(few_threads(TILE_COLUMNS), TILE_COLUMNS == 2 ? 1 : 
     }
 }
 
+template <int TYPE, int TILE_COLUMNS>
+__global__ __launch_bounds__(few_threads(TILE_COLUMNS), TILE_COLUMNS == 2 ? 1 : 2) void paged_few_kernel(AttnArgs a) {
+    constexpr int TEAMS = TILE_COLUMNS == 4 ? 2 : 1, COLUMNS = TILE_COLUMNS / TEAMS;
+    __shared__ __attribute__((aligned(16))) FewShared<COLUMNS, TEAMS, FEW_WAVES> shared;
+    __shared__ uint32_t nan_from[DIM];
+    const uint32_t index = blockIdx.x / a.cache.kv_heads, kv = blockIdx.x % a.cache.kv_heads;
+    const uint32_t items = a.head->items;
+    const Item item = a.items[index];
+    if (!(int(index < items) & int(item_ok(a, item, 1)))) return;
+    take_few<TYPE, COLUMNS, TEAMS, FEW_WAVES, TILE_COLUMNS * FEW_ROWS>(a, item, kv, shared, nan_from);
+}
+
 // A workgroup barrier for what went through LDS: the copies of later steps stay on their way (__syncthreads waits for them).
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
@@ -637,6 +655,10 @@ constexpr uint32_t K_HALVES = 0, V_HALVES = 2 * HALF_BYTES, K_CODES = 4 * HALF_B
 constexpr uint32_t OUT_STRIDE = 128 + 4;  // floats of half a row on its way out, and the row's sum
 constexpr uint32_t OUT_BYTES = CHUNK_ROWS * OUT_STRIDE * 4;
 constexpr uint32_t CHUNK_LDS = OUT_BYTES > V_CODES + PLACES * CODE_BYTES ? OUT_BYTES : V_CODES + PLACES * CODE_BYTES;
+template <int N>
+struct Count {
+    static constexpr int value = N;
+};
 template <int TYPE>
 __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnArgs a) {
     typedef typename Row<TYPE>::value V;
@@ -650,6 +672,17 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
     if (!(int(index < items) & int(item_ok(a, item, 1)))) return;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t rows = item.tokens << a.group_shift;
+    if (rows <= 4 * FEW_ROWS) {  // (a draft beside a chunk, a prompt's last tokens)
+        auto few = [&](auto teams, auto turns) {
+            typedef FewShared<1, decltype(teams)::value, decltype(turns)::value> Shared;
+            static_assert(sizeof(Shared) <= CHUNK_LDS, "in the tiles' place");
+            take_few<TYPE, 1, decltype(teams)::value, decltype(turns)::value, CHUNK_ROWS>(a, item, kv, *reinterpret_cast<Shared *>(tiles), nan_from);
+        };
+        if (rows <= FEW_ROWS) few(Count<1>(), Count<8>());
+        else if (rows <= 2 * FEW_ROWS) few(Count<2>(), Count<4>());
+        else few(Count<4>(), Count<2>());
+        return;
+    }
     for (uint32_t i = tid; i < DIM; i += 64 * CHUNK_WAVES) nan_from[i] = ~0u;
     const uint32_t unit0 = item.key0 / UNIT_TOKENS, end_unit = (item.key1 + UNIT_TOKENS - 1) / UNIT_TOKENS;
     const uint32_t steps = end_unit > unit0 ? (end_unit - unit0 + 1) / 2 : 0;
@@ -1091,7 +1124,7 @@ extern "C" int saetta_paged_split(saetta_stream_t stream, saetta_paged_batch bat
     const bool few = s.columns > 0;
     const SplitArgs a = {batch, reinterpret_cast<SplitHead *>(at), reinterpret_cast<Item *>(at + items_offset()), reinterpret_cast<Item *>(at + tiles_offset(s)),
                          s.tile_tokens, s.target, s.most_items, s.most_joined, s.slots, p.tokens, p.rows,
-                         few, few ? STEP_KEYS * FEW_WAVES : STEP_KEYS, few ? STEP_KEYS * FEW_WAVES : 256u, few ? 0u : CHUNK_EXTRA, few ? 0u : s.tile_tokens / 2};
+                         few, few ? STEP_KEYS * FEW_WAVES : STEP_KEYS, few ? STEP_KEYS * FEW_WAVES : 256u, few ? 0u : CHUNK_EXTRA, few ? 0u : 4 * FEW_ROWS / s.group, few ? 0u : s.tile_tokens / 2};
     // (few tiles: four waves, whose barriers are cheaper)
     if (s.most_tiles <= 256) launch(paged_split_kernel<256>, dim3(1), dim3(256), 0, as_stream(stream), a);
     else launch(paged_split_kernel<1024>, dim3(1), dim3(1024), 0, as_stream(stream), a);

@@ -325,6 +325,29 @@ def test_keys_in_parts(new, block):
     b.compare()
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("heads, kv_heads", [(16, 2), (4, 4), (16, 1)])
+def test_a_few_rows_beside_a_chunk(heads, kv_heads, dtype):
+    """Requests of every width of a tile of few rows, short and long, whole and in parts, in the step of a chunk."""
+    new = [1, 2, 3, 4, 5, 8, 9, 16, 17, 33, 64, 65, 90]
+    b = Batch(18, [2600, 0, 1, 900, 31, 1700, 2, 0, 450, 7, 100, 33, 70], new, 32, heads, kv_heads, dtype, room=3)
+    b.run()
+    b.compare()
+
+
+def test_no_numbers_beside_a_chunk():
+    """NaN among the values and keys of drafts and of a prompt's last tokens: rows that see it are NaN, the others are not touched."""
+    b = Batch(19, [700, 40, 64, 500], [3, 2, 70, 1], 16, 16, 2, F16)
+    block = host(b.tables.block_table)
+    for request, at in ((0, 701), (1, 41), (2, 130), (3, 3)):  # token t of its block, dim 5
+        t = at % 16
+        b.cache.values[int(block[request, at // 16]), 1, (t // 4 * 16 + 5) * 16 + t % 4] = 0x7f
+    b.run()
+    b.compare()
+    got = numbers(b.out)
+    assert np.isnan(got[:, 8:, 5]).sum() == 8 * (2 + 1 + 4 + 1) and not np.isnan(got[:, :8]).any()
+
+
 def test_scales_that_differ_widely():
     """Neighbouring blocks 2^20 apart, keys and values; a block of zeros."""
     for new in (1, 5):
