@@ -969,11 +969,13 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
     }
 }
 
-// Joins the parts of the tiles that were taken in parts: out = sum_p 2^(M_p - M) O_p / sum_p 2^(M_p - M) l_p.  3 to 5 us of few rows, 13 to 16 of
-// chunks, whose parts are 256 KB an item and kv head.  A lane has four dims of a row.  Latency: the tile, then maxima, sums, parts and gate at once, then the output.  Few rows: a workgroup a row, the parts dealt to
-// its four waves in turn.  Chunks: a wave a row.  (Joining in the attention kernel, by the workgroup that ends last, costs more than this launch:
-// all workgroups run at once, so their stores' way to the memory that the XCDs share, the count and the loads come on top of the longest walk;
-// 48 ragged contexts 67 -> 72 us, one of 517 tokens 9.3 -> 9.7.)
+// Joins the parts of the tiles that were taken in parts: out = sum_p 2^(M_p - M) O_p / sum_p 2^(M_p - M) l_p.  A lane has four dims of a row.  3 to
+// 5 us of few rows, by latency: the tile, then maxima, sums, parts and gate at once, then the output; a workgroup a row, the parts dealt to its four waves
+// in turn.  11 to 18 of chunks, whose parts are 256 KB an item and kv head: a wave two rows, one after the other, for half as many workgroups to launch.
+// (Joining in the attention kernel, by the workgroup that ends last, costs more than this launch: all workgroups run at once, so their stores' way
+// to the memory that the XCDs share, the count and the loads come on top of the longest walk; 48 ragged contexts 67 -> 72 us, one of 517 tokens 9.3
+// -> 9.7.)
+constexpr uint32_t MERGE_ROWS = 2;  // of a wave, of chunks: seven prompts 13.2 us with 1, 10.9 with 2, 11.9 with 4; a chunk at 28672 16.8, 13.0, 13.4
 template <int TYPE, int COLUMNS>
 __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, const Item *tiles) {
     typedef typename Row<TYPE>::value V;
@@ -983,66 +985,68 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, const Item
     const Item item = tiles[blockIdx.x];
     if (!(int(blockIdx.x < there) & int(item.parts > 1) & int(item_ok(a, item, item.parts)))) return;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t r = FEW ? blockIdx.y : blockIdx.y * 4 + wave;
-    if (r >= item.tokens << a.group_shift) return;  // (FEW: the whole workgroup)
-    const size_t stride = size_t(a.cache.kv_heads) * TILE, slot = (size_t(item.slot) * a.cache.kv_heads + kv) * TILE + r;
-    const uint32_t row = item.row0 + (r >> a.group_shift);
-    const uint32_t head = kv * a.group + (r & (a.group - 1)), dim = lane * 4;
-    float gate[4];
-    if (a.gate.data) load_values<TYPE, 4>(row_at<const V>(a.gate, row, head) + dim, gate);
+    const uint32_t rows = item.tokens << a.group_shift, r0 = FEW ? blockIdx.y : (blockIdx.y * 4 + wave) * MERGE_ROWS;
+    if (FEW && r0 >= rows) return;  // (the whole workgroup)
+    for (uint32_t r = r0; r < (FEW ? r0 + 1 : min(r0 + MERGE_ROWS, rows)); r++) {
+        const size_t stride = size_t(a.cache.kv_heads) * TILE, slot = (size_t(item.slot) * a.cache.kv_heads + kv) * TILE + r;
+        const uint32_t row = item.row0 + (r >> a.group_shift);
+        const uint32_t head = kv * a.group + (r & (a.group - 1)), dim = lane * 4;
+        float gate[4];
+        if (a.gate.data) load_values<TYPE, 4>(row_at<const V>(a.gate, row, head) + dim, gate);
 
-    float m = NO_MAXIMUM, l = 0.0f;
-    floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t p0 = FEW ? wave : 0; p0 < item.parts; p0 += BY * AT_ONCE) {
-        float2 ml[AT_ONCE];
-        floatx4 x[AT_ONCE];
+        float m = NO_MAXIMUM, l = 0.0f;
+        floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t p0 = FEW ? wave : 0; p0 < item.parts; p0 += BY * AT_ONCE) {
+            float2 ml[AT_ONCE];
+            floatx4 x[AT_ONCE];
 #pragma unroll
-        for (uint32_t i = 0; i < AT_ONCE; i++) {
-            ml[i] = float2{NO_MAXIMUM, 0.0f}, x[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (p0 + i * BY < item.parts) {  // (for the wave alike)
-                const size_t at = slot + (p0 + i * BY) * stride;
-                ml[i] = *reinterpret_cast<const float2 *>(a.part_ml + at * 2);
-                x[i] = *reinterpret_cast<const floatx4 *>(a.part_o + at * DIM + dim);
+            for (uint32_t i = 0; i < AT_ONCE; i++) {
+                ml[i] = float2{NO_MAXIMUM, 0.0f}, x[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+                if (p0 + i * BY < item.parts) {  // (for the wave alike)
+                    const size_t at = slot + (p0 + i * BY) * stride;
+                    ml[i] = *reinterpret_cast<const float2 *>(a.part_ml + at * 2);
+                    x[i] = *reinterpret_cast<const floatx4 *>(a.part_o + at * DIM + dim);
+                }
+            }
+            float top = m;
+#pragma unroll
+            for (uint32_t i = 0; i < AT_ONCE; i++) top = fmaxf(top, ml[i].x);
+            const float down = __builtin_amdgcn_exp2f(m - top);
+            m = top, l *= down, o *= down;
+#pragma unroll
+            for (uint32_t i = 0; i < AT_ONCE; i++) {
+                const float f = __builtin_amdgcn_exp2f(ml[i].x - top);
+                l = fmaf(ml[i].y, f, l);
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[j] = fmaf(x[i][j], f, o[j]);
             }
         }
-        float top = m;
+        if constexpr (FEW) {
+            __shared__ __attribute__((aligned(16))) float part[4][64][4];
+            __shared__ float pml[4][2];
+            *reinterpret_cast<floatx4 *>(part[wave][lane]) = o;
+            if (lane == 0) pml[wave][0] = m, pml[wave][1] = l;
+            __syncthreads();
+            if (wave > 0) return;
+            float top = NO_MAXIMUM;
 #pragma unroll
-        for (uint32_t i = 0; i < AT_ONCE; i++) top = fmaxf(top, ml[i].x);
-        const float down = __builtin_amdgcn_exp2f(m - top);
-        m = top, l *= down, o *= down;
+            for (int w = 0; w < 4; w++) top = fmaxf(top, pml[w][0]);
+            l = 0.0f, o = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (uint32_t i = 0; i < AT_ONCE; i++) {
-            const float f = __builtin_amdgcn_exp2f(ml[i].x - top);
-            l = fmaf(ml[i].y, f, l);
+            for (int w = 0; w < 4; w++) {
+                const float f = __builtin_amdgcn_exp2f(pml[w][0] - top);
+                l = fmaf(pml[w][1], f, l);
+                const floatx4 x = *reinterpret_cast<const floatx4 *>(part[w][lane]);
 #pragma unroll
-            for (int j = 0; j < 4; j++) o[j] = fmaf(x[i][j], f, o[j]);
+                for (int i = 0; i < 4; i++) o[i] = fmaf(x[i], f, o[i]);
+            }
         }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = a.gate.data ? o[i] * inv * sigmoid(gate[i]) : o[i] * inv;
+        store_values<TYPE, 4>(row_at<V>(a.out, row, head) + dim, x);
     }
-    if constexpr (FEW) {
-        __shared__ __attribute__((aligned(16))) float part[4][64][4];
-        __shared__ float pml[4][2];
-        *reinterpret_cast<floatx4 *>(part[wave][lane]) = o;
-        if (lane == 0) pml[wave][0] = m, pml[wave][1] = l;
-        __syncthreads();
-        if (wave > 0) return;
-        float top = NO_MAXIMUM;
-#pragma unroll
-        for (int w = 0; w < 4; w++) top = fmaxf(top, pml[w][0]);
-        l = 0.0f, o = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int w = 0; w < 4; w++) {
-            const float f = __builtin_amdgcn_exp2f(pml[w][0] - top);
-            l = fmaf(pml[w][1], f, l);
-            const floatx4 x = *reinterpret_cast<const floatx4 *>(part[w][lane]);
-#pragma unroll
-            for (int i = 0; i < 4; i++) o[i] = fmaf(x[i], f, o[i]);
-        }
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    float x[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) x[i] = a.gate.data ? o[i] * inv * sigmoid(gate[i]) : o[i] * inv;
-    store_values<TYPE, 4>(row_at<V>(a.out, row, head) + dim, x);
 }
 
 int check_attn(const saetta_paged_attn_params &p, uint32_t requests, const char *what) {
@@ -1084,7 +1088,7 @@ void launch_attn(hipStream_t stream, const AttnArgs &a, const Shape &s, const sa
         case 4: return few(paged_few_kernel<TYPE, 4>, paged_merge_kernel<TYPE, 4>);
     }
     launch(paged_chunk_kernel<TYPE>, grid, dim3(64 * CHUNK_WAVES), CHUNK_LDS, stream, a);
-    launch(paged_merge_kernel<TYPE, 0>, dim3(s.most_joined, CHUNK_ROWS / 4, p.kv_heads), dim3(256), 0, stream, a, tiles);
+    launch(paged_merge_kernel<TYPE, 0>, dim3(s.most_joined, CHUNK_ROWS / 4 / MERGE_ROWS, p.kv_heads), dim3(256), 0, stream, a, tiles);
 }
 
 }  // namespace
