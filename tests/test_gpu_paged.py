@@ -457,6 +457,49 @@ def test_two_calls_at_once():
     one.compare(), two.compare()
 
 
+def test_chunks_same_bits_every_time_and_in_the_place_of_q():
+    """Prompts in parts beside drafts: which workgroup takes what differs from call to call, the bits do not."""
+    b = Batch(20, [6000, 10, 900, 0, 2500], [100, 3, 7, 200, 1], 32, 16, 2, F16)
+    b.run()
+    b.compare()
+    first = b.out.clone()
+    for _ in range(4):
+        b.out.fill_(1.0)
+        b.run()
+        assert torch.equal(b.out, first)
+    b.out = b.q
+    b.run()
+    assert torch.equal(b.out, first)
+
+
+@pytest.mark.parametrize("chunk", [0, 70])
+def test_more_requests_than_a_workgroup_has_threads(chunk):
+    """Tables, split and attention of 1500 requests (and one with a chunk): their rounds."""
+    gen = np.random.default_rng(22)
+    context, new = gen.integers(0, 40, 1500).tolist(), gen.integers(0, 3, 1500).tolist()
+    if chunk:
+        new[1100] = chunk
+    b = Batch(22, context, new, 16, 2, 1, F16, room=2)
+    b.run()
+    b.compare()
+    starts, lens = b.tables.query_starts.clone(), b.tables.kv_lens.clone()
+    t = saetta.PagedTables(1500, sum(new) + 2, b.tables.max_blocks, 6000, 16)
+    state = plain_state(t)
+    t.encode(ints(context), ints(new))
+    compare_tables(t, state, tables(state, context, new, 16, sum(new) + 2), sum(new) + 2)
+    assert torch.equal(t.query_starts, starts) and torch.equal(t.kv_lens, lens)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_blocks_that_requests_share(new):
+    """Three requests behind one prefix: their tables name the same blocks."""
+    b = Batch(23, [96, 96, 96, 5], [new, new, new, 1], 32, 16, 2, BF16)
+    t = b.tables
+    t.block_table[1, :3], t.block_table[2, :3] = t.block_table[0, :3], t.block_table[0, :3]
+    b.run()
+    b.compare()
+
+
 def test_python_objects_refuse_on_the_gpu():
     b = Batch(17, [9], [1], 16, 16, 2, F16)
     other = saetta.PagedTables(2, 1, 2, 4, 16)
