@@ -402,7 +402,8 @@ template <int COLUMNS, int TEAMS, int TURNS>
 struct FewShared {
     float sums[TURNS][FEW_ROWS][FEW_STRIDE];
     float ml[TURNS][FEW_ROWS][2];
-    u32x4 queries[TEAMS > 1 ? COLUMNS * TEAMS : 1][TEAMS > 1 ? 8 : 1][TEAMS > 1 ? 64 : 1];
+    static constexpr bool IN_LDS = TEAMS * TURNS == 8 && TEAMS * COLUMNS > 1;  // the queries: two waves share the registers of a SIMD
+    u32x4 queries[IN_LDS ? COLUMNS * TEAMS : 1][IN_LDS ? 8 : 1][IN_LDS ? 64 : 1];
 };
 // An item of up to COLUMNS * TEAMS groups by TEAMS teams of TURNS waves, COLUMNS groups to a wave; the parts' sums lie TILE rows apart.
 template <int TYPE, int COLUMNS, int TEAMS, int TURNS, uint32_t TILE>
@@ -451,8 +452,8 @@ __device__ __forceinline__ void take_few(const AttnArgs &a, const Item &item, ui
         look_up_scales();
     }
 
-    // The queries: [group][64 dims][8 of 16].  Of two teams they stay in LDS: two waves share the registers of a SIMD.
-    constexpr bool IN_LDS = TEAMS > 1;
+    // The queries: [group][64 dims][8 of 16].
+    constexpr bool IN_LDS = FewShared<COLUMNS, TEAMS, TURNS>::IN_LDS;
     u32x4 q[IN_LDS ? 1 : COLUMNS][8];
     auto &q_lds = shared.queries;
     int32_t sees[COLUMNS];  // keys of this lane's rows
@@ -654,7 +655,8 @@ constexpr uint32_t AHEAD = 3, PLACES = 4;
 constexpr uint32_t K_HALVES = 0, V_HALVES = 2 * HALF_BYTES, K_CODES = 4 * HALF_BYTES, V_CODES = K_CODES + PLACES * CODE_BYTES;
 constexpr uint32_t OUT_STRIDE = 128 + 4;  // floats of half a row on its way out, and the row's sum
 constexpr uint32_t OUT_BYTES = CHUNK_ROWS * OUT_STRIDE * 4;
-constexpr uint32_t CHUNK_LDS = OUT_BYTES > V_CODES + PLACES * CODE_BYTES ? OUT_BYTES : V_CODES + PLACES * CODE_BYTES;
+constexpr uint32_t TILE_LDS = OUT_BYTES > V_CODES + PLACES * CODE_BYTES ? OUT_BYTES : V_CODES + PLACES * CODE_BYTES;
+constexpr uint32_t CHUNK_LDS = TILE_LDS > sizeof(FewShared<2, 1, CHUNK_WAVES>) ? TILE_LDS : sizeof(FewShared<2, 1, CHUNK_WAVES>);
 template <int N>
 struct Count {
     static constexpr int value = N;
@@ -672,15 +674,18 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
     if (!(int(index < items) & int(item_ok(a, item, 1)))) return;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t rows = item.tokens << a.group_shift;
-    if (rows <= 4 * FEW_ROWS) {  // (a draft beside a chunk, a prompt's last tokens)
-        auto few = [&](auto teams, auto turns) {
-            typedef FewShared<1, decltype(teams)::value, decltype(turns)::value> Shared;
+    // A draft beside a chunk, a prompt's last tokens.  (64 requests of 2, 4, 8 tokens at 4000, by this kernel: 44, 55, 76 us; by the one for few rows 44, 50, 69.
+    // With one group to a wave and more teams, which spills no registers, 44, 70, 81.)
+    if (rows <= 4 * FEW_ROWS) {
+        auto few = [&](auto columns, auto teams) {
+            constexpr int COLUMNS = decltype(columns)::value, TEAMS = decltype(teams)::value, TURNS = CHUNK_WAVES / TEAMS;
+            typedef FewShared<COLUMNS, TEAMS, TURNS> Shared;
             static_assert(sizeof(Shared) <= CHUNK_LDS, "in the tiles' place");
-            take_few<TYPE, 1, decltype(teams)::value, decltype(turns)::value, CHUNK_ROWS>(a, item, kv, *reinterpret_cast<Shared *>(tiles), nan_from);
+            take_few<TYPE, COLUMNS, TEAMS, TURNS, CHUNK_ROWS>(a, item, kv, *reinterpret_cast<Shared *>(tiles), nan_from);
         };
-        if (rows <= FEW_ROWS) few(Count<1>(), Count<8>());
-        else if (rows <= 2 * FEW_ROWS) few(Count<2>(), Count<4>());
-        else few(Count<4>(), Count<2>());
+        if (rows <= FEW_ROWS) few(Count<1>(), Count<1>());
+        else if (rows <= 2 * FEW_ROWS) few(Count<2>(), Count<1>());
+        else few(Count<2>(), Count<2>());
         return;
     }
     for (uint32_t i = tid; i < DIM; i += 64 * CHUNK_WAVES) nan_from[i] = ~0u;
