@@ -198,7 +198,7 @@ __global__ __launch_bounds__(256) void paged_gather_kernel(GatherArgs a) {
         of_codes(near ? bytes(units[unit == first ? 0 : 1]) : bytes(codes_of(unit)), x);
 #pragma unroll
         for (int j = 0; j < 4; j++) x[j] *= scale;
-        store_values<TYPE, 4>(static_cast<V *>(a.out[which]) + ((row0 + i) * a.kv_heads + head) * SAETTA_HEAD_DIM + dim, x);
+        store_values<TYPE, 4, true>(static_cast<V *>(a.out[which]) + ((row0 + i) * a.kv_heads + head) * SAETTA_HEAD_DIM + dim, x);
     }
 }
 

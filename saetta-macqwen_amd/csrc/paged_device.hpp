@@ -101,7 +101,7 @@ __device__ __forceinline__ void load_values(const typename Row<TYPE>::value *p, 
         for (int j = 0; j < PER; j++) x[i + j] = Row<TYPE>::load(v[j]);
     }
 }
-template <int TYPE, int N>
+template <int TYPE, int N, bool PASSING = false>  // PASSING: by the caches
 __device__ __forceinline__ void store_values(typename Row<TYPE>::value *p, const float (&x)[N]) {
     typedef typename Row<TYPE>::value V;
     constexpr int PER = N * sizeof(V) < 16 ? N : 16 / sizeof(V);
@@ -111,7 +111,8 @@ __device__ __forceinline__ void store_values(typename Row<TYPE>::value *p, const
         vec v;
 #pragma unroll
         for (int j = 0; j < PER; j++) v[j] = Row<TYPE>::store(x[i + j]);
-        *reinterpret_cast<vec *>(p + i) = v;
+        if constexpr (PASSING) __builtin_nontemporal_store(v, reinterpret_cast<vec *>(p + i));
+        else *reinterpret_cast<vec *>(p + i) = v;
     }
 }
 
