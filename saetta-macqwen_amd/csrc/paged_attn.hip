@@ -392,8 +392,8 @@ __device__ __forceinline__ void put_row(const AttnArgs &a, uint32_t row, uint32_
 // One group is two workgroups to a CU; two have the registers of a SIMD to themselves; of four, two teams of four waves take two each over the
 // same keys, whose codes the second team finds in the caches.  (The kernel for chunks, where most of a tile is empty, takes 102 to 108 us for 64 drafts of 3
 // to 8 rows at 4000 tokens, this one 46 to 69; four groups to a wave are more registers than there are: 353.)
-// Measured, 8 q heads over each of 2 kv heads: a token of 8 requests at 131072 tokens, f16, 184 us, 5.9 TB/s of codes (a large copy reaches 4.8, read and
-// written); of 48 requests at 330 to 30 thousand tokens, bf16, 62 us, 5.2 TB/s; of one at 517 tokens 6.3 us, the launch and three loads that wait for each other.
+// Measured, 8 q heads over each of 2 kv heads: a token of 8 requests at 131072 tokens, f16, 162 us, 6.6 TB/s of codes (a large copy reaches 4.8, read and
+// written); of 48 requests at 330 to 30 thousand tokens, bf16, 55 us, 5.9 TB/s; of one at 517 tokens 6.3 us, the launch and three loads that wait for each other.
 constexpr int few_threads(int columns) { return 64 * FEW_WAVES * (columns == 4 ? 2 : 1); }
 constexpr uint32_t FEW_STEPS = 32;     // steps that a wave looks up at a time
 constexpr int FEW_STRIDE = DIM + 4;    // floats of a row in LDS: neighbouring rows on other banks
@@ -435,13 +435,20 @@ __device__ __forceinline__ void take_few(const AttnArgs &a, const Item &item, ui
     };
     auto look_up_scales = [&] { scales |= uint32_t(a.cache.key_scales[place]) | uint32_t(a.cache.value_scales[place]) << 8; };
     u32x4 k[2][4], v[2][4];  // codes of a step: [unit][64 dims]
+    // (One team's codes are read once, and between two steps of a model its weights go through the caches: marked as such, what is read keeps no
+    // place there.  64 requests of 8000 tokens 93.4 -> 82.3 us, 48 ragged 63 -> 55, 16 of 2000 the same; where the last call left the codes in the caches
+    // 41.8 -> 43.1, where 48 requests share all their 8000 tokens 30.6 -> 37.8.)
     auto fetch = [&](const uint8_t *codes, uint32_t step, u32x4 (&x)[2][4]) {
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             const uint32_t row = __builtin_amdgcn_readlane(place, 2 * step + i), unit = (first + step * (2 * TURNS) + i) & unit_mask;
             const uint8_t *at = codes + row * block_bytes + unit * UNIT_BYTES;
 #pragma unroll
-            for (int j = 0; j < 4; j++) x[i][j] = *reinterpret_cast<const u32x4 *>(at + j * 1024 + lane * 16);
+            for (int j = 0; j < 4; j++) {
+                const u32x4 *from = reinterpret_cast<const u32x4 *>(at + j * 1024 + lane * 16);
+                if constexpr (TEAMS == 1) x[i][j] = __builtin_nontemporal_load(from);
+                else x[i][j] = *from;
+            }
         }
         __builtin_amdgcn_sched_barrier(0);  // (on their way from here on, not where they are wanted)
     };
