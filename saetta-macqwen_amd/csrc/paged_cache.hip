@@ -158,8 +158,9 @@ struct GatherArgs {
 
 // A workgroup takes 16 slots of one kv head, keys or values: a wave a slot at a time, a lane four dims, so that a store is a whole row.
 // Where the slots lie in two units at most (16 that follow each other do), the units come through LDS by whole kilobytes, for values are stored
-// four tokens to a dword; else a lane reads its bytes where they are.  32768 tokens, f16, 2 kv heads: 21.5 us, 4.7 TB/s of what is read and written (a
-// lane's bytes straight from memory: 42 us).
+// four tokens to a dword; else a lane reads its bytes where they are.  32768 tokens, f16, 2 kv heads: 19.4 us, 5.2 TB/s of what is read and written.  (A
+// lane's bytes straight from memory: 42 us.  Rows that keep a place in the caches on their way out: 29 where every call has other data, and who reads them
+// next takes as long either way.)
 constexpr uint32_t GATHER_SLOTS = 16;
 template <int TYPE>
 __global__ __launch_bounds__(256) void paged_gather_kernel(GatherArgs a) {
