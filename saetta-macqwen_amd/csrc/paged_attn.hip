@@ -91,6 +91,8 @@ struct SplitArgs {
 // What an item of a chunk costs besides its keys, in keys (15 us of a workgroup, and its sums' way through memory): seven prompts of 147 to
 // 1645 tokens, attention and merge, 96 us with 0, 94 with 256, 92 with 512, 104 with 768; a chunk beside drafts the same with all.
 constexpr uint32_t CHUNK_EXTRA = 512;
+// Keys that a part has at least.  32 tokens at 992 41 us with 512, 30 with 256, 25 with 128 and 64; 300 at 0 37, 37, 32, 30; 32 at 8000 46, 41, 41, 49.
+constexpr uint32_t LEAST_KEYS = 128;
 
 constexpr uint32_t SIZES = 64;  // classes of items by what they cost
 
@@ -981,25 +983,28 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
     }
 }
 
-// Joins the parts of the tiles that were taken in parts: out = sum_p 2^(M_p - M) O_p / sum_p 2^(M_p - M) l_p.  A lane has four dims of a row.  3 to
-// 5 us of few rows, by latency: the tile, then maxima, sums, parts and gate at once, then the output; a workgroup a row, the parts dealt to its four waves
-// in turn.  11 to 18 of chunks, whose parts are 256 KB an item and kv head: a wave two rows, one after the other, for half as many workgroups to launch.
+// Joins the parts of the tiles that were taken in parts: out = sum_p 2^(M_p - M) O_p / sum_p 2^(M_p - M) l_p.  A lane has four dims of a row.  WIDE:
+// a workgroup a row, the parts dealt to its four waves in turn; 3 to 5 us of few rows, by latency: the tile, then maxima, sums, parts and gate at once,
+// then the output.  Of chunks, whose parts are 256 KB an item and kv head, up to WIDE_TILES tiles are joined so too; else a wave takes two rows, one
+// after the other, for an eighth of the workgroups to launch: 11 to 17 us.
 // (Joining in the attention kernel, by the workgroup that ends last, costs more than this launch: all workgroups run at once, so their stores' way
 // to the memory that the XCDs share, the count and the loads come on top of the longest walk; 48 ragged contexts 67 -> 72 us, one of 517 tokens 9.3
 // -> 9.7.)
-constexpr uint32_t MERGE_ROWS = 2;  // of a wave, of chunks: seven prompts 13.2 us with 1, 10.9 with 2, 11.9 with 4; a chunk at 28672 16.8, 13.0, 13.4
-template <int TYPE, int COLUMNS>
+constexpr uint32_t MERGE_ROWS = 2;  // seven prompts 13.2 us with 1, 10.9 with 2, 11.9 with 4; a chunk at 28672 16.8, 13.0, 13.4
+// 32 tokens at 8000 (2 tiles at most) 17.1 us by waves, 10.9 wide; 100 at 3000 (4) 9.5 and 7.2; 200 at 20000 (7) 12.1 and 12.6; 300 at 0 (10) 4.6 and 5.9; seven
+// prompts 10.9 and 31.9.
+constexpr uint32_t WIDE_TILES = 6;
+template <int TYPE, uint32_t TILE, bool WIDE>
 __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, const Item *tiles) {
     typedef typename Row<TYPE>::value V;
-    constexpr bool FEW = COLUMNS > 0;
-    constexpr uint32_t TILE = FEW ? COLUMNS * FEW_ROWS : CHUNK_ROWS, BY = FEW ? 4 : 1, AT_ONCE = FEW ? 8 : 4;
+    constexpr uint32_t BY = WIDE ? 4 : 1, AT_ONCE = WIDE ? 8 : 4;
     const uint32_t there = a.head->tiles, kv = blockIdx.z;
     const Item item = tiles[blockIdx.x];
     if (!(int(blockIdx.x < there) & int(item.parts > 1) & int(item_ok(a, item, item.parts)))) return;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t rows = item.tokens << a.group_shift, r0 = FEW ? blockIdx.y : (blockIdx.y * 4 + wave) * MERGE_ROWS;
-    if (FEW && r0 >= rows) return;  // (the whole workgroup)
-    for (uint32_t r = r0; r < (FEW ? r0 + 1 : min(r0 + MERGE_ROWS, rows)); r++) {
+    const uint32_t rows = item.tokens << a.group_shift, r0 = WIDE ? blockIdx.y : (blockIdx.y * 4 + wave) * MERGE_ROWS;
+    if (WIDE && r0 >= rows) return;  // (the whole workgroup)
+    for (uint32_t r = r0; r < (WIDE ? r0 + 1 : min(r0 + MERGE_ROWS, rows)); r++) {
         const size_t stride = size_t(a.cache.kv_heads) * TILE, slot = (size_t(item.slot) * a.cache.kv_heads + kv) * TILE + r;
         const uint32_t row = item.row0 + (r >> a.group_shift);
         const uint32_t head = kv * a.group + (r & (a.group - 1)), dim = lane * 4;
@@ -1008,7 +1013,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, const Item
 
         float m = NO_MAXIMUM, l = 0.0f;
         floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (uint32_t p0 = FEW ? wave : 0; p0 < item.parts; p0 += BY * AT_ONCE) {
+        for (uint32_t p0 = WIDE ? wave : 0; p0 < item.parts; p0 += BY * AT_ONCE) {
             float2 ml[AT_ONCE];
             floatx4 x[AT_ONCE];
 #pragma unroll
@@ -1033,7 +1038,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, const Item
                 for (int j = 0; j < 4; j++) o[j] = fmaf(x[i][j], f, o[j]);
             }
         }
-        if constexpr (FEW) {
+        if constexpr (WIDE) {
             __shared__ __attribute__((aligned(16))) float part[4][64][4];
             __shared__ float pml[4][2];
             *reinterpret_cast<floatx4 *>(part[wave][lane]) = o;
@@ -1090,17 +1095,19 @@ uint32_t shift_of(uint32_t n) { return uint32_t(__builtin_ctz(n)); }
 template <int TYPE>
 void launch_attn(hipStream_t stream, const AttnArgs &a, const Shape &s, const saetta_paged_attn_params &p, const Item *tiles) {
     const dim3 grid(s.most_items * p.kv_heads);
+    auto merge_wide = [&](auto merge) { launch(merge, dim3(s.most_joined, s.columns ? p.rows * s.group : CHUNK_ROWS, p.kv_heads), dim3(256), 0, stream, a, tiles); };
     auto few = [&](auto attention, auto merge) {
         launch(attention, grid, dim3(few_threads(int(s.columns))), 0, stream, a);
-        launch(merge, dim3(s.most_joined, p.rows * s.group, p.kv_heads), dim3(256), 0, stream, a, tiles);
+        merge_wide(merge);
     };
     switch (s.columns) {
-        case 1: return few(paged_few_kernel<TYPE, 1>, paged_merge_kernel<TYPE, 1>);
-        case 2: return few(paged_few_kernel<TYPE, 2>, paged_merge_kernel<TYPE, 2>);
-        case 4: return few(paged_few_kernel<TYPE, 4>, paged_merge_kernel<TYPE, 4>);
+        case 1: return few(paged_few_kernel<TYPE, 1>, paged_merge_kernel<TYPE, FEW_ROWS, true>);
+        case 2: return few(paged_few_kernel<TYPE, 2>, paged_merge_kernel<TYPE, 2 * FEW_ROWS, true>);
+        case 4: return few(paged_few_kernel<TYPE, 4>, paged_merge_kernel<TYPE, 4 * FEW_ROWS, true>);
     }
     launch(paged_chunk_kernel<TYPE>, grid, dim3(64 * CHUNK_WAVES), CHUNK_LDS, stream, a);
-    launch(paged_merge_kernel<TYPE, 0>, dim3(s.most_joined, CHUNK_ROWS / 4 / MERGE_ROWS, p.kv_heads), dim3(256), 0, stream, a, tiles);
+    if (s.most_joined <= WIDE_TILES) merge_wide(paged_merge_kernel<TYPE, CHUNK_ROWS, true>);
+    else launch(paged_merge_kernel<TYPE, CHUNK_ROWS, false>, dim3(s.most_joined, CHUNK_ROWS / 4 / MERGE_ROWS, p.kv_heads), dim3(256), 0, stream, a, tiles);
 }
 
 }  // namespace
@@ -1140,7 +1147,7 @@ extern "C" int saetta_paged_split(saetta_stream_t stream, saetta_paged_batch bat
     const bool few = s.columns > 0;
     const SplitArgs a = {batch, reinterpret_cast<SplitHead *>(at), reinterpret_cast<Item *>(at + items_offset()), reinterpret_cast<Item *>(at + tiles_offset(s)),
                          s.tile_tokens, s.target, s.most_items, s.most_joined, s.slots, p.tokens, p.rows,
-                         few, few ? STEP_KEYS * FEW_WAVES : STEP_KEYS, few ? STEP_KEYS * FEW_WAVES : 256u, few ? 0u : CHUNK_EXTRA, few ? 0u : 4 * FEW_ROWS / s.group, few ? 0u : s.tile_tokens / 2};
+                         few, few ? STEP_KEYS * FEW_WAVES : STEP_KEYS, LEAST_KEYS, few ? 0u : CHUNK_EXTRA, few ? 0u : 4 * FEW_ROWS / s.group, few ? 0u : s.tile_tokens / 2};
     // (few tiles: four waves, whose barriers are cheaper)
     if (s.most_tiles <= 256) launch(paged_split_kernel<256>, dim3(1), dim3(256), 0, as_stream(stream), a);
     else launch(paged_split_kernel<1024>, dim3(1), dim3(1024), 0, as_stream(stream), a);

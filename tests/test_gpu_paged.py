@@ -348,6 +348,15 @@ def test_no_numbers_beside_a_chunk():
     assert np.isnan(got[:, 8:, 5]).sum() == 8 * (2 + 1 + 4 + 1) and not np.isnan(got[:, :8]).any()
 
 
+@pytest.mark.parametrize("new", [[20], [9, 40]])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_a_chunk_in_many_parts(new, dtype):
+    """One tile, and a few, whose keys are as many parts as the device has workgroups for."""
+    b = Batch(24, [5001, 1003][:len(new)], new, 64, 8, 1, dtype, room=1)
+    b.run()
+    b.compare()
+
+
 def test_scales_that_differ_widely():
     """Neighbouring blocks 2^20 apart, keys and values; a block of zeros."""
     for new in (1, 5):
