@@ -439,7 +439,7 @@ __device__ __forceinline__ void take_few(const AttnArgs &a, const Item &item, ui
     u32x4 k[2][4], v[2][4];  // codes of a step: [unit][64 dims]
     // (One team's codes are read once, and between two steps of a model its weights go through the caches: marked as such, what is read keeps no
     // place there.  64 requests of 8000 tokens 93.4 -> 82.3 us, 48 ragged 63 -> 55, 16 of 2000 the same; where the last call left the codes in the caches
-    // 41.8 -> 43.1, where 48 requests share all their 8000 tokens 30.6 -> 37.8.)
+    // 41.8 -> 43.1, one of 517 6.3 -> 7.3, where 48 requests share all their 8000 tokens 30.6 -> 37.8.)
     auto fetch = [&](const uint8_t *codes, uint32_t step, u32x4 (&x)[2][4]) {
 #pragma unroll
         for (int i = 0; i < 2; i++) {
