@@ -19,122 +19,212 @@
 namespace saetta {
 namespace {
 
-constexpr int STORE_THREADS = 256;
-// Up to this many tokens a workgroup looks at one, so that a step of single tokens is stored at once; more, where runs are long as a rule, by 16.
-constexpr uint32_t STORE_ALONE = 1024;
+// Waves of a workgroup of the store: four to a unit of tokens, of up to two units at once.
+constexpr uint32_t store_waves(int units) { return 4 * (units < 2 ? units : 2); }
+// A run of up to so many tokens is a wave's, so that a step of single tokens, or drafts, is stored at once.
+constexpr uint32_t SHORT_RUN = 4;
+// Tokens of a block, a lane a token.
+constexpr uint32_t lane_tokens(int units) { return units < 4 ? units * UNIT_TOKENS : 64; }
+// Workgroups (of all kv heads and sides) that look for runs, unless a block's tokens would be fewer than each looks at.
+constexpr uint32_t STORE_GROUPS = 512;
 
 struct StoreArgs {
     saetta_strided_rows x[2];  // keys, values
     const int32_t *slots;
     uint8_t *codes[2], *scales[2];
-    uint32_t blocks, block_tokens, kv_heads, tokens, span;
+    uint32_t blocks, block_tokens, kv_heads, tokens;
 };
 
 // Where the four dims (from `dim` on) of token t, of keys, or dim `dim` of the four tokens from t on, of values, lie in a unit: a dword.
 __device__ __forceinline__ uint32_t key_dword(uint32_t t, uint32_t dim) { return dim / 64 * 1024 + (dim / 16 % 4 * 16 + t) * 16 + dim % 16; }
 __device__ __forceinline__ uint32_t value_dword(uint32_t t, uint32_t dim) { return dim / 64 * 1024 + (t / 4 * 16 + dim % 16) * 16 + dim / 16 % 4 * 4; }
 
-template <int TYPE, int UNITS, bool KEYS>
-__device__ __forceinline__ void store_run(const StoreArgs &a, uint32_t token, uint32_t head, uint32_t block, uint32_t offset, uint32_t count) {
-    typedef typename Row<TYPE>::value V;
-    constexpr int which = KEYS ? 0 : 1;
-    const uint32_t tid = threadIdx.x, token0 = (tid >> 6) * 4, dim = (tid & 63) * 4;
-    const saetta_strided_rows &rows = a.x[which];
-    // the run's token 0 sits at `offset`; token t of the block is row t - offset of the run
-    const V *x = static_cast<const V *>(rows.data) + uint64_t(token) * rows.token_stride + head * rows.head_stride + dim;
-    const size_t at = size_t(block) * a.kv_heads + head;
-    uint8_t *scale = a.scales[which] + at;
-    const int before = int(*scale) - 127;
-    float held[UNITS][4][4];  // [unit][token][dim]
-    float top = 0.0f;
-#pragma unroll
-    for (int u = 0; u < UNITS; u++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t t = u * UNIT_TOKENS + token0 + i;
-#pragma unroll
-            for (int d = 0; d < 4; d++) held[u][i][d] = 0.0f;
-            if (t >= offset && t < offset + count) load_values<TYPE, 4>(x + uint64_t(t - offset) * rows.token_stride, held[u][i]);
-        }
-#pragma unroll
-    for (int u = 0; u < UNITS; u++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const float m = fabsf(held[u][i / 4][i % 4]);
-            top = m < __builtin_inff() ? fmaxf(top, m) : top;
-        }
-    top = group_reduce<64>(top, MaxOp());
-    __shared__ float tops[STORE_THREADS / 64];
-    __syncthreads();  // the last run's have been read
-    if ((tid & 63) == 0) tops[tid >> 6] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < STORE_THREADS / 64; w++) top = fmaxf(top, tops[w]);
-
-    int e = scale_exponent(top);
+// A run's place and scale.
+struct Run {
+    uint8_t *codes;  // of the block and kv head
+    uint32_t dim, offset, count;
+    bool raised;     // the codes before the run are to be moved to another scale
+    float down, moved;
+};
+template <bool KEYS>
+__device__ __forceinline__ Run run_of(const StoreArgs &a, size_t at, uint32_t dim, uint32_t offset, uint32_t count, float top, int before, int &e) {
+    e = scale_exponent(top);
     if (offset > 0) e = max(e, min(max(before, LOWEST_EXPONENT), HIGHEST_EXPONENT));
-    const bool raised = offset > 0 && e != before;
-    const float down = power_of_two(-e), moved = power_of_two(max(before - e, -126));
-    uint8_t *codes = a.codes[which] + at * (size_t(a.block_tokens) * SAETTA_HEAD_DIM);
+    return {a.codes[KEYS ? 0 : 1] + at * (size_t(a.block_tokens) * SAETTA_HEAD_DIM), dim, offset, count, offset > 0 && e != before,
+            power_of_two(-e), power_of_two(max(before - e, -126))};
+}
+// The lane's four dims of tokens t to t + 3 of the block, of which x holds those of the run.
+template <bool KEYS>
+__device__ __forceinline__ void put_tokens(const Run &r, uint32_t t, const float (&x)[4][4]) {
+    const uint32_t token0 = t % UNIT_TOKENS;
+    uint8_t *unit = r.codes + t / UNIT_TOKENS * UNIT_BYTES;
     auto rescaled = [&](uint32_t old) {
         float v[4];
         of_codes(old, v);
-        return to_codes(v[0] * moved, v[1] * moved, v[2] * moved, v[3] * moved);
+        return to_codes(v[0] * r.moved, v[1] * r.moved, v[2] * r.moved, v[3] * r.moved);
     };
+    const uint32_t end = r.offset + r.count;
+    // nothing of the four tokens is new, nor to be moved to another scale
+    if (t >= end || (t + 4 <= r.offset && !r.raised)) return;
+    if constexpr (KEYS) {
 #pragma unroll
-    for (int u = 0; u < UNITS; u++) {
-        const uint32_t t = u * UNIT_TOKENS + token0;
-        // nothing of the four tokens is new, nor to be moved to another scale
-        if (t >= offset + count || (t + 4 <= offset && !raised)) continue;
-        uint8_t *unit = codes + u * UNIT_BYTES;
-        if constexpr (KEYS) {
+        for (int i = 0; i < 4; i++) {
+            uint32_t *p = reinterpret_cast<uint32_t *>(unit + key_dword(token0 + i, r.dim));
+            if (t + i >= end || (t + i < r.offset && !r.raised)) continue;
+            *p = t + i >= r.offset ? to_codes(x[i][0] * r.down, x[i][1] * r.down, x[i][2] * r.down, x[i][3] * r.down) : rescaled(*p);
+        }
+    } else {
+        uint32_t fresh = 0, earlier = 0;  // bytes of tokens that are new; of tokens before them
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                uint32_t *p = reinterpret_cast<uint32_t *>(unit + key_dword(token0 + i, dim));
-                if (t + i >= offset + count || (t + i < offset && !raised)) continue;
-                *p = t + i >= offset ? to_codes(held[u][i][0] * down, held[u][i][1] * down, held[u][i][2] * down, held[u][i][3] * down) : rescaled(*p);
-            }
-        } else {
-            uint32_t fresh = 0, earlier = 0;  // bytes of tokens that are new; of tokens before them
+        for (int i = 0; i < 4; i++) {
+            if (t + i < r.offset) earlier |= 0xffu << (8 * i);
+            else if (t + i < end) fresh |= 0xffu << (8 * i);
+        }
+        uint32_t old[4] = {0, 0, 0, 0};
+        if (fresh != ~0u) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if (t + i < offset) earlier |= 0xffu << (8 * i);
-                else if (t + i < offset + count) fresh |= 0xffu << (8 * i);
-            }
+            for (int d = 0; d < 4; d++) old[d] = *reinterpret_cast<const uint32_t *>(unit + value_dword(token0, r.dim + d));
+        }
 #pragma unroll
-            for (int d = 0; d < 4; d++) {
-                uint32_t *p = reinterpret_cast<uint32_t *>(unit + value_dword(token0, dim + d));
-                uint32_t value = to_codes(held[u][0][d] * down, held[u][1][d] * down, held[u][2][d] * down, held[u][3][d] * down);
-                if (fresh != ~0u) {
-                    const uint32_t old = *p, kept = raised ? rescaled(old) : old;
-                    value = (value & fresh) | (kept & earlier) | (old & ~(fresh | earlier));
-                }
-                *p = value;
-            }
+        for (int d = 0; d < 4; d++) {
+            uint32_t value = to_codes(x[0][d] * r.down, x[1][d] * r.down, x[2][d] * r.down, x[3][d] * r.down);
+            if (fresh != ~0u) value = (value & fresh) | ((r.raised ? rescaled(old[d]) : old[d]) & earlier) | (old[d] & ~(fresh | earlier));
+            *reinterpret_cast<uint32_t *>(unit + value_dword(token0, r.dim + d)) = value;
         }
     }
+}
+__device__ __forceinline__ float largest(float top, const float (&x)[4]) {
+#pragma unroll
+    for (int d = 0; d < 4; d++) {
+        const float m = fabsf(x[d]);
+        top = m < __builtin_inff() ? fmaxf(top, m) : top;
+    }
+    return top;
+}
+template <int TYPE, bool KEYS>
+__device__ __forceinline__ const typename Row<TYPE>::value *row_of_run(const StoreArgs &a, uint32_t token, uint32_t head, uint32_t dim) {
+    const saetta_strided_rows &rows = a.x[KEYS ? 0 : 1];
+    return static_cast<const typename Row<TYPE>::value *>(rows.data) + uint64_t(token) * rows.token_stride + head * rows.head_stride + dim;
+}
+
+// A run by the whole workgroup: a wave has four tokens of a unit, or of UNITS / 4 units, a lane four dims.
+template <int TYPE, int UNITS, bool KEYS>
+__device__ __forceinline__ void store_run(const StoreArgs &a, uint32_t token, uint32_t head, uint32_t block, uint32_t offset, uint32_t count) {
+    constexpr uint32_t WAVES = store_waves(UNITS), AT_ONCE = WAVES / 4, EACH = UNITS / AT_ONCE;
+    constexpr int which = KEYS ? 0 : 1;
+    const uint32_t tid = threadIdx.x, wave = tid >> 6, dim = (tid & 63) * 4;
+    // the run's token 0 sits at `offset`; token t of the block is row t - offset of the run
+    const auto *x = row_of_run<TYPE, KEYS>(a, token, head, dim);
+    const size_t at = size_t(block) * a.kv_heads + head;
+    uint8_t *scale = a.scales[which] + at;
+    const int before = int(*scale) - 127;
+    auto first_of = [&](uint32_t u) { return (u * AT_ONCE + (wave >> 2)) * UNIT_TOKENS + (wave & 3) * 4; };
+    float held[EACH][4][4];  // [unit][token][dim]
+#pragma unroll
+    for (uint32_t u = 0; u < EACH; u++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t t = first_of(u) + i;
+#pragma unroll
+            for (int d = 0; d < 4; d++) held[u][i][d] = 0.0f;
+            if (t >= offset && t < offset + count) load_values<TYPE, 4>(x + uint64_t(t - offset) * a.x[which].token_stride, held[u][i]);
+        }
+    float top = 0.0f;
+#pragma unroll
+    for (uint32_t u = 0; u < EACH; u++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) top = largest(top, held[u][i]);
+    top = group_reduce<64>(top, MaxOp());
+    __shared__ float tops[WAVES];
+    __syncthreads();  // the last run's have been read
+    if ((tid & 63) == 0) tops[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = 0; w < WAVES; w++) top = fmaxf(top, tops[w]);
+    int e;
+    const Run run = run_of<KEYS>(a, at, dim, offset, count, top, before, e);
+#pragma unroll
+    for (uint32_t u = 0; u < EACH; u++) put_tokens<KEYS>(run, first_of(u), held[u]);
     if (tid == 0) *scale = uint8_t(e + 127);  // (everyone has read it: there was a barrier since)
 }
 
-// A workgroup looks at a.span tokens and takes the runs that begin there, one after the other.
+// A run of up to SHORT_RUN tokens by a wave.
+template <int TYPE, bool KEYS>
+__device__ __forceinline__ void store_short(const StoreArgs &a, uint32_t token, uint32_t head, uint32_t block, uint32_t offset, uint32_t count) {
+    static_assert(SHORT_RUN == 4, "the tokens of a dword of values");
+    constexpr int which = KEYS ? 0 : 1;
+    const uint32_t lane = threadIdx.x & 63, dim = lane * 4;
+    const auto *x = row_of_run<TYPE, KEYS>(a, token, head, dim);
+    const size_t at = size_t(block) * a.kv_heads + head;
+    uint8_t *scale = a.scales[which] + at;
+    const int before = int(*scale) - 127;
+    float held[SHORT_RUN][4], top = 0.0f;
+#pragma unroll
+    for (uint32_t j = 0; j < SHORT_RUN; j++) {
+#pragma unroll
+        for (int d = 0; d < 4; d++) held[j][d] = 0.0f;
+        if (j < count) load_values<TYPE, 4>(x + uint64_t(j) * a.x[which].token_stride, held[j]);
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < SHORT_RUN; j++) top = largest(top, held[j]);
+    top = group_reduce<64>(top, MaxOp());
+    int e;
+    const Run run = run_of<KEYS>(a, at, dim, offset, count, top, before, e);
+    for (uint32_t t = run.raised ? 0 : offset & ~3u; t < offset + count; t += 4) {
+        float y[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int d = 0; d < 4; d++) {
+                const uint32_t j = t + i - offset;
+                y[i][d] = j == 0 ? held[0][d] : j == 1 ? held[1][d] : j == 2 ? held[2][d] : held[3][d];
+            }
+        put_tokens<KEYS>(run, t, y);
+    }
+    if (lane == 0) *scale = uint8_t(e + 127);
+}
+
+// A workgroup looks at up to 64 tokens and takes the runs that begin there: the short ones a wave each, then the others one after the other.
 template <int TYPE, int UNITS>
-__global__ __launch_bounds__(STORE_THREADS) void paged_store_kernel(StoreArgs a) {
-    constexpr uint32_t BT = UNITS * UNIT_TOKENS;
-    const uint32_t head = blockIdx.y >> 1, lane = threadIdx.x & 63, first = blockIdx.x * a.span;
-    // Lane i: slot of token first + i; whether a run begins there: what is before it in the call is in another block, or not the slot before.
+__global__ __launch_bounds__(64 * store_waves(UNITS)) void paged_store_kernel(StoreArgs a) {
+    constexpr uint32_t BT = UNITS * UNIT_TOKENS, WAVES = store_waves(UNITS), TOKENS = lane_tokens(UNITS);
+    const uint32_t head = blockIdx.y >> 1, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // Lane i: slot of token token_of(i); whether a run begins there: what is before it in the call is in another block, or not the slot before;
+    // the tokens that follow it in the block, slot by slot, up to SHORT_RUN.
     // (Every wave by itself: no barrier.)
-    uint32_t slot = ~0u;
+    // The i-th token of TOKENS tokens is `step` workgroups further than the first: single tokens one behind the other are everyone's, and the blocks that a long
+    // run fills are neighbours'.  (All by a workgroup: 64 single tokens of a step with room for 2048 47 us; now 5.)
+    const uint32_t step = max(gridDim.x / TOKENS, 1u);
+    auto token_of = [&](uint32_t i) { return (blockIdx.x + TOKENS * gridDim.x - i * step) % gridDim.x * TOKENS + i; };
+    uint32_t slot = ~0u, follow = 0;
     bool begins = false;
-    if (lane < a.span && first + lane < a.tokens) {
-        const uint32_t t = first + lane;
+    const uint32_t t = token_of(lane);
+    if (lane < TOKENS && t < a.tokens) {
         slot = uint32_t(a.slots[t]);
         const uint32_t prior = t > 0 ? uint32_t(a.slots[t - 1]) : ~0u;
+        uint32_t next[SHORT_RUN];
+#pragma unroll
+        for (uint32_t j = 0; j < SHORT_RUN; j++) next[j] = uint32_t(a.slots[min(t + 1 + j, a.tokens - 1)]);
         begins = slot / BT < a.blocks && (slot % BT == 0 || t == 0 || prior != slot - 1);  // (-1 is in no block)
+        bool on = true;
+#pragma unroll
+        for (uint32_t j = 0; j < SHORT_RUN; j++) {
+            on = on && slot % BT + 1 + j < BT && t + 1 + j < a.tokens && next[j] == slot + 1 + j;
+            follow += on;
+        }
     }
-    for (uint64_t runs = __ballot(begins); runs; runs &= runs - 1) {
-        const uint32_t i = uint32_t(__builtin_ctzll(runs)), token = first + i, from = __builtin_amdgcn_readlane(slot, i);
+    const uint64_t all_runs = __ballot(begins), long_runs = __ballot(begins && follow >= SHORT_RUN);
+    uint32_t turn = 0;
+    for (uint64_t runs = all_runs & ~long_runs; runs; runs &= runs - 1, turn++) {
+        if (turn % WAVES != wave) continue;
+        const uint32_t i = uint32_t(__builtin_ctzll(runs)), token = token_of(i), from = __builtin_amdgcn_readlane(slot, i), count = 1 + __builtin_amdgcn_readlane(follow, i);
+        if (blockIdx.y & 1) store_short<TYPE, false>(a, token, head, from / BT, from % BT, count);
+        else store_short<TYPE, true>(a, token, head, from / BT, from % BT, count);
+    }
+    for (uint64_t runs = long_runs; runs; runs &= runs - 1) {
+        const uint32_t i = uint32_t(__builtin_ctzll(runs)), token = token_of(i), from = __builtin_amdgcn_readlane(slot, i);
         const uint32_t block = from / BT, offset = from % BT;
-        // the tokens that follow it in the block, slot by slot: up to 64 at a time
+        // the tokens that follow it in the block: up to 64 at a time
         uint32_t count = 1;
         for (uint32_t j0 = 1; j0 < BT - offset; j0 += 64) {
             const uint32_t j = j0 + lane;
@@ -203,14 +293,21 @@ __global__ __launch_bounds__(256) void paged_gather_kernel(GatherArgs a) {
     }
 }
 
+template <int TYPE, int UNITS>
+void launch_store(hipStream_t stream, const StoreArgs &a) {
+    const uint32_t sides = a.kv_heads * 2;
+    uint32_t groups = STORE_GROUPS / sides < a.tokens ? STORE_GROUPS / sides : a.tokens;
+    const uint32_t least = (a.tokens + lane_tokens(UNITS) - 1) / lane_tokens(UNITS);
+    if (groups < least) groups = least;
+    launch(paged_store_kernel<TYPE, UNITS>, dim3(groups, sides), dim3(64 * store_waves(UNITS)), 0, stream, a);
+}
 template <int TYPE>
 void launch_store(hipStream_t stream, const StoreArgs &a) {
-    const dim3 grid((a.tokens + a.span - 1) / a.span, a.kv_heads * 2);
     switch (a.block_tokens) {
-        case 16: return launch(paged_store_kernel<TYPE, 1>, grid, dim3(STORE_THREADS), 0, stream, a);
-        case 32: return launch(paged_store_kernel<TYPE, 2>, grid, dim3(STORE_THREADS), 0, stream, a);
-        case 64: return launch(paged_store_kernel<TYPE, 4>, grid, dim3(STORE_THREADS), 0, stream, a);
-        default: return launch(paged_store_kernel<TYPE, 8>, grid, dim3(STORE_THREADS), 0, stream, a);
+        case 16: return launch_store<TYPE, 1>(stream, a);
+        case 32: return launch_store<TYPE, 2>(stream, a);
+        case 64: return launch_store<TYPE, 4>(stream, a);
+        default: return launch_store<TYPE, 8>(stream, a);
     }
 }
 
@@ -233,7 +330,7 @@ extern "C" int saetta_paged_store(saetta_stream_t stream, int type, saetta_strid
     if (int rc = ensure_device()) return rc;
     if (tokens == 0) return SAETTA_OK;
     const StoreArgs a = {{keys, values}, slots, {cache.keys, cache.values}, {cache.key_scales, cache.value_scales},
-                         cache.blocks, cache.block_tokens, cache.kv_heads, tokens, tokens <= STORE_ALONE ? 1u : UNIT_TOKENS};
+                         cache.blocks, cache.block_tokens, cache.kv_heads, tokens};
     if (type == SAETTA_F32) launch_store<SAETTA_F32>(as_stream(stream), a);
     else if (type == SAETTA_F16) launch_store<SAETTA_F16>(as_stream(stream), a);
     else launch_store<SAETTA_BF16>(as_stream(stream), a);

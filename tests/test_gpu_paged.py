@@ -179,6 +179,30 @@ def test_store_of_many_short_runs():
         assert np.array_equal(got.e[w], want.e[w]) and np.array_equal(got.rows[w], want.rows[w])
 
 
+@pytest.mark.parametrize("block, kv_heads, room", [(16, 2, 2100), (32, 1, 700), (64, 2, 1300), (128, 3, 5000)])
+def test_store_of_steps_in_a_large_room(block, kv_heads, room):
+    """Steps of single tokens, drafts and a few long runs among many places without a slot; scales that rise at every step."""
+    gen = np.random.default_rng(block)
+    blocks = 40
+    cache, plain = saetta.PagedCache(kv_heads, DIM, blocks, block), Cache(kv_heads, blocks, block)
+    poison(cache, gen)
+    filled = np.zeros(blocks, int)
+    for step in range(5):
+        slots = []
+        for b in gen.permutation(blocks):
+            n = int(min(gen.choice([0, 1, 1, 2, 3, 4, 5, 6, block // 2]), block - filled[b]))
+            slots += [int(b) * block + int(filled[b]) + i for i in range(n)]
+            filled[b] += n
+            slots += [-1] * int(gen.integers(0, 3))
+        slots = (slots + [-1] * room)[:max(room, len(slots))]
+        k, v = (values_of(gen, len(slots), kv_heads, F16) * 2.0 ** step for _ in range(2))
+        cache.encode(k, v, ints(slots))
+        plain.store(numbers(k), numbers(v), slots)
+    there = [b * block + t for b in range(blocks) for t in range(int(filled[b]))]
+    for got, want in zip(Cache.of(cache).gather(there), plain.gather(there)):
+        assert np.array_equal(got, want)
+
+
 def test_store_of_no_numbers_and_the_range():
     """Not finite: NaN, and the others' scale is theirs.  Zero, the smallest, the largest, past the range."""
     cache = saetta.PagedCache(1, DIM, 2, 16)
