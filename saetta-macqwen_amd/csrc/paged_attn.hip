@@ -3,10 +3,11 @@
 // For row i of request r, at position p = kv_lens[r] - n + i, and q head h over kv head h / group:
 //     out = sum_t 2^(s_t) v_t / sum_t 2^(s_t) [* sigmoid(gate)],  s_t = log2(e) scale (q . k_t),  t = 0 .. p.
 // The cache holds codes a, b and exponents: k_t = 2^ek a_t, v_t = 2^ev b_t, one ek and ev per block and kv head.  With
-//     x_t = log2(e) scale 2^ek (q . a_t) + ev,   w_t = 2^(x_t - M),   M = max x_t so far,
+//     x_t = log2(e) scale 2^ek (q . a_t) + ev,   w_t = 2^(x_t - M),
 // out = sum w_t b_t / sum w_t 2^-ev: the values' scale is an addend of the score, the running maximum is that of what a
-// token can add to the output, and the matrix cores see codes alone, which f16 and bf16 hold exactly.  Only w_t is rounded (to
-// f16, half a step 2^-12 of it, as operand of the second product: the sums are f32).
+// token can add to the output, and the matrix cores see codes alone, which f16 and bf16 hold exactly.  M follows the running maximum of x_t, 7 to 15 below it, so
+// that the largest weight is 2^7 to 2^15.  Only w_t is rounded (to f16, as operand of the second product: by up to 2^-11 of it, or 2^-25 where it is below 2^-14, which is
+// 2^-32 of the largest at most; with M at the maximum 2^-25, and 131072 keys just below that were 0.4 % of a row); the sums are f32, that of the weights of unrounded ones.
 //
 // The three kernels: paged_split_kernel deals rows and keys out as items from the lengths; the attention kernel, one
 // workgroup to an item and kv head, paged_few_kernel for tiles of up to 64 rows and paged_chunk_kernel for tiles of
@@ -36,7 +37,8 @@ constexpr int DIM = SAETTA_HEAD_DIM;
 #include "prefill_stream.hpp"  // scores_block, stream_block_alone, settle
 constexpr float NO_SCORE = -__builtin_inff();    // of a key that a row does not see
 constexpr float NO_MAXIMUM = -1e30f;             // where nothing was seen: 2^(NO_SCORE - NO_MAXIMUM) is 0
-constexpr float TAU = 8.0f;                      // the reference maximum is raised only past this many powers of two
+constexpr float TAU = 8.0f;                      // M is raised only when the maximum has risen by this many powers of two
+constexpr float TOP = 7.0f;                      // the maximum less M as M is raised: with TAU the largest weight is 2^15, in f16's range
 constexpr uint32_t STEP_KEYS = 32;               // keys of a step: two units
 constexpr uint32_t FEW_ROWS = 16, CHUNK_ROWS = 256;  // FEW_ROWS: of a group of columns; a tile of few rows has 1, 2 or 4 groups
 constexpr int FEW_WAVES = 4, CHUNK_WAVES = 8;
@@ -555,8 +557,8 @@ __device__ __forceinline__ void take_few(const AttnArgs &a, const Item &item, ui
 #pragma unroll
                 for (int i = 0; i < 2; i++) top = fmaxf(top, fmaf(fmaxf(fmaxf(s[g][i][0], s[g][i][1]), fmaxf(s[g][i][2], s[g][i][3])), ck[i], float(ev[i])));
                 top = across_rows<16, 64>(top, MaxOp());
-                if (__any(top > m[g] + TAU)) {
-                    const float next = top > m[g] + TAU ? top : m[g], down = __builtin_amdgcn_exp2f(m[g] - next);
+                if (__any(top > m[g] + (TOP + TAU))) {
+                    const float next = top > m[g] + (TOP + TAU) ? top - TOP : m[g], down = __builtin_amdgcn_exp2f(m[g] - next);
                     m[g] = next, l[g] *= down;
 #pragma unroll
                     for (int i = 0; i < 16; i++) acc[g][i] *= down;
@@ -799,8 +801,8 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
 #pragma unroll
         for (int r = 0; r < 16; r++) tops[r >> 3] = fmaxf(tops[r >> 3], s[r]);
         const float top = across_rows<32, 64>(fmaxf(fmaf(tops[0], ck[0], float(ev[0])), fmaf(tops[1], ck[1], float(ev[1]))), MaxOp());
-        if (__any(top > m + TAU)) {
-            const float next = top > m + TAU ? top : m, down = __builtin_amdgcn_exp2f(m - next);
+        if (__any(top > m + (TOP + TAU))) {
+            const float next = top > m + (TOP + TAU) ? top - TOP : m, down = __builtin_amdgcn_exp2f(m - next);
             m = next, l *= down;
 #pragma unroll
             for (int i = 0; i < 8; i++) acc[i] *= down;
