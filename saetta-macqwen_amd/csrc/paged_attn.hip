@@ -2,12 +2,16 @@
 //
 // For row i of request r, at position p = kv_lens[r] - n + i, and q head h over kv head h / group:
 //     out = sum_t 2^(s_t) v_t / sum_t 2^(s_t) [* sigmoid(gate)],  s_t = log2(e) scale (q . k_t),  t = 0 .. p.
-// The cache holds codes a, b and exponents: k_t = 2^ek a_t, v_t = 2^ev b_t, one ek and ev per block and kv head.  With
-//     x_t = log2(e) scale 2^ek (q . a_t) + ev,   w_t = 2^(x_t - M),
-// out = sum w_t b_t / sum w_t 2^-ev: the values' scale is an addend of the score, the running maximum is that of what a
-// token can add to the output, and the matrix cores see codes alone, which f16 and bf16 hold exactly.  M follows the running maximum of x_t, 7 to 15 below it, so
-// that the largest weight is 2^7 to 2^15.  Only w_t is rounded (to f16, as operand of the second product: by up to 2^-11 of it, or 2^-25 where it is below 2^-14, which is
-// 2^-32 of the largest at most; with M at the maximum 2^-25, and 131072 keys just below that were 0.4 % of a row); the sums are f32, that of the weights of unrounded ones.
+// The cache holds codes a, b and exponents: k_t = 2^ek a_t, v_t = 2^ev b_t, one ek and ev per block and kv head.  With ev = held + rest, held
+// of -15..7,
+//     x_t = log2(e) scale 2^ek (q . a_t) + rest,   w_t = 2^(x_t - M),
+// out = sum w_t (2^held b_t) / sum w_t 2^-rest.  The matrix cores see codes of keys, which f16 and bf16 hold exactly, and codes of values times 2^held, which
+// f16 holds exactly too (from 2^-9 * 2^-15, its least number, to 448 * 2^7): where a block's largest value is 0.014 to 57344 the weights are
+// the softmax's own, and only past that is what is left of the exponent an addend of the score.  (All of it as an addend, a block that is loud in one dim
+// took the weights of blocks 2^34 quieter out of f16's range in every dim.)
+// M follows the running maximum, 7 to 15 below it, so that the largest weight is 2^7 to 2^15.  Only w_t is rounded (to f16, as operand of the second product:
+// by up to 2^-11 of it, or 2^-25 where it is below 2^-14, which is 2^-32 of the largest at most; with M at the maximum 2^-25, and 131072 keys just below that were
+// 0.4 % of a row); the sums are f32, that of the weights of unrounded ones.
 //
 // The three kernels: paged_split_kernel deals rows and keys out as items from the lengths; the attention kernel, one
 // workgroup to an item and kv head, paged_few_kernel for tiles of up to 64 rows and paged_chunk_kernel for tiles of
@@ -39,6 +43,7 @@ constexpr float NO_SCORE = -__builtin_inff();    // of a key that a row does not
 constexpr float NO_MAXIMUM = -1e30f;             // where nothing was seen: 2^(NO_SCORE - NO_MAXIMUM) is 0
 constexpr float TAU = 8.0f;                      // M is raised only when the maximum has risen by this many powers of two
 constexpr float TOP = 7.0f;                      // the maximum less M as M is raised: with TAU the largest weight is 2^15, in f16's range
+constexpr int LOWEST_HELD = -15, HIGHEST_HELD = 7;  // of a values' exponent, what their conversion to f16 takes
 constexpr uint32_t STEP_KEYS = 32;               // keys of a step: two units
 constexpr uint32_t FEW_ROWS = 16, CHUNK_ROWS = 256;  // FEW_ROWS: of a group of columns; a tile of few rows has 1, 2 or 4 groups
 constexpr int FEW_WAVES = 4, CHUNK_WAVES = 8;
@@ -295,14 +300,14 @@ struct AttnArgs {
     float scale;
 };
 
-// Codes of one dword as four halves.
-__device__ __forceinline__ u32x2 halves_of(uint32_t w) {
-    const half2_ a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true);
+// Codes of one dword as four halves, times a power of two.
+__device__ __forceinline__ u32x2 halves_of(uint32_t w, float scale) {
+    const half2_ a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, true);
     return u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
 }
 template <int TYPE>
 __device__ __forceinline__ u32x2 operands_of(uint32_t w) {
-    if constexpr (TYPE == SAETTA_F16) return halves_of(w);
+    if constexpr (TYPE == SAETTA_F16) return halves_of(w, 1.0f);
     const brain2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true);
     return u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
 }
@@ -347,7 +352,14 @@ __device__ __forceinline__ uint32_t find_scales(const AttnArgs &a, const Unit &u
 }
 // (exponents as the store writes them: what else a byte says would make scores no numbers)
 __device__ __forceinline__ float key_scale(uint32_t scales) { return power_of_two(min(max(int(scales & 0xff) - 127, LOWEST_EXPONENT), HIGHEST_EXPONENT)); }
-__device__ __forceinline__ int value_exponent(uint32_t scales) { return min(max(int(scales >> 8 & 0xff) - 127, LOWEST_EXPONENT), HIGHEST_EXPONENT); }
+// ev of a unit's values, in two: what their conversion takes, and the rest, the score's.
+struct ValueExponent {
+    int held, rest;
+};
+__device__ __forceinline__ ValueExponent value_exponent(uint32_t scales) {
+    const int e = min(max(int(scales >> 8 & 0xff) - 127, LOWEST_EXPONENT), HIGHEST_EXPONENT), held = min(max(e, LOWEST_HELD), HIGHEST_HELD);
+    return {held, e - held};
+}
 
 // An item that the split has made for these buffers.  (A split of other parameters is not followed out of them.)  (No branches: the
 // loads go out together.)
@@ -523,8 +535,9 @@ __device__ __forceinline__ void take_few(const AttnArgs &a, const Item &item, ui
             }
             if (step + 1 < here) fetch(a.cache.keys, step + 1, k);
             const uint32_t scale[2] = {uint32_t(__builtin_amdgcn_readlane(scales, 2 * step)), uint32_t(__builtin_amdgcn_readlane(scales, 2 * step + 1))};
-            const int ev[2] = {value_exponent(scale[0]), value_exponent(scale[1])};
-            const float ck[2] = {c * key_scale(scale[0]), c * key_scale(scale[1])};
+            const ValueExponent exponents[2] = {value_exponent(scale[0]), value_exponent(scale[1])};
+            const int ev[2] = {exponents[0].rest, exponents[1].rest};
+            const float ck[2] = {c * key_scale(scale[0]), c * key_scale(scale[1])}, held[2] = {power_of_two(exponents[0].held), power_of_two(exponents[1].held)};
             const bool masked = key + STEP_KEYS > min(all_see, item.key1) || !(scale[0] & scale[1] & 0x10000);
             // (what follows from the lane is worked out where it is used: kept over the loop it would be in registers that the sums want)
             uint32_t at = lane;
@@ -575,7 +588,7 @@ __device__ __forceinline__ void take_few(const AttnArgs &a, const Item &item, ui
             for (int j = 0; j < 4; j++)
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
-                    const u32x2 v0 = halves_of(v[0][j][t]), v1 = halves_of(v[1][j][t]);
+                    const u32x2 v0 = halves_of(v[0][j][t], held[0]), v1 = halves_of(v[1][j][t], held[1]);
 #pragma unroll
                     for (int g = 0; g < COLUMNS; g++) acc[g][4 * j + t] = product16<SAETTA_F16>(u32x4{v0.x, v0.y, v1.x, v1.y}, w[g], acc[g][4 * j + t]);
                 }
@@ -770,7 +783,9 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
     auto make_values = [&](u32x4 x, uint32_t step) {  // tokens 4 quarter .. + 3 of dims 16 (4 part + i) + t
         const uint32_t at = here(), t = at & 15, quarter = at >> 4;
         const uint32_t key = (unit0 + 2 * step + mine) * UNIT_TOKENS;
-        const bool there = __builtin_amdgcn_readlane(scales, (2 * step + mine) % 64) & 0x10000;
+        const uint32_t scale = __builtin_amdgcn_readlane(scales, (2 * step + mine) % 64);
+        const bool there = scale & 0x10000;
+        const float held = power_of_two(value_exponent(scale).held);
         if (key + UNIT_TOKENS > min(all_see, item.key1) || !there) {
 #pragma unroll
             for (int i = 0; i < 4; i++) x[i] = clean_values(x[i], key + 4 * quarter, there ? item.key1 : 0, all_see, (4 * part + i) * 16 + t, nan_from);
@@ -779,7 +794,7 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const uint32_t dim = (4 * part + i) * 16 + t;
-            *reinterpret_cast<u32x2 *>(to + 2 * (dim >> 5) * 1024 + (dim & 31) * 16) = halves_of(x[i]);
+            *reinterpret_cast<u32x2 *>(to + 2 * (dim >> 5) * 1024 + (dim & 31) * 16) = halves_of(x[i], held);
         }
     };
     // Probabilities of a step from its scores, as operands.
@@ -789,7 +804,7 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
         float ck[2], sum[2] = {0.0f, 0.0f}, tops[2] = {NO_SCORE, NO_SCORE};
         int ev[2];
 #pragma unroll
-        for (int i = 0; i < 2; i++) ck[i] = c * key_scale(scale[i]), ev[i] = value_exponent(scale[i]);
+        for (int i = 0; i < 2; i++) ck[i] = c * key_scale(scale[i]), ev[i] = value_exponent(scale[i]).rest;
         if (key + STEP_KEYS > wave_all || !(scale[0] & scale[1] & 0x10000)) {
             // keys of the step that the row sees, less the lane half's four; none of a unit that is not there
             const int n = min(sees, int(item.key1)) - int(key) - 4 * int(here() >> 5);

@@ -1,13 +1,66 @@
-"""The weights of the attention over paged caches where f16 holds them least well: a great many small ones beside a large one."""
+"""The weights of the attention over paged caches where f16 holds them least well: a great many small ones beside a large one, values of every
+exponent that a block can have, and blocks whose exponents lie far apart.  Against the formula in 64 bits over what the cache holds."""
 import numpy as np
 import pytest
 import torch
 
-from gpu_common import saetta
-from paged_common import DIM
-from test_gpu_paged import F16, ints, numbers
+from gpu_common import host, saetta
+from paged_common import DIM, Cache
+from test_gpu_paged import BF16, F16, F32, HALF_STEP, ints, numbers
 
 pytestmark = pytest.mark.gpu
+
+
+class One:
+    """One request of one kv head, its blocks in order: keys and values [tokens, 256], queries [new, heads, 256]."""
+
+    def __init__(self, keys, values, queries, dtype, block=16, kv_heads=1):
+        tokens, new, heads = len(keys), len(queries), queries.shape[1]
+        blocks = -(-tokens // block)
+        self.cache = saetta.PagedCache(kv_heads, DIM, blocks, block)
+        self.tables = t = saetta.PagedTables(1, new, blocks, blocks, block)
+        t.block_table[0] = ints(range(blocks))
+        t.kv_lens.fill_(tokens), t.query_starts.copy_(ints([0, new]))
+        k, v = (torch.tensor(x, dtype=F32, device="cuda")[:, None].expand(tokens, kv_heads, DIM) for x in (keys, values))
+        self.cache.encode(k, v, ints(range(tokens)))
+        self.q = torch.tensor(queries, dtype=dtype, device="cuda")
+        self.out = torch.zeros(new, heads, DIM, dtype=dtype, device="cuda")
+        self.attention = saetta.PagedAttention(heads, kv_heads, DIM, t, rows=new)
+
+    def run(self):
+        self.attention.encode_split(self.tables)
+        self.attention.encode(self.q, self.cache, self.tables, self.out)
+
+    def compare(self, rows=(0, -1)):
+        """The first head of every kv head, of the rows given.  A weight w = p 2^rest, in units of its largest W in the row, is rounded to f16 by 2^-11 of it or
+        2^-32 of W; a score is off as `attend` has it, by (256 + 4) 2^-24 sum |q k| / 16 and 4 2^-24 of itself, in numerator and denominator; sums
+        of n keys by (n / 16 + 32) 2^-24, 2^-23 for both; then the output's own half step (and half of its least step)."""
+        c, q, got = Cache.of(self.cache), numbers(self.q), numbers(self.out)
+        group, half = q.shape[1] // c.kv_heads, HALF_STEP[self.out.dtype]
+        least = 2.0 ** -25 if self.out.dtype is F16 else 2.0 ** -134
+        for i in rows:
+            seen = int(self.tables.kv_lens[0]) - len(q) + 1 + i % len(q)
+            at = np.arange(seen)
+            block, t = host(self.tables.block_table)[0][at // c.block_tokens], at % c.block_tokens
+            for h in range(c.kv_heads):
+                k, v = c.rows["keys"][block, h, t], c.rows["values"][block, h, t]
+                s = k @ q[i, h * group] / 16.0
+                p = np.exp(s - s.max())
+                p /= p.sum()
+                e = c.e["values"][block, h].astype(float)
+                rest = e - np.clip(e, -15, 7)
+                w = p * np.exp2(rest - rest.max())  # (times 2^rest.max())
+                small = (2.0 ** -32 * w.max() * np.exp2(rest.max() - rest)) @ np.abs(v)
+                spread = np.abs(k) @ np.abs(q[i, h * group]) / 16.0
+                rel = 2.0 ** -11 + 2.0 ** -23 * (264 * spread.max() + 4 * np.abs(s).max() + seen / 16 + 32)
+                want = p @ v
+                bound = rel * (p @ np.abs(v)) + small
+                off = np.abs(got[i, h * group] - want) - (bound * (1 + half) + half * np.abs(want) + least)
+                assert off.max() <= 0, (i, h, off.max(), int(off.argmax()), got[i, h * group][off.argmax()], want[off.argmax()], bound[off.argmax()])
+
+
+# rows of a tile: a token; two, three and five tokens of 8 q heads; a chunk, whose last row is compared (and its first)
+ROWS = [1, 2, 3, 5, 40]
 
 
 @pytest.mark.parametrize("new", [1, 3, 5, 9])
@@ -40,3 +93,32 @@ def test_many_small_weights_behind_a_large_one(new):
         sums = n / 16 + n / 32 if new * 8 > 64 else n / 128 + n / 128
         bound = 2.0 ** -11 + others * 2.0 ** -32 + 2.0 ** -24 * (sums + 64) + 2.0 ** -23 * 16 * 18
         assert np.abs(got[:, i] - want).max() <= bound + 2.0 ** -11, (i, np.abs(got[:, i] - want).max(), bound)
+
+
+@pytest.mark.parametrize("new", ROWS)
+@pytest.mark.parametrize("loud", [-45, -38, -26, -23, -22, -15, -8, 0, 7, 8, 20, 50])
+def test_values_of_every_exponent(new, loud):
+    """Values of sizes over all that e4m3 holds, subnormals too, at loudnesses on both sides of what the conversion to f16 takes of an exponent."""
+    gen = np.random.default_rng(new + 100)
+    keys, queries = gen.standard_normal((300, DIM)), gen.standard_normal((new, 8, DIM))
+    values = gen.standard_normal((300, DIM)) * np.exp2(gen.uniform(-16, 0, (300, DIM))) * 2.0 ** loud
+    b = One(keys, values, queries, BF16)
+    b.run()
+    b.compare()
+
+
+@pytest.mark.parametrize("new", ROWS)
+@pytest.mark.parametrize("gap", [16, 24, 28, 34, 39])
+@pytest.mark.parametrize("first", [False, True])
+def test_a_loud_dim_in_one_block(new, gap, first):
+    """One value of 1 in a block, all others 2^-gap, and 8.7 powers of two of score in favour of the quiet blocks: they are the output of every other dim."""
+    gen = np.random.default_rng(gap)
+    keys, values = np.zeros((128, DIM)), gen.uniform(0.5, 1.0, (128, DIM)) * 2.0 ** -gap
+    at = 3 if first else 100
+    quiet = np.arange(128) // 16 != at // 16
+    keys[quiet, 0], values[at, 9] = 6.0, 1.0  # exp(6) is 2^8.66
+    queries = np.zeros((new, 8, DIM))
+    queries[..., 0] = 16.0
+    b = One(keys, values, queries, BF16)
+    b.run()
+    b.compare()
