@@ -658,7 +658,8 @@ int saetta_paged_split(saetta_stream_t stream, saetta_paged_batch batch, saetta_
  * own.  q, gate and out are f16 or bf16 (type) rows of p.heads heads; gate.data NULL: no gate.  out may be q.  Rows past the step's last token,
  * and tokens of a request past p.rows where p.rows is for few rows, are left as they were; a row that sees nothing (its position is
  * below 0, or its blocks are not there) becomes zeros.  A score (times log2 e) below -1e30 counts as not seen.  A weight of
- * a row's softmax is off by up to 2^-11 of it, or by 2^-32 of the row's largest where that is more.  This is so where the e of the values' blocks are -15..7 (largest
+ * a row's softmax is off by up to 2^-11 of it (2^-22 where a request has up to 16 rows, new tokens times q heads per kv head), or by 2^-32 of the row's largest where
+ * that is more.  This is so where the e of the values' blocks are -15..7 (largest
  * values of 0.014 to 57344); a block's weights count 2^(e - 7) times as much in it where e is larger, 2^(e + 15) times where e is smaller: beside a block of values
  * around 2^39 the weights of ordinary ones are off by 2^-8 of the largest.  split: made by saetta_paged_split with the same batch and p.
  * workspace: 16-byte aligned, of saetta_paged_workspace_bytes, the call's own until its kernels have run; calls that may

@@ -11,7 +11,7 @@
 // took the weights of blocks 2^34 quieter out of f16's range in every dim.)
 // M follows the running maximum, 7 to 15 below it, so that the largest weight is 2^7 to 2^15.  Only w_t is rounded (to f16, as operand of the second product:
 // by up to 2^-11 of it, or 2^-25 where it is below 2^-14, which is 2^-32 of the largest at most; with M at the maximum 2^-25, and 131072 keys just below that were
-// 0.4 % of a row); the sums are f32, that of the weights of unrounded ones.
+// 0.4 % of a row.  Tiles of up to 16 rows add what was rounded off); the sums are f32, that of the weights of unrounded ones.
 //
 // The three kernels: paged_split_kernel deals rows and keys out as items from the lengths; the attention kernel, one
 // workgroup to an item and kv head, paged_few_kernel for tiles of up to 64 rows and paged_chunk_kernel for tiles of
@@ -426,6 +426,10 @@ template <int TYPE, int COLUMNS, int TEAMS, int TURNS, uint32_t TILE>
 __device__ __forceinline__ void take_few(const AttnArgs &a, const Item &item, uint32_t kv, FewShared<COLUMNS, TEAMS, TURNS> &shared, uint32_t *nan_from) {
     typedef typename Row<TYPE>::value V;
     constexpr int TILE_COLUMNS = COLUMNS * TEAMS;
+    // A wave with one group multiplies what is rounded off its weights too, as another f16 (2^-22 of a weight, or 2^-32 of the largest, is left): the matrix cores are idle
+    // there for most of the time.  8 requests at 131072 171.8 -> 172.7 us with split and merge, four layers of 48 ragged 244 -> 246, of 64 requests of two tokens at 4000
+    // 213 -> 215.  With two groups it would be 223 -> 236 for three tokens, with four 333 -> 349 for five.
+    constexpr bool BOTH_HALVES = COLUMNS == 1;
     constexpr uint32_t WAVES = TEAMS * TURNS;
     auto &sums = shared.sums;
     auto &ml = shared.ml;
@@ -552,7 +556,7 @@ __device__ __forceinline__ void take_few(const AttnArgs &a, const Item &item, ui
                         for (int t = 0; t < 4; t++) v[i][j][t] = clean_values(v[i][j][t], from, limit, all_see, (4 * j + t) * 16 + (at & 15), nan_from);
                 }
             }
-            u32x4 w[COLUMNS];
+            u32x4 w[COLUMNS], below[BOTH_HALVES ? COLUMNS : 1];
 #pragma unroll
             for (int g = 0; g < COLUMNS; g++) {
                 if (masked) {
@@ -583,6 +587,14 @@ __device__ __forceinline__ void take_few(const AttnArgs &a, const Item &item, ui
                     for (int r = 0; r < 4; r++) p[i][r] = __builtin_amdgcn_exp2f(fmaf(s[g][i][r], ck[i], float(ev[i]) - m[g])), part[i] += p[i][r];
                 l[g] = fmaf(part[0], power_of_two(-ev[0]), fmaf(part[1], power_of_two(-ev[1]), l[g]));
                 w[g] = u32x4{pack_half2(p[0][0], p[0][1]), pack_half2(p[0][2], p[0][3]), pack_half2(p[1][0], p[1][1]), pack_half2(p[1][2], p[1][3])};
+                if constexpr (BOTH_HALVES) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t both = w[g][i];
+                        const half2_ high = __builtin_bit_cast(half2_, both);
+                        below[g][i] = pack_half2(p[i >> 1][i % 2 * 2] - float(high.x), p[i >> 1][i % 2 * 2 + 1] - float(high.y));
+                    }
+                }
             }
 #pragma unroll
             for (int j = 0; j < 4; j++)
@@ -591,6 +603,10 @@ __device__ __forceinline__ void take_few(const AttnArgs &a, const Item &item, ui
                     const u32x2 v0 = halves_of(v[0][j][t], held[0]), v1 = halves_of(v[1][j][t], held[1]);
 #pragma unroll
                     for (int g = 0; g < COLUMNS; g++) acc[g][4 * j + t] = product16<SAETTA_F16>(u32x4{v0.x, v0.y, v1.x, v1.y}, w[g], acc[g][4 * j + t]);
+                    if constexpr (BOTH_HALVES) {
+#pragma unroll
+                        for (int g = 0; g < COLUMNS; g++) acc[g][4 * j + t] = product16<SAETTA_F16>(u32x4{v0.x, v0.y, v1.x, v1.y}, below[g], acc[g][4 * j + t]);
+                    }
                 }
             if (step + 1 < here) fetch(a.cache.values, step + 1, v);
         }

@@ -122,3 +122,37 @@ def test_a_loud_dim_in_one_block(new, gap, first):
     b = One(keys, values, queries, BF16)
     b.run()
     b.compare()
+
+
+@pytest.mark.parametrize("new, rows_of", [(1, 8), (2, 8), (1, 16), (16, 1)])
+@pytest.mark.parametrize("beside", [False, True])
+def test_weights_of_up_to_16_rows_keep_22_bits(new, rows_of, beside):
+    """Three keys whose values nearly cancel in some dims: a weight off by 2^-12 of it would be seen there, 2^-22 is not.  By themselves and beside a chunk.  Scores are
+    single products; the exponential is off by 2^-23 of it, and so are the few sums."""
+    gen = np.random.default_rng(new * rows_of)
+    keys = np.zeros((2 + new, DIM))
+    keys[:3, 0] = [1.0, 0.875, 0.75]
+    values = gen.uniform(0.25, 1.0, (2 + new, DIM)) * gen.choice([-1.0, 1.0], (2 + new, DIM))
+    queries = np.zeros((new, rows_of, DIM))
+    queries[..., 0] = gen.uniform(2, 30, (new, rows_of))
+    b = One(keys, values, queries, F16)
+    if beside:  # another request, of no keys that count, whose tokens are a chunk's
+        t = saetta.PagedTables(2, new + 130, b.tables.max_blocks, b.cache.blocks, 16)
+        t.block_table[0] = b.tables.block_table[0]
+        t.kv_lens.copy_(ints([2 + new, 130])), t.query_starts.copy_(ints([0, new, new + 130]))
+        b.tables, q = t, b.q
+        b.q = torch.cat([q, torch.ones(130, rows_of, DIM, dtype=F16, device="cuda")])
+        b.out = torch.zeros_like(b.q)
+        b.attention = saetta.PagedAttention(rows_of, 1, DIM, t, rows=130)
+    b.run()
+    c, q, got = Cache.of(b.cache), numbers(b.q), numbers(b.out)
+    for i in range(new):
+        k, v = (c.rows[w][:, 0].reshape(-1, DIM)[:3 + i] for w in ("keys", "values"))
+        for h in range(rows_of):
+            s = k @ q[i, h] / 16.0
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            want, size = p @ v, p @ np.abs(v)
+            rel = 2.0 ** -22 + 2.0 ** -23 * (4 + 8 * np.abs(s).max() + len(s))
+            off = np.abs(got[i, h] - want) - (rel * size * (1 + 2.0 ** -11) + 2.0 ** -11 * np.abs(want) + 2.0 ** -25)
+            assert off.max() <= 0, (i, h, off.max(), int(off.argmax()))
