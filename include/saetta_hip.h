@@ -596,7 +596,10 @@ typedef struct saetta_paged_tables_params {
  * block * block_tokens + position % block_tokens, or -1 where it has no block.  Past the last token slots and positions
  * are -1.  New tokens past the room are no part of the step: lengths, blocks and query_starts count those before it.  *unplaced: the
  * new tokens without a slot, those among them.  kv_lens may be context_lens itself: then the call, replayed, goes on by the step's
- * tokens each time.  requests * max_blocks is less than 2^31. */
+ * tokens each time.  A token that has room but no block is a part of the step and counted in kv_lens, and lies nowhere: it is to come again when
+ * there are blocks.  Where kv_lens is context_lens the next call leaves it out by itself (a context is at most held * block_tokens); lengths of the caller's own must do so,
+ * or the request gets a block in which nobody has stored those tokens, and its attention sees what was left there.
+ * requests * max_blocks is less than 2^31. */
 int saetta_paged_tables(saetta_stream_t stream, const uint32_t *context_lens, const uint32_t *new_lens,
                         saetta_paged_state state, saetta_paged_step step, saetta_paged_tables_params p);
 

@@ -75,6 +75,8 @@ __device__ __forceinline__ Lengths lengths_of(const TablesArgs &a, uint32_t r) {
     Lengths l = {0, 0, 0, 0};
     if (r < a.p.requests) {
         l.context = a.context_lens[r], l.fresh = a.new_lens[r], l.held = min(a.state.held[r], a.p.max_blocks);
+        // (of lengths that a step has left: tokens that it had no block for are counted in them and lie nowhere)
+        if (a.context_lens == a.step.kv_lens) l.context = min(l.context, l.held * a.p.block_tokens);
         l.want = blocks_of(a, add_up(l.context, l.fresh));
     }
     return l;

@@ -731,7 +731,8 @@ class PagedTables:
 
     def record(self, plan, context_lens, new_lens):
         """A step of new_lens[r] tokens behind context_lens[r]: blocks taken or given back, slots, positions, query_starts,
-        kv_lens.  context_lens may be kv_lens: a recorded step then goes on from where the last one ended."""
+        kv_lens.  context_lens may be kv_lens: a recorded step then goes on from where the last one ended, behind the tokens that
+        had a block (those counted in `unplaced` are to come again); other context_lens must leave such tokens out themselves."""
         for t, what in ((context_lens, "context_lens"), (new_lens, "new_lens")):
             _need(t, torch.int32, f"PagedTables {what}")
             if t.numel() != self.requests:

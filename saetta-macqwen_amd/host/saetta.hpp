@@ -979,7 +979,8 @@ struct PagedTables {
         return saetta_paged_batch{static_cast<const uint32_t *>(query_starts.get()), static_cast<const uint32_t *>(kv_lens.get()),
                                   static_cast<const int32_t *>(block_table.get()), uint32_t(requests), uint32_t(max_blocks), uint32_t(block_tokens)};
     }
-    // A step of new_lens[r] tokens behind context_lens[r] (u32 both; context_lens may be kv_lens).
+    // A step of new_lens[r] tokens behind context_lens[r] (u32 both; context_lens may be kv_lens: then behind those that had a block; others must
+    // leave tokens without one out themselves).
     void record(plan::Plan &plan, const View &context_lens, const View &new_lens) const {
         const PagedTables self = *this;
         plan.op("paged_tables", [=](hipStream_t s) { self.step(s, context_lens, new_lens); });
