@@ -525,7 +525,7 @@ int saetta_attn_gemm(saetta_stream_t stream, int bits, const uint16_t *q_f16, sa
                      saetta_flash_params p, uint32_t slice_tokens, uint32_t stages, void *workspace,
                      size_t workspace_bytes);
 
-/* ---- a cache in blocks that several requests share --------------------------- */
+/* ---- a cache in blocks for several requests -------------------------------------- */
 
 /* The reference serves one sequence over a cache that is a plain row array (src/gpu_layers.rs:183-293); these entry
  * points have no counterpart in it.  They serve several requests (conversations) at once: their keys and values lie
@@ -561,7 +561,10 @@ typedef struct saetta_paged_cache {
 } saetta_paged_cache;
 
 /* What the requests hold: row r of block_table [requests][max_blocks] names request r's blocks in order, of which the
- * first held[r] are its own.  free_list [blocks]: the blocks that nobody holds, the first *free_count of it. */
+ * first held[r] are its own.  free_list [blocks]: the blocks that nobody holds, the first *free_count of it.  A block is in one place, of a row or of the free list:
+ * saetta_paged_tables gives what a request no longer needs back without looking at the other rows, so that a block which two rows name would be handed out while the
+ * other still reads it.  Requests behind a common prefix can name its blocks in common where the program keeps table, slots, starts and lengths itself and leaves
+ * saetta_paged_tables out: the other calls only read them. */
 typedef struct saetta_paged_state {
     int32_t *block_table;
     uint32_t *held;

@@ -1,4 +1,4 @@
-// Attention of a step's new tokens over a cache in blocks that several requests share.
+// Attention of a step's new tokens over a cache in blocks for several requests.
 //
 // For row i of request r, at position p = kv_lens[r] - n + i, and q head h over kv head h / group:
 //     out = sum_t 2^(s_t) v_t / sum_t 2^(s_t) [* sigmoid(gate)],  s_t = log2(e) scale (q . k_t),  t = 0 .. p.

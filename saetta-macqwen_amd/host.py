@@ -701,7 +701,8 @@ class PagedCache:
 class PagedTables:
     """Which blocks the requests hold, and what a step's tokens are given: all on the GPU, from the requests' lengths.
     `requests` rows, room for `tokens` new tokens a step, up to `max_blocks` blocks a request of a cache of `blocks`.
-    (The tensors are a program's own to fill in place, too, where it keeps tables on the host.)"""
+    (The tensors are a program's own to fill in place, too, where it keeps tables on the host.  It does so for requests that name
+    blocks in common: `encode` and `record` take a block to be one request's, and give it back with that one.)"""
 
     def __init__(self, requests, tokens, max_blocks, blocks, block_tokens=64, device="cuda"):
         if requests < 1 or tokens < 1 or max_blocks < 1 or blocks < 1:

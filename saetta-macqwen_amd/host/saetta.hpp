@@ -902,7 +902,7 @@ class RowBackup {
 
 }  // namespace gpu_layers
 
-// A cache in blocks that several requests share, the tables over it and the attention that reads it (include/saetta_hip.h; the
+// A cache in blocks for several requests, the tables over it and the attention that reads it (include/saetta_hip.h; the
 // reference's caches are one sequence's).
 namespace paged {
 
@@ -958,7 +958,7 @@ struct PagedCache {
     }
 };
 
-// Which blocks the requests hold, and what a step's tokens are given.
+// Which blocks the requests hold, each one request's, and what a step's tokens are given.
 struct PagedTables {
     size_t requests, tokens, max_blocks, blocks, block_tokens;
     gpu::Buffer block_table, held, free_list, free_count, query_starts, kv_lens, slots, positions, unplaced;
