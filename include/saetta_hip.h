@@ -661,7 +661,8 @@ int saetta_paged_split(saetta_stream_t stream, saetta_paged_batch batch, saetta_
 
 /* out = softmax(q K^T scale) V [* sigmoid(gate)] for the new tokens of all requests, whose keys and values are in
  * the cache already: token i of the n that request r has now sits at position kv_lens[r] - n + i and sees the positions up to its
- * own.  q, gate and out are f16 or bf16 (type) rows of p.heads heads; gate.data NULL: no gate.  out may be q.  Rows past the step's last token,
+ * own.  q, gate and out are f16 or bf16 (type) rows of p.heads heads; gate.data NULL: no gate.  out's rows must not
+ * overlap; out may be q, row for row, and no other part of it.  Rows past the step's last token,
  * and tokens of a request past p.rows where p.rows is for few rows, are left as they were; a row that sees nothing (its position is
  * below 0, or its blocks are not there) becomes zeros.  A score (times log2 e) below -1e30 counts as not seen.  A weight of
  * a row's softmax is off by up to 2^-11 of it (2^-22 where a request has up to 16 rows, new tokens times q heads per kv head), or by 2^-32 of the row's largest where

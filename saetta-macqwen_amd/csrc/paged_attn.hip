@@ -1122,6 +1122,18 @@ int check_batch(const saetta_paged_batch &b, const char *what) {
 size_t items_offset() { return sizeof(SplitHead); }
 size_t tiles_offset(const Shape &s) { return items_offset() + sizeof(Item) * s.most_items; }
 
+// Whether no two of the rows overlap.  (Strides from 0 up: rows h heads and t tokens apart, and the same with h taken back, are |h head_stride - t token_stride| apart
+// at least; of a head's t the two next to its place are the nearest.)
+bool rows_apart(const saetta_strided_rows &r, uint64_t tokens, uint64_t heads) {
+    const uint64_t ts = r.token_stride, hs = r.head_stride;
+    if ((heads == 1 || hs >= DIM) && (tokens <= 1 || ts >= (heads - 1) * hs + DIM)) return true;
+    for (uint64_t h = 0; h < heads; h++) {
+        const uint64_t at = h * hs, t0 = ts ? at / ts : 0;
+        for (uint64_t t = t0; t <= t0 + 1; t++)
+            if (t < tokens && (h || t) && (at > t * ts ? at - t * ts : t * ts - at) < DIM) return false;
+    }
+    return true;
+}
 Rows narrow(const saetta_strided_rows &r) { return {r.data, uint32_t(r.token_stride), uint32_t(r.head_stride)}; }
 uint32_t shift_of(uint32_t n) { return uint32_t(__builtin_ctz(n)); }
 
@@ -1202,6 +1214,8 @@ extern "C" int saetta_paged_attn(saetta_stream_t stream, int type, saetta_stride
     for (const saetta_strided_rows &r : {q, gate, out})
         SAETTA_REQUIRE(r.token_stride < (1ull << 32) && r.head_stride < (1ull << 32), SAETTA_E_SHAPE, "paged_attn: strides of %llu and %llu values (less than 2^32)",
                        static_cast<unsigned long long>(r.token_stride), static_cast<unsigned long long>(r.head_stride));
+    SAETTA_REQUIRE(rows_apart(out, p.tokens, p.heads), SAETTA_E_SHAPE, "paged_attn: out's rows overlap (strides of %llu and %llu values)",
+                   static_cast<unsigned long long>(out.token_stride), static_cast<unsigned long long>(out.head_stride));
     SAETTA_REQUIRE(aligned(split, 16) && aligned(workspace, 16), SAETTA_E_ALIGN, "paged_attn: split and workspace must be 16-byte aligned");
     const size_t need = saetta_paged_workspace_bytes(p, batch.requests);
     SAETTA_REQUIRE(workspace_bytes >= need, SAETTA_E_SCRATCH, "paged_attn: workspace of %zu bytes (%zu needed)", workspace_bytes, need);

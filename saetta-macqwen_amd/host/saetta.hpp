@@ -910,7 +910,7 @@ constexpr size_t HEAD_DIM = SAETTA_HEAD_DIM;
 enum class Type { F32 = SAETTA_F32, F16 = SAETTA_F16, BF16 = SAETTA_BF16 };
 inline size_t type_bytes(Type t) { return t == Type::F32 ? 4 : 2; }
 
-// Rows of `heads` rows of 256 values; strides in values (0: contiguous).
+// Rows of `heads` rows of 256 values, contiguous or with strides in values (0: the same row again, of what is read).
 struct Rows {
     View view;
     uint64_t token_stride, head_stride;

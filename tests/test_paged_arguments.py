@@ -1,0 +1,27 @@
+"""What the paged calls refuse of strides and sizes, by arguments alone: on the CPU."""
+import pytest
+
+from test_paged_refusals import A, batch, cache, ffi, params, refused, rows
+
+
+def attn(out, **over):
+    p = params(**over)
+    return ffi.lib().saetta_paged_attn(None, 1, rows(), cache(kv_heads=p.kv_heads), batch(), A, rows(None), out, p, A, 1 << 40)
+
+
+@pytest.mark.parametrize("token, head, over", [
+    (0, 0, {}), (0, 256, {}), (4096, 0, {}), (4096, 128, {}), (128, 4096, {}), (4088, 256, {}), (512, 256, {}), (256, 256, {}), (3840, 256, {}), (256, 1024, {}),
+    (768, 512, {}),  # three heads on is two tokens on
+    (256, 8, dict(tokens=2, heads=2)), (0, 256, dict(tokens=2, heads=2)), (4294967288, 4294967288, dict(tokens=3, heads=16))])
+def test_rows_of_the_output_that_overlap(token, head, over):
+    refused(attn(rows(token=token, head=head), **over), -2, "overlap")
+
+
+@pytest.mark.parametrize("token, head, over", [
+    (4096, 256, {}), (256, 1280, {}), (8192, 512, {}), (0, 256, dict(tokens=1)), (256, 0, dict(heads=1, kv_heads=1)), (0, 0, dict(tokens=1, heads=1, kv_heads=1)),
+    (768, 512, dict(tokens=2, heads=4, kv_heads=4)), (4096, 256, dict(tokens=(1 << 24) - 1)), (0, 0, dict(tokens=0, heads=1, kv_heads=1))])
+def test_rows_of_the_output_that_lie_apart(token, head, over):
+    """Refused for something else that is looked at later: a workspace that is not aligned."""
+    p = params(**over)
+    out = ffi.lib().saetta_paged_attn(None, 1, rows(), cache(kv_heads=p.kv_heads), batch(), A, rows(None), rows(token=token, head=head), p, A + 8, 1 << 40)
+    refused(out, -4, "split and workspace")
