@@ -641,7 +641,17 @@ def _rows_of(t, heads, dtypes, what):
     return ffi.StridedRowsC(t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if heads > 1 else 0)
 
 
-class PagedCache:
+class _Kept:
+    """What stays as it was made: eager and recorded calls hold its buffers and sizes, so that one replaced later would be another call's memory.  (Buffers are
+    filled in place.)"""
+
+    def __setattr__(self, name, value):
+        if name in self.__dict__:
+            raise AttributeError(f"{type(self).__name__}.{name} cannot be replaced (buffers are filled in place)")
+        super().__setattr__(name, value)
+
+
+class PagedCache(_Kept):
     """The keys and values of one layer for several requests at once, in blocks of 16, 32, 64 or 128 tokens: 8-bit
     floating point codes (e4m3) with one power of two per block and kv head, for keys and for values.  The reference
     has no counterpart (its caches are one sequence's).  Slot s is token s % block_tokens of block s // block_tokens."""
@@ -698,7 +708,7 @@ class PagedCache:
         _calls.paged_gather(slots, keys, values, self._parts, _handle(stream))
 
 
-class PagedTables:
+class PagedTables(_Kept):
     """Which blocks the requests hold, and what a step's tokens are given: all on the GPU, from the requests' lengths.
     `requests` rows, room for `tokens` new tokens a step, up to `max_blocks` blocks a request of a cache of `blocks`.
     (The tensors are a program's own to fill in place, too, where it keeps tables on the host.  It does so for requests that name
@@ -748,7 +758,7 @@ class PagedTables:
         _calls.paged_tables(context_lens, new_lens, self._state, self._sizes, _handle(stream))
 
 
-class PagedAttention:
+class PagedAttention(_Kept):
     """Attention of a step's new tokens over paged caches: scratch and launches for tables of one size and up to `rows`
     new tokens a request (1: a token each; a verify step's rows; a chunk's tokens; any mixture).  The scratch is one
     call's at a time: calls, or graphs of them, that may overlap want objects of their own."""

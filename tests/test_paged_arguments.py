@@ -1,7 +1,8 @@
 """What the paged calls refuse of strides and sizes, by arguments alone: on the CPU."""
 import pytest
+import torch
 
-from test_paged_refusals import A, batch, cache, ffi, params, refused, rows
+from test_paged_refusals import A, batch, cache, ffi, params, refused, rows, saetta
 
 
 def attn(out, **over):
@@ -25,3 +26,14 @@ def test_rows_of_the_output_that_lie_apart(token, head, over):
     p = params(**over)
     out = ffi.lib().saetta_paged_attn(None, 1, rows(), cache(kv_heads=p.kv_heads), batch(), A, rows(None), rows(token=token, head=head), p, A + 8, 1 << 40)
     refused(out, -4, "split and workspace")
+
+
+def test_buffers_and_sizes_cannot_be_replaced():
+    """A buffer put in another's place was read by recorded calls and not by others."""
+    for made, names in ((saetta.PagedCache(2, 256, 4, 64, device="cpu"), ("keys", "value_scales", "blocks", "kv_heads")),
+                        (saetta.PagedTables(2, 4, 4, 8, device="cpu"), ("block_table", "free_count", "kv_lens", "slots", "tokens", "max_blocks"))):
+        for name in names:
+            was = getattr(made, name)
+            with pytest.raises(AttributeError, match=name):
+                setattr(made, name, was.clone() if isinstance(was, torch.Tensor) else was + 1)
+            assert getattr(made, name) is was
