@@ -621,7 +621,7 @@ typedef struct saetta_strided_rows {
  * become what they stand for times 2^(their e - e), rounded to nearest even like the new ones; e falls only when the
  * block begins anew.  A value that is not finite, or larger than 448 * 2^60, is stored as NaN.  The tokens of one block follow each other
  * in the call, at rising slots without a gap, as saetta_paged_tables gives them; what a block holds that a call
- * names by two such runs is undefined.  What a block holds behind the last token that was stored in it counts no more.  tokens < 2^28, as for saetta_paged_gather. */
+ * names by two such runs is undefined.  What a block holds behind the last token that was stored in it counts no more.  At most 2^28 - 32 tokens, as for saetta_paged_gather. */
 int saetta_paged_store(saetta_stream_t stream, int type, saetta_strided_rows keys, saetta_strided_rows values,
                        const int32_t *slots, saetta_paged_cache cache, uint32_t tokens);
 

@@ -28,6 +28,9 @@ constexpr uint32_t lane_tokens(int units) { return units < 4 ? units * UNIT_TOKE
 // Workgroups (of all kv heads and sides) that look for runs, unless a block's tokens would be fewer than each looks at.
 constexpr uint32_t STORE_GROUPS = 512;
 
+// The most tokens of a call: 2^32 threads are one more than a launch has, and a workgroup of the store has 512 for 32 tokens, or 256 for 16, at most.
+constexpr uint32_t MOST_TOKENS = (1u << 28) - 32;
+
 struct StoreArgs {
     saetta_strided_rows x[2];  // keys, values
     const int32_t *slots;
@@ -326,7 +329,7 @@ extern "C" int saetta_paged_store(saetta_stream_t stream, int type, saetta_strid
     if (int rc = check_cache(cache, "paged_store")) return rc;
     SAETTA_REQUIRE(aligned(slots, 4) && rows_aligned(keys, type) && rows_aligned(values, type), SAETTA_E_ALIGN,
                    "paged_store: keys and values must be 16-byte aligned, with strides of multiples of 16 bytes");
-    SAETTA_REQUIRE(tokens < (1u << 28), SAETTA_E_SHAPE, "paged_store: %u tokens (fewer than 2^28)", tokens);
+    SAETTA_REQUIRE(tokens <= MOST_TOKENS, SAETTA_E_SHAPE, "paged_store: %u tokens (at most 2^28 - 32)", tokens);
     if (int rc = ensure_device()) return rc;
     if (tokens == 0) return SAETTA_OK;
     const StoreArgs a = {{keys, values}, slots, {cache.keys, cache.values}, {cache.key_scales, cache.value_scales},
@@ -343,7 +346,7 @@ extern "C" int saetta_paged_gather(saetta_stream_t stream, int type, saetta_page
     SAETTA_REQUIRE(tokens == 0 || slots, SAETTA_E_NULL, "paged_gather: null slots");
     if (int rc = check_cache(cache, "paged_gather")) return rc;
     SAETTA_REQUIRE(aligned(slots, 4) && aligned(keys, 16) && aligned(values, 16), SAETTA_E_ALIGN, "paged_gather: keys and values must be 16-byte aligned");
-    SAETTA_REQUIRE(tokens < (1u << 28), SAETTA_E_SHAPE, "paged_gather: %u tokens (fewer than 2^28)", tokens);
+    SAETTA_REQUIRE(tokens <= MOST_TOKENS, SAETTA_E_SHAPE, "paged_gather: %u tokens (at most 2^28 - 32)", tokens);
     if (int rc = ensure_device()) return rc;
     if (tokens == 0 || (!keys && !values)) return SAETTA_OK;
     const GatherArgs a = {{cache.keys, cache.values}, {cache.key_scales, cache.value_scales}, slots, {keys, values},

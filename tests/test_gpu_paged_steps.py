@@ -48,3 +48,19 @@ def test_a_step_short_of_blocks(room):
         assert (np.abs(numbers(out)[:n] - want) <= bound * 1.001 + 2.0 ** -11 * np.abs(want) + 2.0 ** -25).all()
         short.append(step["unplaced"][0])
     assert [s > 0 for s in short] == [False, True, True, False, True, True, False, True, True, False]
+
+
+@pytest.mark.parametrize("block", [16, 32, 128])
+def test_the_most_tokens_of_a_call(block):
+    """Nearly 2^28 of them, all but a few without a slot; their rows are one and the same."""
+    tokens, cache = (1 << 28) - 32, saetta.PagedCache(1, DIM, 4, block)
+    k = torch.randn(1, 1, DIM, device="cuda")
+    slots = torch.full((tokens,), -1, dtype=torch.int32, device="cuda")
+    there = {5: block, (1 << 27) + 3: 2 * block, tokens - 1: 0}
+    for at, slot in there.items():
+        slots[at] = slot
+    cache.encode(k.expand(tokens, 1, DIM), k.expand(tokens, 1, DIM), slots)
+    plain = Cache(1, 4, block)
+    plain.store(numbers(k), numbers(k), [0])
+    for want, got in zip(plain.gather([0, 0, 0]), Cache.of(cache).gather(list(there.values()))):
+        assert np.array_equal(want, got)

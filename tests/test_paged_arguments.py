@@ -37,3 +37,13 @@ def test_buffers_and_sizes_cannot_be_replaced():
             with pytest.raises(AttributeError, match=name):
                 setattr(made, name, was.clone() if isinstance(was, torch.Tensor) else was + 1)
             assert getattr(made, name) is was
+
+
+@pytest.mark.parametrize("tokens, ok", [((1 << 28) - 32, True), ((1 << 28) - 31, False), ((1 << 28) - 1, False)])
+def test_the_most_tokens_of_a_call(tokens, ok):
+    """A launch has fewer than 2^32 threads."""
+    l = ffi.lib()
+    for size in (16, 32, 64):
+        for rc in (l.saetta_paged_store(None, 1, rows(), rows(), A + (2 if ok else 0), cache(block_tokens=size), tokens),
+                   l.saetta_paged_gather(None, 1, cache(block_tokens=size), A + (2 if ok else 0), A, A, tokens)):
+            refused(rc, -4, "") if ok else refused(rc, -2, "2^28 - 32")
