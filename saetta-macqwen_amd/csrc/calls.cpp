@@ -272,6 +272,10 @@ PyObject *item(PyObject *tuple, Py_ssize_t i, Py_ssize_t n, const char *what) {
     if (!PyTuple_Check(tuple) || PyTuple_GET_SIZE(tuple) != n) raise(PyExc_TypeError, "%s: expected a tuple of %zd", what, n);
     return PyTuple_GET_ITEM(tuple, i);
 }
+// Sizes that the library takes in 32 bits.
+void fits32(long long n, const char *what) {
+    if (n > 0xffffffffll) raise(PyExc_ValueError, "%s: %lld of them (fewer than 2^32)", what, n);
+}
 // A contiguous tensor of `dtype` on the current device.
 const at::Tensor &here(PyObject *o, at::ScalarType dtype, const char *what) {
     if (!THPVariable_Check(o)) raise(PyExc_TypeError, "%s: expected a tensor", what);
@@ -355,6 +359,7 @@ PyObject *paged_store(PyObject *module, PyObject *const *a, Py_ssize_t n) {
         const at::Tensor &slots = here(a[2], at::kInt, "PagedCache slots");
         if (k.type != v.type || k.tokens != v.tokens || slots.numel() != k.tokens)
             raise(PyExc_ValueError, "PagedCache: k, v and slots must be of as many tokens, k and v of one type");
+        fits32(k.tokens, "PagedCache slots");
         State &st = state_of(module);
         const Library &lib = library(st);
         const saetta_stream_t s = stream_of(a[4]);
@@ -384,6 +389,7 @@ PyObject *paged_gather(PyObject *module, PyObject *const *a, Py_ssize_t n) {
             type = is, to[i] = t.data_ptr();
         }
         if (type < 0) raise(PyExc_ValueError, "PagedCache: keys or values or both");
+        fits32(slots.numel(), "PagedCache slots");
         State &st = state_of(module);
         const Library &lib = library(st);
         const saetta_stream_t s = stream_of(a[4]);

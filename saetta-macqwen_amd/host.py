@@ -631,6 +631,12 @@ def _one_device(what, *tensors):
         raise ValueError(f"{what}: tensors of one device, got " + ", ".join(sorted({str(t.device) for t in tensors if t is not None})))
 
 
+def _fits32(what, *sizes):
+    """The library takes sizes in 32 bits, and ctypes would cut them."""
+    if any(not 0 <= n < 1 << 32 for n in sizes):
+        raise ValueError(f"{what}: sizes of less than 2^32, got " + ", ".join(str(n) for n in sizes))
+
+
 def _rows_of(t, heads, dtypes, what):
     """[tokens, heads, 256] with any strides that the library takes, as StridedRowsC."""
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes):
@@ -661,6 +667,7 @@ class PagedCache(_Kept):
             raise ValueError("a paged cache is written for head dim 256")
         if kv_heads < 1 or block_tokens not in (16, 32, 64, 128) or blocks < 1 or blocks * block_tokens >= 1 << 31:
             raise ValueError("PagedCache: blocks of 16, 32, 64 or 128 tokens, fewer than 2^31 in all")
+        _fits32("PagedCache", kv_heads, blocks)
         self.kv_heads, self.head_dim, self.blocks, self.block_tokens = kv_heads, head_dim, blocks, block_tokens
         self.keys, self.values = (torch.zeros(blocks, kv_heads, block_tokens * DIM, dtype=torch.uint8, device=device) for _ in range(2))
         self.key_scales, self.value_scales = (torch.full((blocks, kv_heads), 127 - 40, dtype=torch.uint8, device=device) for _ in range(2))
@@ -682,6 +689,7 @@ class PagedCache(_Kept):
         _need(slots, torch.int32, "PagedCache slots")
         if k.dtype is not v.dtype or k.shape[0] != v.shape[0] or slots.numel() != k.shape[0]:
             raise ValueError("PagedCache: k, v and slots must be of as many tokens, k and v of one type")
+        _fits32("PagedCache", slots.numel())
         _one_device("PagedCache", k, v, slots, *self.tensors())
         plan.op("paged_store", _Call("saetta_paged_store", "paged_store", (
             _TYPES[k.dtype], *rows, _ptr(slots), self.c(), slots.numel()), (k, v, slots, *self.tensors())))
@@ -699,6 +707,7 @@ class PagedCache(_Kept):
             _need(t, outs[0].dtype, "PagedCache keys and values")
             if t.numel() < slots.numel() * self.kv_heads * DIM:
                 raise ValueError("PagedCache: keys and values do not hold the slots' rows")
+        _fits32("PagedCache", slots.numel())
         _one_device("PagedCache", slots, keys, values, *self.tensors())
         plan.op("paged_gather", _Call("saetta_paged_gather", "paged_gather", (
             _TYPES[outs[0].dtype], self.c(), _ptr(slots), *[None if t is None else _ptr(t) for t in (keys, values)], slots.numel()),
@@ -719,6 +728,7 @@ class PagedTables(_Kept):
             raise ValueError("PagedTables: sizes of one at least")
         if block_tokens not in (16, 32, 64, 128) or blocks * block_tokens >= 1 << 31 or max_blocks * block_tokens >= 1 << 31:
             raise ValueError("PagedTables: blocks of 16, 32, 64 or 128 tokens, fewer than 2^31 in all")
+        _fits32("PagedTables", requests, tokens)
         self.requests, self.tokens, self.max_blocks, self.blocks, self.block_tokens = requests, tokens, max_blocks, blocks, block_tokens
         ints = {"dtype": torch.int32, "device": device}
         self.block_table = torch.full((requests, max_blocks), -1, **ints)
@@ -770,6 +780,7 @@ class PagedAttention(_Kept):
             raise ValueError("paged attention needs 1, 2, 4, 8 or 16 q heads per kv head")
         if rows < 1:
             raise ValueError("paged attention: rows of one at least")
+        _fits32("paged attention", heads, kv_heads, rows)
         self.heads, self.kv_heads, self.rows = heads, kv_heads, rows
         self.shape = (tables.requests, tables.tokens, tables.max_blocks, tables.block_tokens)
         self._params = (heads, kv_heads, tables.tokens, rows, 1.0 / math.sqrt(DIM))

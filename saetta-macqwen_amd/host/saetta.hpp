@@ -909,6 +909,11 @@ namespace paged {
 constexpr size_t HEAD_DIM = SAETTA_HEAD_DIM;
 enum class Type { F32 = SAETTA_F32, F16 = SAETTA_F16, BF16 = SAETTA_BF16 };
 inline size_t type_bytes(Type t) { return t == Type::F32 ? 4 : 2; }
+// A size as the library takes it, in 32 bits.
+inline uint32_t size32(size_t n, const char *what) {
+    if (n > 0xffffffffu) throw std::runtime_error(std::string(what) + ": a size of 2^32 or more");
+    return uint32_t(n);
+}
 
 // Rows of `heads` rows of 256 values, contiguous or with strides in values (0: the same row again, of what is read).
 struct Rows {
@@ -928,6 +933,7 @@ struct PagedCache {
     PagedCache(const gpu::Gpu &gpu, size_t kv_heads_, size_t head_dim, size_t blocks_, size_t block_tokens_ = 64)
         : kv_heads(kv_heads_), blocks(blocks_), block_tokens(block_tokens_) {
         if (head_dim != HEAD_DIM) throw std::runtime_error("a paged cache is written for head dim 256");
+        size32(kv_heads, "PagedCache::new");
         if (kv_heads == 0 || blocks == 0 || (block_tokens != 16 && block_tokens != 32 && block_tokens != 64 && block_tokens != 128) ||
             blocks >= (size_t(1) << 31) / block_tokens)
             throw std::runtime_error("PagedCache::new: blocks of 16, 32, 64 or 128 tokens, fewer than 2^31 in all");
@@ -949,12 +955,12 @@ struct PagedCache {
     }
     // What the slots hold, as [tokens][kv_heads][256] of the type.
     void encode_dequantize(const gpu::Gpu &gpu, Type type, const View &slots, const View &keys_out, const View &values_out, size_t tokens) const {
-        check(saetta_paged_gather(gpu.stream(), int(type), c(), slots.ptr<int32_t>(), keys_out.ptr<void>(), values_out.ptr<void>(), uint32_t(tokens)), "paged_gather");
+        check(saetta_paged_gather(gpu.stream(), int(type), c(), slots.ptr<int32_t>(), keys_out.ptr<void>(), values_out.ptr<void>(), size32(tokens, "paged_gather")), "paged_gather");
     }
 
   private:
     void store(hipStream_t s, Type type, const Rows &k, const Rows &v, const View &slots, size_t tokens) const {
-        check(saetta_paged_store(s, int(type), k.c(), v.c(), slots.ptr<int32_t>(), c(), uint32_t(tokens)), "paged_store");
+        check(saetta_paged_store(s, int(type), k.c(), v.c(), slots.ptr<int32_t>(), c(), size32(tokens, "paged_store")), "paged_store");
     }
 };
 
@@ -965,6 +971,7 @@ struct PagedTables {
 
     PagedTables(const gpu::Gpu &gpu, size_t requests_, size_t tokens_, size_t max_blocks_, size_t blocks_, size_t block_tokens_ = 64)
         : requests(requests_), tokens(tokens_), max_blocks(max_blocks_), blocks(blocks_), block_tokens(block_tokens_) {
+        for (size_t n : {requests, tokens, max_blocks, blocks, block_tokens}) size32(n, "PagedTables::new");
         if (requests == 0 || tokens == 0 || max_blocks == 0 || blocks == 0) throw std::runtime_error("PagedTables::new: sizes of one at least");
         block_table = gpu.buffer_from(std::vector<int32_t>(requests * max_blocks, -1));
         held = gpu.buffer(requests * 4);
@@ -1002,7 +1009,7 @@ struct PagedTables {
 class PagedAttention {
   public:
     PagedAttention(const gpu::Gpu &gpu, size_t heads, size_t kv_heads, size_t head_dim, const PagedTables &tables, size_t rows)
-        : tables_(tables), p_{uint32_t(heads), uint32_t(kv_heads), uint32_t(tables.tokens), uint32_t(rows), 1.0f / 16.0f} {
+        : tables_(tables), p_{size32(heads, "PagedAttention::new"), size32(kv_heads, "PagedAttention::new"), uint32_t(tables.tokens), size32(rows, "PagedAttention::new"), 1.0f / 16.0f} {
         if (head_dim != HEAD_DIM) throw std::runtime_error("paged attention is written for head dim 256");
         const size_t split = saetta_paged_split_bytes(p_, uint32_t(tables.requests)), workspace = saetta_paged_workspace_bytes(p_, uint32_t(tables.requests));
         if (split == 0 || workspace == 0) throw std::runtime_error(std::string("PagedAttention::new: ") + saetta_last_error());

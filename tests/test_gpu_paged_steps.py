@@ -64,3 +64,12 @@ def test_the_most_tokens_of_a_call(block):
     plain.store(numbers(k), numbers(k), [0])
     for want, got in zip(plain.gather([0, 0, 0]), Cache.of(cache).gather(list(there.values()))):
         assert np.array_equal(want, got)
+
+
+def test_more_slots_than_32_bits_count():
+    """Refused, by the calls that are made at once and by those that are recorded: 2^32 + 1 slots were taken for one."""
+    n, cache = (1 << 32) + 1, saetta.PagedCache(1, DIM, 1, 16)
+    slots, k = torch.empty(n, dtype=torch.int32, device="cuda"), torch.zeros(1, 1, DIM, device="cuda").expand(n, 1, DIM)
+    for call in (lambda: cache.encode(k, k, slots), lambda: cache.record(saetta.Plan(), k, k, slots)):
+        with pytest.raises(ValueError, match="2\\^32"):
+            call()

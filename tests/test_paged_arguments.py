@@ -47,3 +47,16 @@ def test_the_most_tokens_of_a_call(tokens, ok):
         for rc in (l.saetta_paged_store(None, 1, rows(), rows(), A + (2 if ok else 0), cache(block_tokens=size), tokens),
                    l.saetta_paged_gather(None, 1, cache(block_tokens=size), A + (2 if ok else 0), A, A, tokens)):
             refused(rc, -4, "") if ok else refused(rc, -2, "2^28 - 32")
+
+
+def test_sizes_past_32_bits():
+    """Cut to 32 bits they would be another call's: rows 2^32 + 1 were taken for 1."""
+    tables = saetta.PagedTables(2, 4, 4, 8, device="cpu")
+    for over in (dict(rows=(1 << 32) + 1), dict(heads=(1 << 32) + 16, kv_heads=(1 << 32) + 16)):
+        with pytest.raises(ValueError, match="2\\^32"):
+            saetta.PagedAttention(**{**dict(heads=16, kv_heads=2, head_dim=256, tables=tables, rows=1), **over})
+    for over in (dict(requests=(1 << 32) + 1), dict(tokens=1 << 32)):
+        with pytest.raises(ValueError, match="2\\^32"):
+            saetta.PagedTables(**{**dict(requests=1, tokens=1, max_blocks=1, blocks=1, device="meta"), **over})
+    with pytest.raises(ValueError, match="2\\^32"):
+        saetta.PagedCache((1 << 32) + 2, 256, 4, 64, device="meta")
