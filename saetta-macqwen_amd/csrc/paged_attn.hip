@@ -407,9 +407,9 @@ __device__ __forceinline__ void put_row(const AttnArgs &a, uint32_t row, uint32_
 // unit a lane: no barrier in the walk, and the scales, which only the scores want, come behind the first codes.
 // One group is two workgroups to a CU; two have the registers of a SIMD to themselves; of four, two teams of four waves take two each over the
 // same keys, whose codes the second team finds in the caches.  (The kernel for chunks, where most of a tile is empty, takes 102 to 108 us for 64 drafts of 3
-// to 8 rows at 4000 tokens, this one 46 to 69; four groups to a wave are more registers than there are: 353.)
-// Measured, 8 q heads over each of 2 kv heads: a token of 8 requests at 131072 tokens, f16, 162 us, 6.6 TB/s of codes (a large copy reaches 4.8, read and
-// written); of 48 requests at 330 to 30 thousand tokens, bf16, 55 us, 5.9 TB/s; of one at 517 tokens 6.3 us, the launch and three loads that wait for each other.
+// to 8 tokens at 4000, this one 49 to 69; four groups to a wave are more registers than there are: 353.)
+// Measured, 8 q heads over each of 2 kv heads: a token of 8 requests at 131072 tokens, f16, 162 us, 6.6 TB/s of codes (a large copy reaches 4.9, read and
+// written); of 48 requests at 330 to 30 thousand tokens, bf16, 56 us, 5.9 TB/s; of one at 517 tokens 7 to 8 us, the launch and three loads that wait for each other.
 constexpr int few_threads(int columns) { return 64 * FEW_WAVES * (columns == 4 ? 2 : 1); }
 constexpr uint32_t FEW_STEPS = 32;     // steps that a wave looks up at a time
 constexpr int FEW_STRIDE = DIM + 4;    // floats of a row in LDS: neighbouring rows on other banks
@@ -687,9 +687,9 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 //   waves 0..3:  softmax(s)                | O(s) + S(s+1)
 //   waves 4..7:  O(s) + S(s+1)             | softmax(s+1)
 // Step s reads V(s) and K(s+1) as halves and makes V(s+1) and K(s+2), in the places of V(s-1) and K(s): one barrier a step.
-// Bound by the matrix cores and the clock that they leave (1.8 GHz): 4096 tokens at 28672, bf16, 16 q heads over 2 kv heads, 1.78 to 1.87 ms, 1.10 to 1.16 PFLOP/s (a
-// large product of the library: 1.23); the streams of products alone 1.45 ms; without the priority that keeps the two waves in opposite order 2.28.  A short item
-// is bound by its start and end, 13 to 16 us: seven prompts of 147 to 1645 tokens 76 us, a tile of 32 tokens 20.
+// Bound by the matrix cores and the clock that they leave (1.8 GHz): 4096 tokens at 28672, bf16, 16 q heads over 2 kv heads, 1.75 to 1.87 ms, 1.10 to 1.18 PFLOP/s (a
+// large product of the library: 1.20 to 1.28); the streams of products alone 1.45 ms; without the priority that keeps the two waves in opposite order 2.28.  A short item
+// is bound by its start and end, 13 to 16 us: seven prompts of 147 to 1645 tokens 73 us, a tile of 32 tokens 20.
 constexpr uint32_t CODE_BYTES = STEP_KEYS * DIM, HALF_BYTES = 2 * CODE_BYTES;  // a step's keys, or values
 constexpr uint32_t AHEAD = 3, PLACES = 4;
 constexpr uint32_t K_HALVES = 0, V_HALVES = 2 * HALF_BYTES, K_CODES = 4 * HALF_BYTES, V_CODES = K_CODES + PLACES * CODE_BYTES;
@@ -714,7 +714,7 @@ __global__ __launch_bounds__(64 * CHUNK_WAVES, 2) void paged_chunk_kernel(AttnAr
     if (!(int(index < items) & int(item_ok(a, item, 1)))) return;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t rows = item.tokens << a.group_shift;
-    // A draft beside a chunk, a prompt's last tokens.  (64 requests of 2, 4, 8 tokens at 4000, by this kernel: 44, 55, 76 us; by the one for few rows 44, 50, 69.
+    // A draft beside a chunk, a prompt's last tokens.  (64 requests of 2, 4, 8 tokens at 4000, by this kernel: 46, 58, 73 us; by the one for few rows 46, 50, 68.
     // With one group to a wave and more teams, which spills no registers, 44, 70, 81.)
     if (rows <= 4 * FEW_ROWS) {
         auto few = [&](auto columns, auto teams) {

@@ -10,8 +10,8 @@
 // from the slots alone), one kv head, keys or values; its largest magnitude is known before the first code is written, with the values held in
 // registers.  A wave has four tokens of a unit, a lane four dims of each: a load is a token's row, and what a wave stores of four tokens fills lines of 64
 // bytes.  A run of up to four tokens is one wave's, so that a step's tokens and drafts are stored at once.  Measured, 2 kv heads: 9700 tokens of five
-// prompts, f32, blocks of 16, 13.2 us, 3.8 TB/s of what is read and written (a large copy: 4.8; with whole tokens to a wave, whose stores fill no lines, 22.8);
-// 16384 tokens, f16, blocks of 64, 19 us; 64 single tokens 4.8 us, the chain of slot, row, maximum and codes, and no more in a step that has room for 4096.
+// prompts, f32, blocks of 16, 13 us, 3.8 TB/s of what is read and written (a large copy: 4.9; with whole tokens to a wave, whose stores fill no lines, 22.8);
+// 16384 tokens in 16 bits, blocks of 16, 32, 64 and 128, 17, 18, 20 and 48 us: a long run's loads, barrier and stores follow each other; 64 single tokens 4.8 us, the chain of slot, row, maximum and codes, and no more in a step that has room for 4096.
 #include "common.hpp"
 #include "lanes.hpp"
 #include "paged_device.hpp"
@@ -251,7 +251,7 @@ struct GatherArgs {
 
 // A workgroup takes 16 slots of one kv head, keys or values: a wave a slot at a time, a lane four dims, so that a store is a whole row.
 // Where the slots lie in two units at most (16 that follow each other do), the units come through LDS by whole kilobytes, for values are stored
-// four tokens to a dword; else a lane reads its bytes where they are.  32768 tokens, f16, 2 kv heads: 19.4 us, 5.2 TB/s of what is read and written.  (A
+// four tokens to a dword; else a lane reads its bytes where they are.  32768 tokens, f16, 2 kv heads: 19 to 20 us, 5.2 TB/s of what is read and written.  (A
 // lane's bytes straight from memory: 42 us.  Rows that keep a place in the caches on their way out: 29 where every call has other data, and who reads them
 // next takes as long either way.)
 constexpr uint32_t GATHER_SLOTS = 16;

@@ -11,7 +11,7 @@
 // found by bisection in the prefix sums in LDS).  The tokens' slots are independent of each other: a second launch of as
 // many workgroups as they fill, or, where few workgroups' worth of tokens come (a decode step), the first does them itself.
 // Measured: 32 requests with a token and three drafts each 2.9 us; 512 requests of up to 1900 tokens admitted at once (8200 blocks, 126 thousand
-// tokens) 7.9 us and 2.9 for the slots.
+// tokens) 8 us and 3 to 5 for the slots.
 #include "common.hpp"
 #include "lanes.hpp"
 #include "paged_device.hpp"

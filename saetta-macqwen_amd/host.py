@@ -771,7 +771,7 @@ class PagedTables(_Kept):
 class PagedAttention(_Kept):
     """Attention of a step's new tokens over paged caches: scratch and launches for tables of one size and up to `rows`
     new tokens a request (1: a token each; a verify step's rows; a chunk's tokens; any mixture).  The scratch is one
-    call's at a time: calls, or graphs of them, that may overlap want objects of their own."""
+    call's at a time: calls, or graphs of them, that may overlap want objects of their own (135 MB each where `rows` are a chunk's, over 2 kv heads)."""
 
     def __init__(self, heads, kv_heads, head_dim, tables, rows, device=None):
         if head_dim != DIM:
