@@ -687,8 +687,8 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 //   waves 0..3:  softmax(s)                | O(s) + S(s+1)
 //   waves 4..7:  O(s) + S(s+1)             | softmax(s+1)
 // Step s reads V(s) and K(s+1) as halves and makes V(s+1) and K(s+2), in the places of V(s-1) and K(s): one barrier a step.
-// Bound by the matrix cores and the clock that they leave (1.8 GHz): 4096 tokens at 28672, bf16, 16 q heads over 2 kv heads, 1.75 to 1.87 ms, 1.10 to 1.18 PFLOP/s (a
-// large product of the library: 1.20 to 1.28); the streams of products alone 1.45 ms; without the priority that keeps the two waves in opposite order 2.28.  A short item
+// Bound by the matrix cores and the clock that they leave (1.8 GHz): 4096 tokens at 28672, bf16, 16 q heads over 2 kv heads, 1.75 to 1.93 ms, 1.07 to 1.18 PFLOP/s (a
+// large product of the library on the same cards: 1.17 to 1.25); the streams of products alone 1.45 ms; without the priority that keeps the two waves in opposite order 2.28.  A short item
 // is bound by its start and end, 13 to 16 us: seven prompts of 147 to 1645 tokens 73 us, a tile of 32 tokens 20.
 constexpr uint32_t CODE_BYTES = STEP_KEYS * DIM, HALF_BYTES = 2 * CODE_BYTES;  // a step's keys, or values
 constexpr uint32_t AHEAD = 3, PLACES = 4;

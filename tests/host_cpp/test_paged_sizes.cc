@@ -1,5 +1,5 @@
 // What the paged objects of the C++ host mirror refuse of sizes that 32 bits do not hold: cut to them they would be another call's.
-// Exit code 0 = all passed.  Run by tests/test_gpu_paged_host_cpp_sizes.py on a GPU box.
+// Exit code 0 = all passed.  Run by tests/test_gpu_paged_host_cpp_sizes.py on a GPU.
 #include <cstdio>
 
 #include "../../saetta-macqwen_amd/host/saetta.hpp"
