@@ -11,7 +11,9 @@
 // registers.  A wave has four tokens of a unit, a lane four dims of each: a load is a token's row, and what a wave stores of four tokens fills lines of 64
 // bytes.  A run of up to four tokens is one wave's, so that a step's tokens and drafts are stored at once.  Measured, 2 kv heads: 9700 tokens of five
 // prompts, f32, blocks of 16, 13 us, 3.8 TB/s of what is read and written (a large copy: 4.9; with whole tokens to a wave, whose stores fill no lines, 22.8);
-// 16384 tokens in 16 bits, blocks of 16, 32, 64 and 128, 17, 18, 20 and 48 us: a long run's loads, barrier and stores follow each other; 64 single tokens 4.8 us, the chain of slot, row, maximum and codes, and no more in a step that has room for 4096.
+// 16384 tokens in 16 bits, blocks of 16, 32, 64 and 128, 17, 18, 20 and 48 us: a long run's loads, barrier and stores follow each other, and runs of 128 tokens
+// begin in every other workgroup, so that half of the XCDs have none; 100 prompts of 90 tokens 14, 24, 22 and 33 us, by what the workgroups with several runs take; 64 single
+// tokens 4.8 us, the chain of slot, row, maximum and codes, and no more in a step that has room for 4096.
 #include "common.hpp"
 #include "lanes.hpp"
 #include "paged_device.hpp"
