@@ -172,6 +172,7 @@ __global__ __launch_bounds__(SPLIT_THREADS) void paged_split_kernel(SplitArgs a)
     // alike.  Where one round holds all (as a rule) the tile is found once.
     bool found = false;
     Item mine;
+    mine.tokens = 0;  // (and remains so where no request has a new token)
     auto for_tiles = [&](auto f) {
         if (found) return f(mine);
         uint32_t most = a.most_items - a.target;  // as many tiles as there can be, whatever the starts say
